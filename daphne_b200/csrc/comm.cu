@@ -88,6 +88,9 @@ static int nccl_dtype(int dtype) {
     }
 }
 
+// combining and gathering go by the value type: the 16-bit and 8-bit floating-point types are not combined
+static bool combinable(int dtype) { return dtype != DB2_F16 && dtype != DB2_BF16 && dtype != DB2_F8E4M3; }
+
 // ---- one process, several devices (group.cu) ----
 
 // One communicator per context of a device group (ncclCommInitAll); the devices must be distinct.
@@ -121,6 +124,8 @@ void nccl_destroy_group(const std::vector<db2_context *> &ctxs) {
 int nccl_allreduce_group(const std::vector<db2_context *> &ctxs, const std::vector<db2_matrix *> &ms, int combine) {
     Nccl *n = nccl();
     DB2_CHECK(n, DB2_ENCCL, "NCCL library (libnccl.so.2) could not be loaded");
+    for (const db2_matrix *m : ms)
+        DB2_CHECK(combinable(m->dtype), DB2_EUNSUPPORTED, "all-reduce: value type %d is not combined", m->dtype);
     const int op = combine == DB2_COMBINE_ADD ? ncclSum : (combine == DB2_COMBINE_MIN ? ncclMin : ncclMax);
     DB2_NCCL(n->GroupStart());
     int rc = ncclSuccess;
@@ -282,6 +287,7 @@ int db2_allreduce(db2_context *ctx, db2_matrix *m, int combine) {
         return DB2_OK;
     }
     DB2_CHECK(ctx->comm, DB2_ENCCL, "no communicator: call db2_comm_init first");
+    DB2_CHECK(combinable(m->dtype), DB2_EUNSUPPORTED, "all-reduce: value type %d is not combined", m->dtype);
     bind_device(ctx);
     DB2_TRY(ensure_device(m));
     DB2_CHECK(m->dev_ld == m->cols || m->rows == 1, DB2_EUNSUPPORTED, "all-reduce of a strided view");
@@ -316,6 +322,7 @@ int db2_allreduce_async(db2_context *ctx, db2_matrix *m, int combine) {
     if (m->combined || g_override) // nothing to do / the test table of stand-ins: the plain path
         return db2_allreduce(ctx, m, combine);
     DB2_CHECK(ctx->comm, DB2_ENCCL, "no communicator: call db2_comm_init first");
+    DB2_CHECK(combinable(m->dtype), DB2_EUNSUPPORTED, "all-reduce: value type %d is not combined", m->dtype);
     bind_device(ctx);
     DB2_TRY(ensure_device(m));
     DB2_CHECK(m->dev_ld == m->cols || m->rows == 1, DB2_EUNSUPPORTED, "all-reduce of a strided view");
@@ -357,6 +364,8 @@ int db2_allgatherv_rows(db2_context *ctx, db2_matrix *local, int64_t total_rows,
     bind_device(ctx);
     DB2_TRY(ensure_device(local));
     DB2_CHECK(local->dev_ld == local->cols || local->rows <= 1, DB2_EUNSUPPORTED, "all-gather of a strided view");
+    DB2_CHECK(combinable(local->dtype) || ctx->world == 1, DB2_EUNSUPPORTED, "all-gather: value type %d is not combined",
+              local->dtype);
     DB2_TRY(prepare_result(ctx, full, local->dtype, total_rows, local->cols));
     db2_matrix *f = *full;
     const size_t es = local->esize(), n = (size_t)local->rows * local->cols;

@@ -75,7 +75,16 @@ struct PerDeviceOnce {
 };
 
 inline size_t dtype_size(int dtype) {
-    return dtype == DB2_U8 ? 1 : ((dtype == DB2_F32 || dtype == DB2_I32 || dtype == DB2_U32) ? 4 : 8);
+    switch (dtype) {
+    case DB2_U8:
+    case DB2_F8E4M3: return 1;
+    case DB2_F16:
+    case DB2_BF16: return 2;
+    case DB2_F32:
+    case DB2_I32:
+    case DB2_U32: return 4;
+    default: return 8;
+    }
 }
 
 inline cudaStream_t as_stream(void *s) { return reinterpret_cast<cudaStream_t>(s); }

@@ -1,0 +1,812 @@
+// Embedding: rows of a table picked by token and scaled, and the gradient of the table.
+//
+//   res[i]  = scale * table[token[i]]                               (token -1: a row of zeros)
+//   dtable[v] = scale * sum over i with token[i] == v of grad[i]    (in the order of i)
+//
+// It is the product of the one-hot matrix of the tokens with the table, P @ E and t(P) @ dY, without P.
+//
+// The gradient sorts the tokens (stably, by key and position), so that equal tokens lie side by side and every sum has
+// one fixed order of additions: no floating-point atomics, the same bits in every run.
+#include "runtime.h"
+#include "seq.cuh"
+
+namespace db2 {
+
+namespace {
+
+constexpr int EMB_THREADS = 256;
+constexpr int EMB_UNROLL = 4; // packets of a row in flight per thread
+
+// tokens are int64 or int32
+template <typename I> __device__ __forceinline__ int64_t token_at(const void *tokens, int64_t ld, int64_t i) {
+    return (int64_t) static_cast<const I *>(tokens)[i * ld];
+}
+
+// Rows are copied by `1 << log_tpr` threads each; a CTA holds EMB_THREADS >> log_tpr rows, blockIdx.y cuts long rows.
+// Bound by memory: one read and one write per element.
+template <typename T, int N, typename I>
+__global__ void __launch_bounds__(EMB_THREADS)
+    embed_kernel(const T *__restrict__ table, int64_t vocab, int64_t cols, int64_t table_ld, const void *tokens,
+                 int64_t tokens_ld, int64_t n, wide_t<T> scale, T *__restrict__ res, int64_t res_ld, int log_tpr,
+                 int32_t *status) {
+    const int tpr = 1 << log_tpr, tx = threadIdx.x & (tpr - 1), ty = threadIdx.x >> log_tpr;
+    const int rows_per_cta = EMB_THREADS >> log_tpr;
+    const int64_t packets = cols / N;
+    for (int64_t r = (int64_t)blockIdx.x * rows_per_cta + ty; r < n; r += (int64_t)gridDim.x * rows_per_cta) {
+        const int64_t t = token_at<I>(tokens, tokens_ld, r);
+        const bool ok = t >= 0 && t < vocab;
+        if (!ok && t != -1 && status && tx == 0 && blockIdx.y == 0)
+            *status = 1;
+        const T *src = table + (ok ? t : 0) * table_ld;
+        T *dst = res + r * res_ld;
+        for (int64_t p0 = (int64_t)blockIdx.y * tpr * EMB_UNROLL + tx; p0 < packets;
+             p0 += (int64_t)gridDim.y * tpr * EMB_UNROLL) {
+            Vec<T, N> x[EMB_UNROLL];
+#pragma unroll
+            for (int u = 0; u < EMB_UNROLL; u++)
+                if (ok && p0 + u * tpr < packets)
+                    x[u] = ld_vec<T, N>(src + (p0 + u * tpr) * N);
+#pragma unroll
+            for (int u = 0; u < EMB_UNROLL; u++)
+                if (p0 + u * tpr < packets) {
+                    Vec<T, N> y;
+#pragma unroll
+                    for (int k = 0; k < N; k++)
+                        y.v[k] = narrow<T>(ok ? widen(x[u].v[k]) * scale : wide_t<T>(0));
+                    st_vec<T, N>(dst + (p0 + u * tpr) * N, y);
+                }
+        }
+        if (N > 1 && blockIdx.y == 0)
+            for (int64_t c = packets * N + tx; c < cols; c += tpr)
+                dst[c] = narrow<T>(ok ? widen(src[c]) * scale : wide_t<T>(0));
+    }
+}
+
+int log2_ceil(int64_t x) {
+    int b = 0;
+    while (((int64_t)1 << b) < x)
+        b++;
+    return b;
+}
+
+template <typename T, int N, typename I>
+int embed_launch(const void *table, int64_t vocab, int64_t cols, int64_t table_ld, const void *tokens,
+                 int64_t tokens_ld, int64_t n, double scale, void *res, int64_t res_ld, int32_t *status,
+                 cudaStream_t st) {
+    // a thread takes up to EMB_UNROLL packets of a row in one go
+    const int64_t packets = cols / N;
+    int log_tpr = log2_ceil((packets + EMB_UNROLL - 1) / EMB_UNROLL);
+    if (log_tpr > 8)
+        log_tpr = 8;
+    const int64_t row_groups = (n + (EMB_THREADS >> log_tpr) - 1) / (EMB_THREADS >> log_tpr);
+    const int64_t span = ((int64_t)1 << log_tpr) * EMB_UNROLL;
+    int64_t gy = (packets + span - 1) / span;
+    const int64_t cap = (int64_t)sm_count() * 16;
+    gy = gy < 1 ? 1 : (gy > 64 ? 64 : gy);
+    const int64_t gx = row_groups < cap ? row_groups : cap;
+    embed_kernel<T, N, I><<<dim3((unsigned)gx, (unsigned)gy), EMB_THREADS, 0, st>>>(
+        static_cast<const T *>(table), vocab, cols, table_ld, tokens, tokens_ld, n, (wide_t<T>)scale,
+        static_cast<T *>(res), res_ld, log_tpr, status);
+    return after_launch("embed_kernel");
+}
+
+// ---- sorting the tokens ----
+//
+// Every sort delivers key[] (ascending) and pos[] (ascending among equal keys).  A token that names no row gets the key
+// `vocab`, behind all others.
+
+constexpr int RANK_MAX = 16384; // tokens that are sorted by counting (their keys fill 64 KB of shared memory)
+constexpr int RANK_THREADS = 512;
+constexpr int RANK_SHARE = 8;                            // threads that count for one token
+constexpr int RANK_TILE = RANK_THREADS / RANK_SHARE * 2; // tokens of a CTA: two per thread, which share the loads
+
+template <typename I>
+__device__ __forceinline__ uint32_t token_key(const void *tokens, int64_t ld, int64_t i, int64_t vocab,
+                                              int32_t *status) {
+    const int64_t t = token_at<I>(tokens, ld, i);
+    if (t >= 0 && t < vocab)
+        return (uint32_t)t;
+    if (t != -1 && status)
+        *status = 1;
+    return (uint32_t)vocab;
+}
+
+// Place of token i in sorted order = how many tokens have a smaller key, or the same key and a smaller position.  All
+// keys lie in shared memory; RANK_SHARE threads count for a token, each over every RANK_SHARE-th packet of four keys.
+// n^2 comparisons in one launch without any exchange between CTAs: fewer microseconds than the launches of a radix sort
+// as long as the keys of all tokens fit (measured in the comment at embed_sort).
+template <typename I>
+__global__ void __launch_bounds__(RANK_THREADS)
+    token_rank_kernel(const void *tokens, int64_t tokens_ld, int n, int64_t vocab, uint32_t *__restrict__ key,
+                      uint32_t *__restrict__ pos, int32_t *status) {
+    extern __shared__ uint4 rank_smem[];
+    uint32_t *k = reinterpret_cast<uint32_t *>(rank_smem);
+    const int padded = (n + 3) / 4 * 4;
+    for (int i = threadIdx.x; i < padded; i += RANK_THREADS)
+        k[i] = i < n ? token_key<I>(tokens, tokens_ld, i, vocab, blockIdx.x == 0 ? status : nullptr) : 0xffffffffu;
+    __syncthreads();
+    const int part = threadIdx.x % RANK_SHARE, i0 = blockIdx.x * RANK_TILE + threadIdx.x / RANK_SHARE * 2;
+    const unsigned stay = __ballot_sync(0xffffffffu, i0 < n); // the threads of a token stay or leave together
+    if (i0 >= n)
+        return;
+    const uint32_t ka = k[i0], kb = i0 + 1 < n ? k[i0 + 1] : 0xffffffffu;
+    int ca = 0, cb = 0;
+    // tokens in packets before the own one also count when their key is the same, those behind only when it is smaller
+    // (the largest key is below 2^32 - 1, so key + 1 does not wrap)
+    const int own = i0 / 4;
+    for (int q = part; q < own; q += RANK_SHARE) {
+        const uint4 x = rank_smem[q];
+        ca += (x.x <= ka) + (x.y <= ka) + (x.z <= ka) + (x.w <= ka);
+        cb += (x.x <= kb) + (x.y <= kb) + (x.z <= kb) + (x.w <= kb);
+    }
+    for (int q = own + 1 + part; q < padded / 4; q += RANK_SHARE) {
+        const uint4 x = rank_smem[q];
+        ca += (x.x < ka) + (x.y < ka) + (x.z < ka) + (x.w < ka);
+        cb += (x.x < kb) + (x.y < kb) + (x.z < kb) + (x.w < kb);
+    }
+    if (part == 0)
+        for (int j = own * 4; j < own * 4 + 4; j++) {
+            ca += k[j] < ka || (k[j] == ka && j < i0);
+            cb += k[j] < kb || (k[j] == kb && j < i0 + 1);
+        }
+#pragma unroll
+    for (int o = RANK_SHARE / 2; o >= 1; o >>= 1) {
+        ca += __shfl_xor_sync(stay, ca, o);
+        cb += __shfl_xor_sync(stay, cb, o);
+    }
+    if (part == 0) {
+        key[ca] = ka;
+        pos[ca] = (uint32_t)i0;
+        if (i0 + 1 < n) {
+            key[cb] = kb;
+            pos[cb] = (uint32_t)(i0 + 1);
+        }
+    }
+}
+
+// Radix sort, lowest digit first, up to 9 bits a pass: tiles of RADIX_TILE tokens are counted by digit, the counts of all
+// tiles are scanned (digit by digit, tile by tile), and every tile moves its tokens to their places in order.
+constexpr int RADIX_THREADS = 256, RADIX_WARPS = RADIX_THREADS / 32;
+constexpr int RADIX_PER_WARP = 512;
+constexpr int RADIX_TILE = RADIX_WARPS * RADIX_PER_WARP;
+constexpr int RADIX_BITS = 9, RADIX_BINS = 1 << RADIX_BITS;
+
+struct RadixIn { // the tokens themselves in the first pass (key == nullptr), keys and positions later
+    const void *tokens;
+    int64_t tokens_ld, vocab;
+    const uint32_t *key, *pos;
+};
+template <typename I>
+__device__ __forceinline__ void radix_load(const RadixIn &in, int64_t i, uint32_t *key, uint32_t *pos,
+                                           int32_t *status) {
+    if (in.key) {
+        *key = in.key[i];
+        *pos = in.pos[i];
+    } else {
+        *key = token_key<I>(in.tokens, in.tokens_ld, i, in.vocab, status);
+        *pos = (uint32_t)i;
+    }
+}
+
+template <typename I>
+__global__ void __launch_bounds__(RADIX_THREADS)
+    radix_count_kernel(RadixIn in, int64_t n, int shift, int bins, uint32_t *__restrict__ counts, int32_t *status) {
+    __shared__ uint32_t h[RADIX_BINS];
+    for (int b = threadIdx.x; b < bins; b += RADIX_THREADS)
+        h[b] = 0;
+    __syncthreads();
+    const int64_t base = (int64_t)blockIdx.x * RADIX_TILE;
+    for (int i = threadIdx.x; i < RADIX_TILE && base + i < n; i += RADIX_THREADS) {
+        uint32_t key, pos;
+        radix_load<I>(in, base + i, &key, &pos, status);
+        atomicAdd(&h[(key >> shift) & (bins - 1)], 1u); // integer counts: the order of additions does not show
+    }
+    __syncthreads();
+    for (int b = threadIdx.x; b < bins; b += RADIX_THREADS)
+        counts[(int64_t)b * gridDim.x + blockIdx.x] = h[b];
+}
+
+// exclusive prefix over all counts, in place, by one CTA
+__global__ void __launch_bounds__(1024) radix_scan_kernel(uint32_t *__restrict__ counts, int64_t m) {
+    __shared__ uint32_t warp_sum[32];
+    const int t = threadIdx.x, lane = t % 32, warp = t / 32;
+    uint32_t carry = 0;
+    for (int64_t b = 0; b < m; b += 4096) {
+        uint32_t v[4], sum = 0;
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const int64_t i = b + t * 4 + k;
+            v[k] = i < m ? counts[i] : 0u;
+            sum += v[k];
+        }
+        uint32_t inc = sum;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint32_t y = __shfl_up_sync(0xffffffffu, inc, o);
+            if (lane >= o)
+                inc += y;
+        }
+        if (lane == 31)
+            warp_sum[warp] = inc;
+        __syncthreads();
+        uint32_t before = 0, all = 0;
+        for (int w = 0; w < 32; w++) {
+            before += w < warp ? warp_sum[w] : 0u;
+            all += warp_sum[w];
+        }
+        uint32_t run = carry + before + inc - sum;
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const int64_t i = b + t * 4 + k;
+            if (i < m)
+                counts[i] = run;
+            run += v[k];
+        }
+        carry += all;
+        __syncthreads();
+    }
+}
+
+// A warp owns RADIX_PER_WARP consecutive tokens of the tile and walks them 32 at a time; next[w][d] is the place of warp
+// w's next token with digit d.  Lanes with the same digit take consecutive places in lane order.
+template <typename I>
+__global__ void __launch_bounds__(RADIX_THREADS)
+    radix_move_kernel(RadixIn in, int64_t n, int shift, int bins, const uint32_t *__restrict__ offsets,
+                      uint32_t *__restrict__ key_out, uint32_t *__restrict__ pos_out) {
+    __shared__ uint32_t next[RADIX_WARPS][RADIX_BINS];
+    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+    for (int b = threadIdx.x; b < RADIX_WARPS * RADIX_BINS; b += RADIX_THREADS)
+        (&next[0][0])[b] = 0;
+    __syncthreads();
+    const int64_t base = (int64_t)blockIdx.x * RADIX_TILE + warp * RADIX_PER_WARP;
+    for (int i = lane; i < RADIX_PER_WARP && base + i < n; i += 32) {
+        uint32_t key, pos;
+        radix_load<I>(in, base + i, &key, &pos, nullptr);
+        atomicAdd(&next[warp][(key >> shift) & (bins - 1)], 1u);
+    }
+    __syncthreads();
+    for (int b = threadIdx.x; b < bins; b += RADIX_THREADS) {
+        uint32_t run = offsets[(int64_t)b * gridDim.x + blockIdx.x];
+        for (int w = 0; w < RADIX_WARPS; w++) {
+            const uint32_t c = next[w][b];
+            next[w][b] = run;
+            run += c;
+        }
+    }
+    __syncthreads();
+    for (int i = 0; i < RADIX_PER_WARP; i += 32) { // the same trips for all lanes
+        const bool in_range = base + i + lane < n;
+        uint32_t key = 0, pos = 0;
+        if (in_range)
+            radix_load<I>(in, base + i + lane, &key, &pos, nullptr);
+        const uint32_t d = in_range ? (key >> shift) & (bins - 1) : (uint32_t)RADIX_BINS;
+        const unsigned peers = __match_any_sync(0xffffffffu, d);
+        const int before = __popc(peers & ((1u << lane) - 1u));
+        uint32_t place = 0;
+        if (in_range)
+            place = next[warp][d] + before;
+        __syncwarp();
+        if (in_range && before == 0)
+            next[warp][d] += __popc(peers);
+        __syncwarp();
+        if (in_range) {
+            key_out[place] = key;
+            pos_out[place] = pos;
+        }
+    }
+}
+
+// ---- sums over equal tokens ----
+
+constexpr int SUM_THREADS = 128;
+constexpr int SUM_RUN = 32;   // sorted tokens that one group of threads adds up
+constexpr int SUM_AHEAD = 4;  // gradient rows in flight per thread
+constexpr int FILL_ROWS = 32; // table rows per CTA that are looked at for being untouched
+
+struct SumArgs {
+    const uint32_t *key, *pos;
+    int64_t n, cols, vocab, grad_ld, res_ld, part_ld;
+    int64_t runs;     // ceil(n / SUM_RUN)
+    unsigned fill_x;  // CTAs (in x) that write zeros
+    int log_tpr;
+};
+
+// A run of SUM_RUN sorted tokens x a block of columns: rows of equal tokens are added in registers (32 bits or more);
+// where the token changes, the sum is finished -- written to the table when all its rows lie in the run, to `part`
+// otherwise: part[run][0] holds the sum of a token that came over from the run before, part[run][1] that of a token that
+// starts in the run and goes on behind it.  Equal amounts of work whatever the tokens' frequencies.
+// The CTAs in front write zeros to the table's untouched rows (not when adding to the table).
+// Bound by memory: every gradient row is read once, every table row written once.
+template <typename T, typename R, int N, bool ADD>
+__global__ void __launch_bounds__(SUM_THREADS)
+    embed_sum_kernel(SumArgs a, const T *__restrict__ grad, wide_t<T> scale, R *__restrict__ res,
+                     wide_t<T> *__restrict__ part) {
+    using W = wide_t<T>;
+    if (blockIdx.x < a.fill_x) {
+        __shared__ uint32_t hit;
+        const int64_t v0 = (int64_t)blockIdx.x * FILL_ROWS;
+        if (threadIdx.x == 0)
+            hit = 0;
+        __syncthreads();
+        // first sorted token >= v0
+        int64_t lo = 0, hi = a.n;
+        while (lo < hi) {
+            const int64_t mid = (lo + hi) / 2;
+            if ((int64_t)a.key[mid] < v0)
+                lo = mid + 1;
+            else
+                hi = mid;
+        }
+        // the tokens of the block: mark them
+        for (int64_t i = lo + threadIdx.x; i < a.n; i += SUM_THREADS) {
+            const int64_t v = (int64_t)a.key[i] - v0;
+            if (v >= FILL_ROWS)
+                break;
+            if (i == lo || a.key[i] != a.key[i - 1])
+                atomicOr(&hit, 1u << v);
+        }
+        __syncthreads();
+        const uint32_t mask = hit;
+        const int64_t packets = a.cols / N;
+        for (int j = 0; j < FILL_ROWS && v0 + j < a.vocab; j++) {
+            if (mask >> j & 1u)
+                continue;
+            R *dst = res + (v0 + j) * a.res_ld;
+            Vec<R, N> z;
+#pragma unroll
+            for (int k = 0; k < N; k++)
+                z.v[k] = narrow<R>(W(0));
+            for (int64_t p = (int64_t)blockIdx.y * SUM_THREADS + threadIdx.x; p < packets;
+                 p += (int64_t)gridDim.y * SUM_THREADS)
+                st_vec<R, N>(dst + p * N, z);
+            if (N > 1 && blockIdx.y == 0)
+                for (int64_t c = packets * N + threadIdx.x; c < a.cols; c += SUM_THREADS)
+                    dst[c] = narrow<R>(W(0));
+        }
+        return;
+    }
+    const int tpr = 1 << a.log_tpr, tx = threadIdx.x & (tpr - 1), ty = threadIdx.x >> a.log_tpr;
+    const int64_t run = (int64_t)(blockIdx.x - a.fill_x) * (SUM_THREADS >> a.log_tpr) + ty;
+    if (run >= a.runs)
+        return;
+    const int64_t b = run * SUM_RUN, e = b + SUM_RUN < a.n ? b + SUM_RUN : a.n;
+    const uint32_t vocab = (uint32_t)a.vocab;
+    const uint32_t before = b > 0 ? a.key[b - 1] : 0xffffffffu, behind = e < a.n ? a.key[e] : 0xffffffffu;
+    // packets of N columns; the columns behind the last whole packet are a packet of their own with single accesses
+    const int64_t packets = (a.cols + N - 1) / N;
+    for (int64_t p = (int64_t)blockIdx.y * tpr + tx; p < packets; p += (int64_t)gridDim.y * tpr) {
+        const int64_t c = p * N;
+        const int width = a.cols - c < N ? (int)(a.cols - c) : N;
+        W acc[N];
+#pragma unroll
+        for (int k = 0; k < N; k++)
+            acc[k] = W(0);
+        uint32_t cur = a.key[b];
+        int slot = cur == before ? 0 : -1; // -1: the sum starts in this run
+        auto finish = [&](uint32_t next) {
+            if (cur >= vocab)
+                return;
+            if (slot < 0 && next != cur) {
+                R *dst = res + (int64_t)cur * a.res_ld + c;
+                if (width == N) {
+                    Vec<R, N> y;
+                    if constexpr (ADD)
+                        y = ld_vec<R, N>(dst);
+#pragma unroll
+                    for (int k = 0; k < N; k++)
+                        y.v[k] = narrow<R>(ADD ? W(widen(y.v[k])) + acc[k] * scale : acc[k] * scale);
+                    st_vec<R, N>(dst, y);
+                } else {
+                    for (int k = 0; k < N; k++)
+                        if (k < width)
+                            dst[k] = narrow<R>(ADD ? W(widen(dst[k])) + acc[k] * scale : acc[k] * scale);
+                }
+            } else {
+                W *dst = part + (run * 2 + (slot < 0 ? 1 : 0)) * a.part_ld + c;
+#pragma unroll
+                for (int k = 0; k < N; k++)
+                    if (k < width)
+                        dst[k] = acc[k];
+            }
+        };
+        for (int64_t i = b; i < e; i += SUM_AHEAD) {
+            Vec<T, N> x[SUM_AHEAD];
+            uint32_t kk[SUM_AHEAD];
+#pragma unroll
+            for (int u = 0; u < SUM_AHEAD; u++) {
+                kk[u] = i + u < e ? a.key[i + u] : 0xffffffffu;
+                if (kk[u] < vocab) {
+                    const T *src = grad + (int64_t)a.pos[i + u] * a.grad_ld + c;
+                    if (width == N)
+                        x[u] = ld_vec<T, N>(src);
+                    else
+                        for (int k = 0; k < N; k++)
+                            if (k < width)
+                                x[u].v[k] = src[k];
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < SUM_AHEAD; u++) {
+                if (i + u >= e)
+                    break;
+                if (kk[u] != cur) {
+                    finish(kk[u]);
+                    cur = kk[u];
+                    slot = -1;
+#pragma unroll
+                    for (int k = 0; k < N; k++)
+                        acc[k] = W(0);
+                }
+                if (cur < vocab) {
+#pragma unroll
+                    for (int k = 0; k < N; k++)
+                        if (k < width)
+                            acc[k] += widen(x[u].v[k]);
+                }
+            }
+        }
+        finish(behind);
+    }
+}
+
+// Tokens whose rows span several runs: the run in which such a token starts adds the partial sums behind it, in order.
+// JOIN_Y groups of threads take equal shares of the runs, their sums are added in the order of the shares.
+constexpr int JOIN_X = 32, JOIN_Y = 8;
+template <typename T, typename R, bool ADD>
+__global__ void __launch_bounds__(JOIN_X *JOIN_Y)
+    embed_join_kernel(SumArgs a, wide_t<T> scale, R *__restrict__ res, const wide_t<T> *__restrict__ part) {
+    using W = wide_t<T>;
+    __shared__ W sums[JOIN_Y][JOIN_X];
+    const int tx = threadIdx.x % JOIN_X, ty = threadIdx.x / JOIN_X;
+    for (int64_t run = blockIdx.x; run + 1 < a.runs; run += gridDim.x) {
+        const int64_t b = run * SUM_RUN, e = b + SUM_RUN; // e < n: the run is not the last
+        const uint32_t v = a.key[e - 1];
+        if (v >= (uint32_t)a.vocab || a.key[e] != v || (b > 0 && a.key[b] == v && a.key[b - 1] == v))
+            continue; // uniform over the CTA: the last token ends here, or started in an earlier run
+        // one past the last row with this token
+        int64_t lo = e + 1, hi = a.n;
+        while (lo < hi) {
+            const int64_t mid = (lo + hi) / 2;
+            if (a.key[mid] == v)
+                lo = mid + 1;
+            else
+                hi = mid;
+        }
+        const int64_t more = (lo - 1) / SUM_RUN - run; // runs behind this one that hold a part
+        const int64_t share = (more + JOIN_Y) / JOIN_Y;
+        const int64_t first = ty * share, last = first + share < more + 1 ? first + share : more + 1;
+        for (int64_t c0 = (int64_t)blockIdx.y * JOIN_X; c0 < a.cols; c0 += (int64_t)gridDim.y * JOIN_X) {
+            const int64_t c = c0 + tx;
+            W acc = W(0);
+            if (c < a.cols) {
+#pragma unroll 8
+                for (int64_t j = first; j < last; j++)
+                    acc += part[((run + j) * 2 + (j == 0 ? 1 : 0)) * a.part_ld + c];
+            }
+            __syncthreads();
+            sums[ty][tx] = acc;
+            __syncthreads();
+            if (ty == 0 && c < a.cols) {
+                W s = sums[0][tx];
+                for (int k = 1; k < JOIN_Y; k++)
+                    s += sums[k][tx];
+                R *dst = res + (int64_t)v * a.res_ld + c;
+                *dst = narrow<R>(ADD ? W(widen(*dst)) + s * scale : s * scale);
+            }
+        }
+    }
+}
+
+struct GradPlan {
+    int64_t runs, part_ld, tiles;
+    int bits, passes;
+    size_t key_off[2], pos_off[2], counts_off, part_off, bytes;
+};
+size_t take(size_t *at, size_t bytes) {
+    const size_t here = *at;
+    *at += (bytes + 255) / 256 * 256;
+    return here;
+}
+GradPlan grad_plan(size_t wide_size, int64_t vocab, int64_t cols, int64_t n) {
+    GradPlan p{};
+    p.runs = (n + SUM_RUN - 1) / SUM_RUN;
+    p.part_ld = (cols + 7) / 8 * 8;
+    p.bits = log2_ceil(vocab + 1);
+    p.passes = n <= RANK_MAX ? 0 : (p.bits + RADIX_BITS - 1) / RADIX_BITS;
+    p.tiles = (n + RADIX_TILE - 1) / RADIX_TILE;
+    size_t at = 0;
+    for (int i = 0; i < (p.passes > 1 ? 2 : 1); i++) {
+        p.key_off[i] = take(&at, (size_t)n * 4);
+        p.pos_off[i] = take(&at, (size_t)n * 4);
+    }
+    if (p.passes)
+        p.counts_off = take(&at, (size_t)p.tiles * RADIX_BINS * 4);
+    p.part_off = take(&at, (size_t)p.runs * 2 * p.part_ld * wide_size);
+    p.bytes = at;
+    return p;
+}
+
+template <typename I>
+int embed_sort(const GradPlan &p, const void *tokens, int64_t tokens_ld, int64_t n, int64_t vocab, char *scratch,
+               const uint32_t **key, const uint32_t **pos, int32_t *status, cudaStream_t st) {
+    uint32_t *k[2], *q[2];
+    for (int i = 0; i < 2; i++) {
+        k[i] = reinterpret_cast<uint32_t *>(scratch + p.key_off[i]);
+        q[i] = reinterpret_cast<uint32_t *>(scratch + p.pos_off[i]);
+    }
+    if (p.passes == 0) {
+        static PerDeviceOnce once;
+        if (once.need()) {
+            DB2_CUDA(cudaFuncSetAttribute(token_rank_kernel<I>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                          RANK_MAX * 4));
+            once.mark();
+        }
+        const int grid = (int)((n + RANK_TILE - 1) / RANK_TILE);
+        token_rank_kernel<I><<<grid, RANK_THREADS, (size_t)(n + 3) / 4 * 16, st>>>(tokens, tokens_ld, (int)n, vocab,
+                                                                                  k[0], q[0], status);
+        DB2_TRY(after_launch("token_rank_kernel"));
+        *key = k[0];
+        *pos = q[0];
+        return DB2_OK;
+    }
+    uint32_t *counts = reinterpret_cast<uint32_t *>(scratch + p.counts_off);
+    RadixIn in{tokens, tokens_ld, vocab, nullptr, nullptr};
+    int shift = 0;
+    for (int pass = 0; pass < p.passes; pass++) {
+        const int bits = (p.bits - shift + p.passes - pass - 1) / (p.passes - pass), bins = 1 << bits;
+        const int to = pass % 2;
+        radix_count_kernel<I><<<(unsigned)p.tiles, RADIX_THREADS, 0, st>>>(in, n, shift, bins, counts, status);
+        DB2_TRY(after_launch("radix_count_kernel"));
+        radix_scan_kernel<<<1, 1024, 0, st>>>(counts, p.tiles * bins);
+        DB2_TRY(after_launch("radix_scan_kernel"));
+        radix_move_kernel<I><<<(unsigned)p.tiles, RADIX_THREADS, 0, st>>>(in, n, shift, bins, counts, k[to], q[to]);
+        DB2_TRY(after_launch("radix_move_kernel"));
+        in.key = k[to];
+        in.pos = q[to];
+        shift += bits;
+    }
+    *key = in.key;
+    *pos = in.pos;
+    return DB2_OK;
+}
+
+template <typename T, typename R, int N, bool ADD>
+int embed_sum(SumArgs a, const void *grad, double scale, void *res, void *part, cudaStream_t st) {
+    const int64_t packets = (a.cols + N - 1) / N;
+    a.log_tpr = log2_ceil(packets);
+    if (a.log_tpr > 7)
+        a.log_tpr = 7;
+    const int64_t groups = SUM_THREADS >> a.log_tpr;
+    const int64_t gx = (a.runs + groups - 1) / groups;
+    int64_t gy = (packets + (1 << a.log_tpr) - 1) >> a.log_tpr;
+    gy = gy > 1024 ? 1024 : gy;
+    a.fill_x = ADD ? 0u : (unsigned)((a.vocab + FILL_ROWS - 1) / FILL_ROWS);
+    embed_sum_kernel<T, R, N, ADD><<<dim3((unsigned)(gx + a.fill_x), (unsigned)gy), SUM_THREADS, 0, st>>>(
+        a, static_cast<const T *>(grad), (wide_t<T>)scale, static_cast<R *>(res), static_cast<wide_t<T> *>(part));
+    DB2_TRY(after_launch("embed_sum_kernel"));
+    if (a.runs > 1) {
+        int64_t jy = (a.cols + JOIN_X - 1) / JOIN_X;
+        jy = jy > 128 ? 128 : jy;
+        int64_t jx = a.runs - 1;
+        jx = jx > 4096 ? 4096 : jx;
+        embed_join_kernel<T, R, ADD><<<dim3((unsigned)jx, (unsigned)jy), JOIN_X * JOIN_Y, 0, st>>>(
+            a, (wide_t<T>)scale, static_cast<R *>(res), static_cast<const wide_t<T> *>(part));
+        DB2_TRY(after_launch("embed_join_kernel"));
+    }
+    return DB2_OK;
+}
+
+template <typename T, typename R>
+int embed_sum_any(const SumArgs &a, const void *grad, double scale, void *res, void *part, int accumulate,
+                  cudaStream_t st) {
+    constexpr int N = 16 / (sizeof(T) > sizeof(R) ? sizeof(T) : sizeof(R)); // both sides' packets are at most 16 bytes
+    const bool wide = rows_aligned(grad, a.grad_ld, sizeof(T), N * sizeof(T)) &&
+                      rows_aligned(res, a.res_ld, sizeof(R), N * sizeof(R));
+    if (wide)
+        return accumulate ? embed_sum<T, R, N, true>(a, grad, scale, res, part, st)
+                          : embed_sum<T, R, N, false>(a, grad, scale, res, part, st);
+    return accumulate ? embed_sum<T, R, 1, true>(a, grad, scale, res, part, st)
+                      : embed_sum<T, R, 1, false>(a, grad, scale, res, part, st);
+}
+
+bool seq_type(int dtype) {
+    return dtype == DB2_F64 || dtype == DB2_F32 || dtype == DB2_F16 || dtype == DB2_BF16;
+}
+
+void count(db2_context *ctx, uint64_t before) {
+    std::lock_guard<std::mutex> lock(ctx->mu);
+    ctx->stats.launches += g_launches.load(std::memory_order_relaxed) - before;
+}
+
+// the status word of the token checks: its place among the context's words, cleared before the launch and read after it
+constexpr int EMB_STATUS = 40;
+int clear_status(db2_context *ctx) {
+    DB2_CUDA(cudaMemsetAsync(ctx->dev_status + EMB_STATUS, 0, sizeof(int32_t), ctx->stream));
+    return DB2_OK;
+}
+int check_status(db2_context *ctx, const char *what, int64_t vocab) {
+    DB2_CUDA(cudaMemcpyAsync(ctx->host_status + EMB_STATUS, ctx->dev_status + EMB_STATUS, sizeof(int32_t),
+                             cudaMemcpyDeviceToHost, ctx->stream));
+    DB2_CUDA(cudaStreamSynchronize(ctx->stream));
+    DB2_CHECK(ctx->host_status[EMB_STATUS] == 0, DB2_EDOMAIN,
+              "%s: a token lies outside the %lld rows of the table (-1 marks padding)", what, (long long)vocab);
+    return DB2_OK;
+}
+
+} // namespace
+
+int prepare_update(db2_matrix *m) {
+    DB2_TRY(ensure_device(m));
+    if (!m->is_view && m->dev.use_count() > 1) {
+        // other handles read the buffer: the update goes to a copy
+        auto fresh = make_devbuf(m->ctx, (size_t)m->rows * m->cols * m->esize());
+        if (m->rows * m->cols > 0)
+            DB2_CUDA(cudaMemcpy2DAsync(fresh->ptr, (size_t)m->cols * m->esize(), m->dev_ptr(),
+                                       (size_t)m->dev_ld * m->esize(), (size_t)m->cols * m->esize(), (size_t)m->rows,
+                                       cudaMemcpyDeviceToDevice, m->ctx->stream));
+        m->dev = fresh;
+        m->dev_off = 0;
+        m->dev_ld = m->cols;
+    } else if (m->dev) {
+        m->dev->version++;
+    }
+    m->is_seq = false;
+    m->combined = false;
+    m->host_valid = false;
+    return DB2_OK;
+}
+
+} // namespace db2
+
+using namespace db2;
+
+extern "C" {
+
+int db2k_embed(int dtype, const void *table, int64_t vocab, int64_t cols, int64_t table_ld, int index_dtype,
+               const void *tokens, int64_t tokens_ld, int64_t n, double scale, void *res, int64_t res_ld,
+               int32_t *dev_status, void *stream) {
+    DB2_CHECK(seq_type(dtype), DB2_EUNSUPPORTED, "embed: unsupported value type code %d", dtype);
+    DB2_CHECK(index_dtype == DB2_I64 || index_dtype == DB2_I32, DB2_EUNSUPPORTED, "embed: tokens are int64 or int32");
+    DB2_CHECK(vocab >= 0 && cols >= 0 && n >= 0, DB2_EINVAL, "embed: negative shape");
+    if (n == 0 || cols == 0)
+        return DB2_OK;
+    DB2_CHECK((table || vocab == 0) && tokens && res, DB2_EINVAL, "embed: null operand");
+    DB2_CHECK(ld_ok(table_ld, vocab, cols) && ld_ok(res_ld, n, cols) && ld_ok(tokens_ld, n, 1), DB2_EINVAL,
+              "embed: a leading dimension is smaller than the number of columns");
+#define DB2_EMBED(N, I)                                                                                                \
+    return embed_launch<T, N, I>(table, vocab, cols, table_ld, tokens, tokens_ld, n, scale, res, res_ld, dev_status,   \
+                                 as_stream(stream))
+    DB2_DISPATCH_SEQ(dtype, T, {
+        constexpr int N = 16 / sizeof(T);
+        if (rows_aligned(table, table_ld, sizeof(T), 16) && rows_aligned(res, res_ld, sizeof(T), 16)) {
+            if (index_dtype == DB2_I64)
+                DB2_EMBED(N, int64_t);
+            DB2_EMBED(N, int32_t);
+        }
+        if (index_dtype == DB2_I64)
+            DB2_EMBED(1, int64_t);
+        DB2_EMBED(1, int32_t);
+    });
+#undef DB2_EMBED
+    return DB2_OK;
+}
+
+size_t db2k_embed_grad_scratch_bytes(int dtype, int64_t vocab, int64_t cols, int64_t n) {
+    if (vocab <= 0 || cols <= 0 || n <= 0)
+        return 0;
+    return grad_plan(dtype == DB2_F64 ? 8 : 4, vocab, cols, n).bytes;
+}
+
+int db2k_embed_grad(int dtype, const void *grad, int64_t grad_ld, int64_t n, int64_t cols, int index_dtype,
+                    const void *tokens, int64_t tokens_ld, double scale, int res_dtype, void *res, int64_t vocab,
+                    int64_t res_ld, int accumulate, void *scratch, size_t scratch_bytes, int32_t *dev_status,
+                    void *stream) {
+    DB2_CHECK(seq_type(dtype), DB2_EUNSUPPORTED, "embedGrad: unsupported value type code %d", dtype);
+    DB2_CHECK(res_dtype == dtype || (res_dtype == DB2_F32 && dtype != DB2_F64), DB2_EUNSUPPORTED,
+              "embedGrad: the result has the value type of the gradient, or float");
+    DB2_CHECK(index_dtype == DB2_I64 || index_dtype == DB2_I32, DB2_EUNSUPPORTED,
+              "embedGrad: tokens are int64 or int32");
+    DB2_CHECK(vocab >= 0 && cols >= 0 && n >= 0, DB2_EINVAL, "embedGrad: negative shape");
+    DB2_CHECK(n < ((int64_t)1 << 31) && vocab < ((int64_t)1 << 31) - 1, DB2_EUNSUPPORTED,
+              "embedGrad: fewer than 2^31 tokens and table rows");
+    if (vocab == 0 || cols == 0)
+        return DB2_OK;
+    DB2_CHECK(res && ld_ok(res_ld, vocab, cols), DB2_EINVAL, "embedGrad: null result or a leading dimension too small");
+    cudaStream_t st = as_stream(stream);
+    if (n == 0) {
+        if (!accumulate)
+            DB2_CUDA(cudaMemset2DAsync(res, (size_t)(vocab > 1 ? res_ld : cols) * dtype_size(res_dtype), 0,
+                                       (size_t)cols * dtype_size(res_dtype), (size_t)vocab, st));
+        return DB2_OK;
+    }
+    const GradPlan p = grad_plan(dtype == DB2_F64 ? 8 : 4, vocab, cols, n);
+    DB2_CHECK(grad && tokens && ld_ok(grad_ld, n, cols) && ld_ok(tokens_ld, n, 1), DB2_EINVAL,
+              "embedGrad: null operand or a leading dimension too small");
+    DB2_CHECK(scratch && scratch_bytes >= p.bytes && aligned16(scratch), DB2_EINVAL,
+              "embedGrad: scratch smaller than db2k_embed_grad_scratch_bytes, or not 16-byte aligned");
+    SumArgs a{};
+    char *s = static_cast<char *>(scratch);
+    if (index_dtype == DB2_I64)
+        DB2_TRY(embed_sort<int64_t>(p, tokens, tokens_ld, n, vocab, s, &a.key, &a.pos, dev_status, st));
+    else
+        DB2_TRY(embed_sort<int32_t>(p, tokens, tokens_ld, n, vocab, s, &a.key, &a.pos, dev_status, st));
+    a.n = n;
+    a.cols = cols;
+    a.vocab = vocab;
+    a.grad_ld = grad_ld;
+    a.res_ld = res_ld;
+    a.part_ld = p.part_ld;
+    a.runs = p.runs;
+    DB2_DISPATCH_SEQ(dtype, T, {
+        if constexpr (sizeof(T) == 2) {
+            if (res_dtype == DB2_F32)
+                return embed_sum_any<T, float>(a, grad, scale, res, s + p.part_off, accumulate, st);
+        }
+        return embed_sum_any<T, T>(a, grad, scale, res, s + p.part_off, accumulate, st);
+    });
+    return DB2_OK;
+}
+
+int db2_embed(db2_context *ctx, db2_matrix **res, db2_matrix *table, db2_matrix *tokens, double scale) {
+    DB2_API_BEGIN
+    DB2_CHECK(ctx && res && table && tokens, DB2_EINVAL, "null argument");
+    DB2_CHECK(seq_type(table->dtype), DB2_EUNSUPPORTED, "embed: unsupported value type code %d", table->dtype);
+    DB2_CHECK(tokens->cols == 1, DB2_EINVAL, "embed: tokens must be a column matrix");
+    DB2_CHECK(tokens->dtype == DB2_I64 || tokens->dtype == DB2_I32, DB2_EUNSUPPORTED,
+              "embed: tokens are int64 or int32");
+    bind_device(ctx);
+    const uint64_t before = g_launches.load();
+    DB2_TRY(ensure_device(table));
+    DB2_TRY(ensure_device(tokens));
+    DB2_TRY(prepare_result(ctx, res, table->dtype, tokens->rows, table->cols));
+    DB2_TRY(clear_status(ctx));
+    DB2_TRY(db2k_embed(table->dtype, table->dev_ptr(), table->rows, table->cols, table->dev_ld, tokens->dtype,
+                       tokens->dev_ptr(), tokens->dev_ld, tokens->rows, scale, (*res)->dev_ptr(), (*res)->dev_ld,
+                       ctx->dev_status + EMB_STATUS, ctx->stream));
+    count(ctx, before);
+    return check_status(ctx, "embed", table->rows);
+    DB2_API_END
+}
+
+int db2_embedGrad(db2_context *ctx, db2_matrix **res, db2_matrix *grad, db2_matrix *tokens, int64_t vocab, double scale,
+                  int res_dtype, int accumulate) {
+    DB2_API_BEGIN
+    DB2_CHECK(ctx && res && grad && tokens, DB2_EINVAL, "null argument");
+    DB2_CHECK(seq_type(grad->dtype), DB2_EUNSUPPORTED, "embedGrad: unsupported value type code %d", grad->dtype);
+    DB2_CHECK(tokens->cols == 1 && tokens->rows == grad->rows, DB2_EINVAL,
+              "embedGrad: tokens must be a column matrix with as many rows as grad (%lld), got (%lld x %lld)",
+              (long long)grad->rows, (long long)tokens->rows, (long long)tokens->cols);
+    DB2_CHECK(tokens->dtype == DB2_I64 || tokens->dtype == DB2_I32, DB2_EUNSUPPORTED,
+              "embedGrad: tokens are int64 or int32");
+    DB2_CHECK(res_dtype == grad->dtype || (res_dtype == DB2_F32 && grad->dtype != DB2_F64), DB2_EUNSUPPORTED,
+              "embedGrad: the result has the value type of the gradient, or float");
+    DB2_CHECK(vocab >= 0, DB2_EINVAL, "embedGrad: negative number of table rows");
+    DB2_CHECK(*res || !accumulate, DB2_EINVAL, "embedGrad: adding needs a matrix to add to");
+    DB2_CHECK(*res != grad, DB2_EINVAL, "embedGrad: the result must not be the gradient");
+    bind_device(ctx);
+    const uint64_t before = g_launches.load();
+    DB2_TRY(ensure_device(grad));
+    DB2_TRY(ensure_device(tokens));
+    if (accumulate) {
+        DB2_CHECK((*res)->dtype == res_dtype && (*res)->rows == vocab && (*res)->cols == grad->cols, DB2_EINVAL,
+                  "embedGrad: the matrix to add to has shape (%lld x %lld) / type %d, expected (%lld x %lld) / type %d",
+                  (long long)(*res)->rows, (long long)(*res)->cols, (*res)->dtype, (long long)vocab,
+                  (long long)grad->cols, res_dtype);
+        DB2_TRY(prepare_update(*res));
+    } else {
+        DB2_TRY(prepare_result(ctx, res, res_dtype, vocab, grad->cols));
+    }
+    const size_t sb = db2k_embed_grad_scratch_bytes(grad->dtype, vocab, grad->cols, grad->rows);
+    void *scratch = nullptr;
+    DB2_TRY(ctx_scratch(ctx, sb, &scratch));
+    DB2_TRY(clear_status(ctx));
+    DB2_TRY(db2k_embed_grad(grad->dtype, grad->dev_ptr(), grad->dev_ld, grad->rows, grad->cols, tokens->dtype,
+                            tokens->dev_ptr(), tokens->dev_ld, scale, res_dtype, (*res)->dev_ptr(), vocab,
+                            (*res)->dev_ld, accumulate, scratch, ctx->scratch_bytes, ctx->dev_status + EMB_STATUS,
+                            ctx->stream));
+    count(ctx, before);
+    return check_status(ctx, "embedGrad", vocab);
+    DB2_API_END
+}
+
+} // extern "C"

@@ -163,6 +163,8 @@ int db2_readDaphne(db2_context *ctx, db2_matrix **res, const char *path) {
 int db2_writeDaphne(db2_context *ctx, db2_matrix *m, const char *path) {
     DB2_API_BEGIN
     DB2_CHECK(ctx && m && path, DB2_EINVAL, "null argument");
+    DB2_CHECK(m->dtype != DB2_F16 && m->dtype != DB2_BF16 && m->dtype != DB2_F8E4M3, DB2_EUNSUPPORTED,
+              "the file format has no value type for 16-bit and 8-bit floating-point matrices");
     DB2_CHECK(m->rows <= (int64_t)UINT32_MAX && m->cols <= (int64_t)UINT32_MAX, DB2_EUNSUPPORTED,
               "a single .dbdf block holds at most 2^32 - 1 rows and columns");
     bind_device(ctx);

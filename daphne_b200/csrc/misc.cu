@@ -99,6 +99,8 @@ extern "C" int db2k_transpose(int dtype, const void *arg, int64_t rows, int64_t 
     DB2_CHECK(rows >= 0 && cols >= 0, DB2_EINVAL, "negative dimension");
     if (rows * cols == 0)
         return DB2_OK;
+    DB2_CHECK(dtype_size(dtype) >= 4, DB2_EUNSUPPORTED, "transpose: value types of 4 and 8 bytes only (got code %d)",
+              dtype);
     const int64_t ntiles = ((rows + 31) / 32) * ((cols + 31) / 32);
     const int64_t cap = (int64_t)sm_count() * 8;
     const int grid = (int)(ntiles < cap ? ntiles : cap);
@@ -120,6 +122,9 @@ extern "C" int db2k_fill(int dtype, void *res, int64_t rows, int64_t cols, int64
     if (dtype_size(dtype) == 1)
         fill_kernel<uint8_t><<<grid, 256, 0, as_stream(stream)>>>(static_cast<uint8_t *>(res), rows, cols, ld,
                                                                  *static_cast<const uint8_t *>(value));
+    else if (dtype_size(dtype) == 2)
+        fill_kernel<uint16_t><<<grid, 256, 0, as_stream(stream)>>>(static_cast<uint16_t *>(res), rows, cols, ld,
+                                                                  *static_cast<const uint16_t *>(value));
     else if (dtype_size(dtype) == 8)
         fill_kernel<uint64_t><<<grid, 256, 0, as_stream(stream)>>>(static_cast<uint64_t *>(res), rows, cols, ld,
                                                                   *static_cast<const uint64_t *>(value));

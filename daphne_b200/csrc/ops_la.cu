@@ -2,6 +2,7 @@
 // seq, diagMatrix, ctable, castObj): argument checks with the reference's messages, result allocation, scratch.
 #include "fused.cuh"
 #include "runtime.h"
+#include "seq.cuh"
 
 #include <cmath>
 
@@ -18,6 +19,14 @@ __global__ void cast_kernel(const FROM *__restrict__ in, int64_t rows, int64_t c
 static void count(db2_context *ctx, uint64_t before) {
     std::lock_guard<std::mutex> lock(ctx->mu);
     ctx->stats.launches += g_launches.load(std::memory_order_relaxed) - before;
+}
+
+template <typename TO, typename FROM>
+__global__ void cast_seq_kernel(const FROM *__restrict__ in, int64_t rows, int64_t cols, int64_t ld,
+                                TO *__restrict__ out, int64_t out_ld) {
+    const int64_t n = rows * cols;
+    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x)
+        out[(i / cols) * out_ld + (i % cols)] = narrow<TO>(widen(in[(i / cols) * ld + (i % cols)]));
 }
 
 // The f32 contraction (tensor-core kernel with bounded waits) leaves a status word at the start of its scratch area;
@@ -480,6 +489,27 @@ int db2_castObj(db2_context *ctx, db2_matrix **res, db2_matrix *arg, int dtype) 
     DB2_CAST(DB2_I64, int64_t, DB2_I64, int64_t)
     DB2_CAST(DB2_U64, uint64_t, DB2_U64, uint64_t)
 #undef DB2_CAST
+// 16-bit and 8-bit floating point from and to double and float: one rounding to nearest even
+#define DB2_CAST_SEQ(FROM_CODE, FROM_T, TO_CODE, TO_T)                                                                 \
+    if (arg->dtype == FROM_CODE && dtype == TO_CODE) {                                                                 \
+        cast_seq_kernel<TO_T, FROM_T><<<grid, 256, 0, ctx->stream>>>(static_cast<const FROM_T *>(arg->dev_ptr()),      \
+                                                                     arg->rows, arg->cols, arg->dev_ld,                \
+                                                                     static_cast<TO_T *>(r->dev_ptr()), r->dev_ld);    \
+        DB2_TRY(after_launch("cast_seq_kernel"));                                                                      \
+        count(ctx, before);                                                                                            \
+        return DB2_OK;                                                                                                 \
+    }
+    DB2_CAST_SEQ(DB2_F64, double, DB2_F16, __half)
+    DB2_CAST_SEQ(DB2_F64, double, DB2_BF16, __nv_bfloat16)
+    DB2_CAST_SEQ(DB2_F32, float, DB2_F16, __half)
+    DB2_CAST_SEQ(DB2_F32, float, DB2_BF16, __nv_bfloat16)
+    DB2_CAST_SEQ(DB2_F16, __half, DB2_F64, double)
+    DB2_CAST_SEQ(DB2_F16, __half, DB2_F32, float)
+    DB2_CAST_SEQ(DB2_BF16, __nv_bfloat16, DB2_F64, double)
+    DB2_CAST_SEQ(DB2_BF16, __nv_bfloat16, DB2_F32, float)
+    DB2_CAST_SEQ(DB2_F8E4M3, __nv_fp8_e4m3, DB2_F64, double)
+    DB2_CAST_SEQ(DB2_F8E4M3, __nv_fp8_e4m3, DB2_F32, float)
+#undef DB2_CAST_SEQ
     return set_error(DB2_EUNSUPPORTED, "castObj from value type %d to %d", arg->dtype, dtype);
     DB2_API_END
 }

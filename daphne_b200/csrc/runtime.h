@@ -274,6 +274,8 @@ int nccl_allreduce_group(const std::vector<db2_context *> &ctxs, const std::vect
 int ensure_device(db2_matrix *m);
 // result allocation following the reference's "*res == nullptr means allocate" convention; checks shape/type otherwise
 int prepare_result(db2_context *ctx, db2_matrix **res, int dtype, int64_t rows, int64_t cols);
+// makes m the target of an update in place: current on the device, in a buffer that no other handle reads (embed.cu)
+int prepare_update(db2_matrix *m);
 } // namespace db2
 
 #define DB2_API_BEGIN try {

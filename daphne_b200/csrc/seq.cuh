@@ -1,0 +1,85 @@
+// Value types of the operators on sequences of tokens (embed.cu, rms_norm.cu, gated_scan.cu): storage type T, the type
+// W it is computed in (float; double for double), conversions and packets of several elements.
+#pragma once
+
+#include "common.cuh"
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+
+namespace db2 {
+
+template <typename T> struct WideOf {
+    using type = float;
+};
+template <> struct WideOf<double> {
+    using type = double;
+};
+template <typename T> using wide_t = typename WideOf<T>::type;
+
+__device__ __forceinline__ double widen(double x) { return x; }
+__device__ __forceinline__ float widen(float x) { return x; }
+__device__ __forceinline__ float widen(__half x) { return __half2float(x); }
+__device__ __forceinline__ float widen(__nv_bfloat16 x) { return __bfloat162float(x); }
+__device__ __forceinline__ float widen(__nv_fp8_e4m3 x) { return static_cast<float>(x); }
+
+// one rounding to nearest even
+template <typename T, typename W> __device__ __forceinline__ T narrow(W x) {
+    if constexpr (std::is_same_v<T, __half>) {
+        if constexpr (std::is_same_v<W, double>)
+            return __double2half(x);
+        else
+            return __float2half_rn(x);
+    } else if constexpr (std::is_same_v<T, __nv_bfloat16>) {
+        if constexpr (std::is_same_v<W, double>)
+            return __double2bfloat16(x);
+        else
+            return __float2bfloat16_rn(x);
+    } else
+        return static_cast<T>(x);
+}
+
+// N elements that are loaded and stored at once (N * sizeof(T) <= 16, the address a multiple of that)
+template <typename T, int N> struct alignas(sizeof(T) * N) Vec {
+    T v[N];
+};
+template <typename T, int N> __device__ __forceinline__ Vec<T, N> ld_vec(const T *p) {
+    return *reinterpret_cast<const Vec<T, N> *>(p);
+}
+template <typename T, int N> __device__ __forceinline__ void st_vec(T *p, const Vec<T, N> &x) {
+    *reinterpret_cast<Vec<T, N> *>(p) = x;
+}
+
+// whether rows of ld elements of es bytes starting at p all lie on multiples of `bytes` (absent operands do)
+inline bool rows_aligned(const void *p, int64_t ld, size_t es, size_t bytes) {
+    return !p || (reinterpret_cast<uintptr_t>(p) % bytes == 0 && (size_t)ld * es % bytes == 0);
+}
+
+// a matrix operand of `rows` rows: the leading dimension covers the columns (one row needs none)
+inline bool ld_ok(int64_t ld, int64_t rows, int64_t cols) { return ld >= cols || rows <= 1; }
+
+} // namespace db2
+
+// the four storage types of the sequence operators
+#define DB2_DISPATCH_SEQ(dtype, T, ...)                                                                                \
+    switch (dtype) {                                                                                                   \
+    case DB2_F64: {                                                                                                    \
+        using T = double;                                                                                              \
+        __VA_ARGS__;                                                                                                   \
+    } break;                                                                                                           \
+    case DB2_F32: {                                                                                                    \
+        using T = float;                                                                                               \
+        __VA_ARGS__;                                                                                                   \
+    } break;                                                                                                           \
+    case DB2_F16: {                                                                                                    \
+        using T = __half;                                                                                              \
+        __VA_ARGS__;                                                                                                   \
+    } break;                                                                                                           \
+    case DB2_BF16: {                                                                                                   \
+        using T = __nv_bfloat16;                                                                                       \
+        __VA_ARGS__;                                                                                                   \
+    } break;                                                                                                           \
+    default:                                                                                                           \
+        return ::db2::set_error(DB2_EUNSUPPORTED, "unsupported value type code %d", (int)(dtype));                     \
+    }

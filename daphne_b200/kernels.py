@@ -17,8 +17,21 @@ from .lib import Db2Error, check, lib
 
 _NP2DT = {np.dtype(np.float64): _l.F64, np.dtype(np.float32): _l.F32, np.dtype(np.int64): _l.I64,
           np.dtype(np.uint64): _l.U64, np.dtype(np.int32): _l.I32, np.dtype(np.uint32): _l.U32,
-          np.dtype(np.uint8): _l.U8}
-_DT2NP = {v: k for k, v in _NP2DT.items()}
+          np.dtype(np.uint8): _l.U8, np.dtype(np.float16): _l.F16}
+# value types that numpy does not have go by these names; their matrices come to the host as bit patterns
+BFLOAT16, FLOAT8_E4M3 = "bfloat16", "float8_e4m3"
+_NAMED = {BFLOAT16: _l.BF16, FLOAT8_E4M3: _l.F8E4M3}
+_DT2NP = {**{v: k for k, v in _NP2DT.items()}, _l.BF16: np.dtype(np.uint16), _l.F8E4M3: np.dtype(np.uint8)}
+
+
+def _code(dtype) -> int:
+    """The value type code of a numpy type, or of BFLOAT16 / FLOAT8_E4M3."""
+    if isinstance(dtype, str) and dtype in _NAMED:
+        return _NAMED[dtype]
+    try:
+        return _NP2DT[np.dtype(dtype)]
+    except (KeyError, TypeError):
+        raise Db2Error(4, f"unsupported value type {dtype!r}") from None
 
 
 class BinaryOpCode(enum.IntEnum):  # BinaryOpCode.h:29-56
@@ -97,6 +110,7 @@ class DenseMatrix:
 
     @property
     def dtype(self):
+        """The numpy type that the values come to the host in (bit patterns for bfloat16 and float8_e4m3)."""
         return _DT2NP[self.dtype_code]
 
     @staticmethod
@@ -117,14 +131,13 @@ class DenseMatrix:
     @staticmethod
     def empty(ctx: Context, rows: int, cols: int, dtype=np.float64, zero: bool = False) -> "DenseMatrix":
         h = C.c_void_p()
-        check(lib.db2_matrix_create(ctx.handle, _NP2DT[np.dtype(dtype)], rows, cols, int(zero), C.byref(h)))
+        check(lib.db2_matrix_create(ctx.handle, _code(dtype), rows, cols, int(zero), C.byref(h)))
         return DenseMatrix(ctx, h)
 
     @staticmethod
     def wrap_device(ctx: Context, ptr: int, rows: int, cols: int, ld: int, dtype=np.float64, keep=None):
         h = C.c_void_p()
-        check(lib.db2_matrix_wrap_device(ctx.handle, _NP2DT[np.dtype(dtype)], rows, cols, ld, C.c_void_p(ptr),
-                                         C.byref(h)))
+        check(lib.db2_matrix_wrap_device(ctx.handle, _code(dtype), rows, cols, ld, C.c_void_p(ptr), C.byref(h)))
         return DenseMatrix(ctx, h, keep=keep)
 
     def slice_rows(self, r0: int, r1: int) -> "DenseMatrix":
@@ -428,7 +441,33 @@ def ctable(lhs: DenseMatrix, rhs: DenseMatrix, weight: float = 1.0, resNumRows: 
 def castObj(arg: DenseMatrix, dtype, ctx: Optional[Context] = None) -> DenseMatrix:
     ctx = ctx or arg.ctx
     h = C.c_void_p()
-    check(lib.db2_castObj(ctx.handle, C.byref(h), arg.handle, _NP2DT[np.dtype(dtype)]))
+    check(lib.db2_castObj(ctx.handle, C.byref(h), arg.handle, _code(dtype)))
+    return _res(ctx, h)
+
+
+# ---- operators on sequences of tokens (no counterpart in the reference) ----
+
+
+def embed(table: DenseMatrix, tokens: DenseMatrix, scale: float = 1.0, ctx: Optional[Context] = None) -> DenseMatrix:
+    """res[i] = scale * table[tokens[i]]; token -1 gives a row of zeros, any other token outside the table is an error."""
+    ctx = ctx or table.ctx
+    h = C.c_void_p()
+    check(lib.db2_embed(ctx.handle, C.byref(h), table.handle, tokens.handle, float(scale)))
+    return _res(ctx, h)
+
+
+def embedGrad(grad: DenseMatrix, tokens: DenseMatrix, vocab: int, scale: float = 1.0, dtype=None,
+              add_to: Optional[DenseMatrix] = None, ctx: Optional[Context] = None) -> DenseMatrix:
+    """Gradient of the table of `vocab` rows: scale * (sum of the rows of grad per token), as a new matrix of `dtype`
+    (default: the type of grad; np.float32 for the 16-bit types too) or added to `add_to`, which is returned."""
+    ctx = ctx or grad.ctx
+    if add_to is not None:
+        check(lib.db2_embedGrad(ctx.handle, C.byref(add_to._h), grad.handle, tokens.handle, int(vocab), float(scale),
+                                add_to.dtype_code, 1))
+        return add_to
+    h = C.c_void_p()
+    code = grad.dtype_code if dtype is None else _code(dtype)
+    check(lib.db2_embedGrad(ctx.handle, C.byref(h), grad.handle, tokens.handle, int(vocab), float(scale), code, 0))
     return _res(ctx, h)
 
 

@@ -12,7 +12,7 @@ _PKG = Path(__file__).resolve().parent
 LIB_PATH = _PKG / "libdaphne_b200.so"
 
 # value type codes (include/daphne_b200.h)
-F64, F32, I64, U64, I32, U32, U8 = 0, 1, 2, 3, 4, 5, 6
+F64, F32, I64, U64, I32, U32, U8, F16, BF16, F8E4M3 = 0, 1, 2, 3, 4, 5, 6, 7, 8, 9
 
 
 class Db2Error(RuntimeError):
@@ -92,6 +92,10 @@ _SIGS = {
     "db2k_ctable": (i32, [vp, i64, vp, i64, i64, C.c_double, vp, i64, i64, i64, i32, vp]),
     "db2k_solve_scratch_bytes": (sz, [i64]),
     "db2k_solve": (i32, [i32, vp, i64, vp, vp, vp, sz, vp]),
+    "db2k_embed": (i32, [i32, vp, i64, i64, i64, i32, vp, i64, i64, C.c_double, vp, i64, vp, vp]),
+    "db2k_embed_grad_scratch_bytes": (sz, [i32, i64, i64, i64]),
+    "db2k_embed_grad": (i32, [i32, vp, i64, i64, i64, i32, vp, i64, C.c_double, i32, vp, i64, i64, i32, vp, sz, vp,
+                              vp]),
     # runtime
     "db2_context_create": (i32, [i32, _P(vp)]),
     "db2_context_destroy": (i32, [vp]),
@@ -178,6 +182,8 @@ _SIGS = {
     "db2_extractCol": (i32, [vp, _P(vp), vp, vp]),
     "db2_ctable": (i32, [vp, _P(vp), vp, vp, C.c_double, i64, i64]),
     "db2_castObj": (i32, [vp, _P(vp), vp, i32]),
+    "db2_embed": (i32, [vp, _P(vp), vp, vp, C.c_double]),
+    "db2_embedGrad": (i32, [vp, _P(vp), vp, vp, i64, C.c_double, i32, i32]),
     "db2_readDaphne": (i32, [vp, _P(vp), C.c_char_p]),
     "db2_writeDaphne": (i32, [vp, vp, C.c_char_p]),
     "db2_vectorizedPipeline": (i32, [vp, _P(vp), sz, _P(i32), _P(vp), sz, _P(i64), _P(i64), _P(i64), _P(i64), vp, i64]),

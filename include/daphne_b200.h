@@ -50,8 +50,13 @@ enum { DB2_OK = 0, DB2_EINVAL = 1, DB2_ECUDA = 2, DB2_ENOMEM = 3, DB2_EUNSUPPORT
 /* value types (kernels.json instantiates the hot kernels for double, float, int64_t; size_t is the value type of
  * idxMin/idxMax results, AggRow.h:71-96).  The elementwise binary kernels (matrix and scalar rhs), fill and transpose
  * also take uint64_t, int32_t and uint32_t like the reference's CUDA instantiations (kernels/CUDA/EwBinaryMat.cu:265-270,
- * EwBinaryObjSca.cu:89-94); DB2_U8 (uint8_t and bool) exists for fill only (CUDA/Fill.cu:44-49). */
-enum { DB2_F64 = 0, DB2_F32 = 1, DB2_I64 = 2, DB2_U64 = 3, DB2_I32 = 4, DB2_U32 = 5, DB2_U8 = 6 };
+ * EwBinaryObjSca.cu:89-94); DB2_U8 (uint8_t and bool) exists for fill only (CUDA/Fill.cu:44-49).
+ * DB2_F16 (IEEE binary16), DB2_BF16 (the upper half of a binary32) and DB2_F8E4M3 (1 + 4 + 3 bits, largest value 448, no
+ * infinities) are storage types of the operators on sequences of tokens: embed, rmsNorm, gatedScan and their gradients
+ * compute in 32 bits and round once per stored value.  fill, castObj, views, copies and transfers take them too (castObj
+ * from DB2_F8E4M3, not to it); every other operator refuses them (DB2_EUNSUPPORTED). */
+enum { DB2_F64 = 0, DB2_F32 = 1, DB2_I64 = 2, DB2_U64 = 3, DB2_I32 = 4, DB2_U32 = 5, DB2_U8 = 6, DB2_F16 = 7,
+       DB2_BF16 = 8, DB2_F8E4M3 = 9 };
 
 /* BinaryOpCode (src/runtime/local/kernels/BinaryOpCode.h:29-56) */
 enum { DB2_ADD = 0, DB2_SUB, DB2_MUL, DB2_DIV, DB2_POW, DB2_MOD, DB2_LOG, DB2_EQ, DB2_NEQ, DB2_LT, DB2_LE, DB2_GT,
@@ -253,6 +258,29 @@ size_t db2k_solve_scratch_bytes(int64_t n);
 int db2k_solve(int dtype, void *a_work, int64_t n, void *x_inout, int32_t *dev_status, void *scratch,
                size_t scratch_bytes, void *stream);
 
+/* ---- operators on sequences of tokens (no counterpart in the reference) ----
+ * Value types DB2_F64, DB2_F32, DB2_F16 and DB2_BF16; sums, statistics and states are double for DB2_F64 and float for
+ * the others ("wide" below), and every stored value is rounded once.  All calls are asynchronous on `stream`, allocate
+ * nothing and may be captured into a graph; scratch belongs to one call at a time and must be 16-byte aligned. */
+
+/* Embedding: res[i] = scale * table[tokens[i]] for n tokens (DB2_I64 or DB2_I32, stride tokens_ld) and a table of vocab
+ * rows.  Token -1 marks padding and gives a row of zeros; any other token outside [0, vocab) gives a row of zeros and
+ * sets *dev_status (a device int32, may be NULL; never cleared here) to 1.  The product of one-hot rows with the table,
+ * without the one-hot rows. */
+int db2k_embed(int dtype, const void *table, int64_t vocab, int64_t cols, int64_t table_ld, int index_dtype,
+               const void *tokens, int64_t tokens_ld, int64_t n, double scale, void *res, int64_t res_ld,
+               int32_t *dev_status, void *stream);
+/* Its gradient: res[v] = scale * sum of grad[i] over the i with tokens[i] == v, for all vocab rows (rows of other tokens
+ * become zero), or, with accumulate != 0, added to res[v] (other rows are left alone).  The sums are formed in the wide
+ * type over the tokens sorted by (token, position), in an order that the inputs alone determine: the same bits in every
+ * run.  res_dtype: dtype, or DB2_F32 for the 16-bit types.  Tokens that name no row are skipped, *dev_status as above.
+ * res must not overlap grad.  Fewer than 2^31 tokens and rows (DB2_EUNSUPPORTED). */
+size_t db2k_embed_grad_scratch_bytes(int dtype, int64_t vocab, int64_t cols, int64_t n);
+int db2k_embed_grad(int dtype, const void *grad, int64_t grad_ld, int64_t n, int64_t cols, int index_dtype,
+                    const void *tokens, int64_t tokens_ld, double scale, int res_dtype, void *res, int64_t vocab,
+                    int64_t res_ld, int accumulate, void *scratch, size_t scratch_bytes, int32_t *dev_status,
+                    void *stream);
+
 /* ------------------------------------------------------------------------- */
 /* db2_*: runtime -- context, matrix handles with residency, operator calls   */
 /* ------------------------------------------------------------------------- */
@@ -403,8 +431,15 @@ int db2_sliceCol(db2_context *ctx, db2_matrix **res, db2_matrix *arg, int64_t lo
  * of `dtype`.  Replaces RandMatrix<DenseMatrix<VT>, VT> (src/runtime/local/kernels/RandMatrix.h:82-161). */
 int db2_randMatrix(db2_context *ctx, db2_matrix **res, int dtype, int64_t rows, int64_t cols, const void *min,
                    const void *max, double sparsity, int64_t seed);
-/* value-type cast between f64 / i64 / u64 (CastObj, used for idxMin results feeding ctable) */
+/* value-type cast between f64 / i64 / u64 (CastObj, used for idxMin results feeding ctable), f64 / f32, and from and to
+ * the 16-bit floating-point types (from DB2_F8E4M3 only) */
 int db2_castObj(db2_context *ctx, db2_matrix **res, db2_matrix *arg, int dtype);
+/* Operators on sequences of tokens: db2k_embed, db2k_embed_grad (see there) on handles.  tokens: column matrix of int64
+ * or int32.  A token outside the table that is not -1 is DB2_EDOMAIN; to say so the calls wait for the device (the
+ * db2k_ forms do not).  embedGrad with accumulate adds to *res, which must be given. */
+int db2_embed(db2_context *ctx, db2_matrix **res, db2_matrix *table, db2_matrix *tokens, double scale);
+int db2_embedGrad(db2_context *ctx, db2_matrix **res, db2_matrix *grad, db2_matrix *tokens, int64_t vocab, double scale,
+                  int res_dtype, int accumulate);
 
 /* ------------------------------------------------------------------------- */
 /* row-partition scheduler                                                    */
