@@ -635,6 +635,17 @@ int check_status(db2_context *ctx, const char *what, int64_t vocab) {
 
 } // namespace
 
+DeviceOperand::DeviceOperand(db2_matrix *m) {
+    if (!m)
+        return;
+    const int rc = ensure_device(m);
+    if (rc != DB2_OK)
+        throw Error(rc, err_buf());
+    keep = m->dev;
+    ptr = m->dev_ptr();
+    ld = m->dev_ld;
+}
+
 int prepare_update(db2_matrix *m) {
     DB2_TRY(ensure_device(m));
     if (!m->is_view && m->dev.use_count() > 1) {
@@ -737,13 +748,11 @@ int db2k_embed_grad(int dtype, const void *grad, int64_t grad_ld, int64_t n, int
     a.res_ld = res_ld;
     a.part_ld = p.part_ld;
     a.runs = p.runs;
-    DB2_DISPATCH_SEQ(dtype, T, {
-        if constexpr (sizeof(T) == 2) {
-            if (res_dtype == DB2_F32)
-                return embed_sum_any<T, float>(a, grad, scale, res, s + p.part_off, accumulate, st);
-        }
-        return embed_sum_any<T, T>(a, grad, scale, res, s + p.part_off, accumulate, st);
-    });
+    if (dtype == DB2_F16 && res_dtype == DB2_F32)
+        return embed_sum_any<__half, float>(a, grad, scale, res, s + p.part_off, accumulate, st);
+    if (dtype == DB2_BF16 && res_dtype == DB2_F32)
+        return embed_sum_any<__nv_bfloat16, float>(a, grad, scale, res, s + p.part_off, accumulate, st);
+    DB2_DISPATCH_SEQ(dtype, T, return (embed_sum_any<T, T>(a, grad, scale, res, s + p.part_off, accumulate, st)));
     return DB2_OK;
 }
 
@@ -756,13 +765,11 @@ int db2_embed(db2_context *ctx, db2_matrix **res, db2_matrix *table, db2_matrix 
               "embed: tokens are int64 or int32");
     bind_device(ctx);
     const uint64_t before = g_launches.load();
-    DB2_TRY(ensure_device(table));
-    DB2_TRY(ensure_device(tokens));
+    const DeviceOperand dt(table), di(tokens);
     DB2_TRY(prepare_result(ctx, res, table->dtype, tokens->rows, table->cols));
     DB2_TRY(clear_status(ctx));
-    DB2_TRY(db2k_embed(table->dtype, table->dev_ptr(), table->rows, table->cols, table->dev_ld, tokens->dtype,
-                       tokens->dev_ptr(), tokens->dev_ld, tokens->rows, scale, (*res)->dev_ptr(), (*res)->dev_ld,
-                       ctx->dev_status + EMB_STATUS, ctx->stream));
+    DB2_TRY(db2k_embed(table->dtype, dt.ptr, table->rows, table->cols, dt.ld, tokens->dtype, di.ptr, di.ld, tokens->rows,
+                       scale, (*res)->dev_ptr(), (*res)->dev_ld, ctx->dev_status + EMB_STATUS, ctx->stream));
     count(ctx, before);
     return check_status(ctx, "embed", table->rows);
     DB2_API_END
@@ -782,11 +789,9 @@ int db2_embedGrad(db2_context *ctx, db2_matrix **res, db2_matrix *grad, db2_matr
               "embedGrad: the result has the value type of the gradient, or float");
     DB2_CHECK(vocab >= 0, DB2_EINVAL, "embedGrad: negative number of table rows");
     DB2_CHECK(*res || !accumulate, DB2_EINVAL, "embedGrad: adding needs a matrix to add to");
-    DB2_CHECK(*res != grad, DB2_EINVAL, "embedGrad: the result must not be the gradient");
     bind_device(ctx);
     const uint64_t before = g_launches.load();
-    DB2_TRY(ensure_device(grad));
-    DB2_TRY(ensure_device(tokens));
+    const DeviceOperand dg(grad), di(tokens);
     if (accumulate) {
         DB2_CHECK((*res)->dtype == res_dtype && (*res)->rows == vocab && (*res)->cols == grad->cols, DB2_EINVAL,
                   "embedGrad: the matrix to add to has shape (%lld x %lld) / type %d, expected (%lld x %lld) / type %d",
@@ -800,10 +805,9 @@ int db2_embedGrad(db2_context *ctx, db2_matrix **res, db2_matrix *grad, db2_matr
     void *scratch = nullptr;
     DB2_TRY(ctx_scratch(ctx, sb, &scratch));
     DB2_TRY(clear_status(ctx));
-    DB2_TRY(db2k_embed_grad(grad->dtype, grad->dev_ptr(), grad->dev_ld, grad->rows, grad->cols, tokens->dtype,
-                            tokens->dev_ptr(), tokens->dev_ld, scale, res_dtype, (*res)->dev_ptr(), vocab,
-                            (*res)->dev_ld, accumulate, scratch, ctx->scratch_bytes, ctx->dev_status + EMB_STATUS,
-                            ctx->stream));
+    DB2_TRY(db2k_embed_grad(grad->dtype, dg.ptr, dg.ld, grad->rows, grad->cols, tokens->dtype, di.ptr, di.ld, scale,
+                            res_dtype, (*res)->dev_ptr(), vocab, (*res)->dev_ld, accumulate, scratch,
+                            ctx->scratch_bytes, ctx->dev_status + EMB_STATUS, ctx->stream));
     count(ctx, before);
     return check_status(ctx, "embedGrad", vocab);
     DB2_API_END

@@ -1,0 +1,837 @@
+// Root-mean-square norm of the rows of a matrix, with the addition of a residual in front of it, and its gradient.
+//
+//   s = x + residual (rounded to the value type: what is stored is what is normalised)      s = x without a residual
+//   rstd = 1 / sqrt(mean(s^2) + eps)          y = s * rstd * weight
+//   8-bit result: per group of columns  scale = max|y| / 448,  q = e4m3(y / scale)
+//
+//   t = dy * weight       dx = rstd * (t - s * rstd^2 * mean(t * s)) + dsum       dweight = column sums of dy * s * rstd
+//
+// Statistics, products and sums are float (double for double).  All of it is bound by memory: a row is read once, kept
+// in registers while its sum is formed, and written from there.
+#include "runtime.h"
+#include "seq.cuh"
+
+namespace db2 {
+
+namespace {
+
+constexpr float E4M3_MAX = 448.0f;
+
+// sum over the `tpr` threads of a row (a power of two; rows lie side by side in the CTA), in one fixed order.  Every
+// thread of the CTA calls it the same number of times; `red` alternates between two halves, so one barrier is enough.
+template <typename W, int BLOCK> struct RowSum {
+    W *red; // 2 * BLOCK / 32
+    int turn = 0;
+    __device__ W operator()(W v, int tpr) {
+        const int in_warp = tpr < 32 ? tpr : 32;
+        for (int o = in_warp >> 1; o >= 1; o >>= 1)
+            v += shfl_xor(v, o);
+        if (tpr <= 32)
+            return v;
+        W *half = red + turn * (BLOCK / 32);
+        turn ^= 1;
+        const int warp = threadIdx.x / 32;
+        if (threadIdx.x % 32 == 0)
+            half[warp] = v;
+        __syncthreads();
+        const int warps = tpr / 32, first = warp / warps * warps;
+        W s = half[first];
+        for (int k = 1; k < warps; k++)
+            s += half[first + k];
+        return s;
+    }
+};
+
+// packet p (N columns) of a row; the last one may be narrower
+template <typename T, int N> __device__ __forceinline__ Vec<T, N> load_packet(const T *row, int64_t p, int64_t cols) {
+    const int64_t c = p * N;
+    if constexpr (N > 1)
+        if (c + N > cols) {
+            Vec<T, N> x;
+#pragma unroll
+            for (int k = 0; k < N; k++)
+                x.v[k] = c + k < cols ? row[c + k] : narrow<T>(0.0f);
+            return x;
+        }
+    return ld_vec<T, N>(row + c);
+}
+template <typename T, int N>
+__device__ __forceinline__ void store_packet(T *row, int64_t p, int64_t cols, const Vec<T, N> &x) {
+    const int64_t c = p * N;
+    if constexpr (N > 1)
+        if (c + N > cols) {
+#pragma unroll
+            for (int k = 0; k < N; k++)
+                if (c + k < cols)
+                    row[c + k] = x.v[k];
+            return;
+        }
+    st_vec<T, N>(row + c, x);
+}
+
+template <typename T> struct NormArgs { // x, residual and sum may be the same matrix, and res one of x and residual
+    const T *x, *residual, *weight;
+    T *sum;
+    void *res; // T, or e4m3
+    float *scales;
+    wide_t<T> *rstd;
+    int64_t rows, cols, x_ld, residual_ld, sum_ld, res_ld, scales_ld;
+    int64_t group;  // columns per scale; 0: one scale a row
+    int64_t groups; // scales per row
+    wide_t<T> eps;
+};
+
+template <typename T, int N>
+__device__ __forceinline__ Vec<T, N> add_residual(const Vec<T, N> &x, const Vec<T, N> &r) {
+    Vec<T, N> s;
+#pragma unroll
+    for (int k = 0; k < N; k++)
+        s.v[k] = narrow<T>(widen(x.v[k]) + widen(r.v[k]));
+    return s;
+}
+template <typename T, int N> __device__ __forceinline__ void squares(const Vec<T, N> &s, wide_t<T> *ss) {
+#pragma unroll
+    for (int k = 0; k < N; k++) {
+        const wide_t<T> v = widen(s.v[k]);
+        *ss += v * v;
+    }
+}
+// y of a packet; columns behind the end give 0 (their s is 0)
+template <typename T, int N>
+__device__ __forceinline__ void normalised(const Vec<T, N> &s, const T *weight, int64_t p, int64_t cols, wide_t<T> rstd,
+                                           wide_t<T> *y) {
+    Vec<T, N> w;
+    if (weight)
+        w = load_packet<T, N>(weight, p, cols);
+#pragma unroll
+    for (int k = 0; k < N; k++)
+        y[k] = weight ? widen(s.v[k]) * rstd * widen(w.v[k]) : widen(s.v[k]) * rstd;
+}
+// |y| as an integer: the order of non-negative floats is that of their bits, and a NaN is above infinity, so a maximum
+// over the bits does not depend on the order and keeps a NaN
+template <int N> __device__ __forceinline__ unsigned largest(const float *y) {
+    unsigned m = 0;
+#pragma unroll
+    for (int k = 0; k < N; k++)
+        m = max(m, __float_as_uint(y[k]) & 0x7fffffffu);
+    return m;
+}
+// 1 for a group of zeros; never below the smallest normal number, whose reciprocal is finite
+__device__ __forceinline__ float scale_of(unsigned most) {
+    if (most == 0)
+        return 1.0f;
+    const float m = __uint_as_float(most);
+    if (m != m)
+        return m;
+    return fmaxf(m / E4M3_MAX, 1.17549435e-38f);
+}
+template <int N>
+__device__ __forceinline__ void store_q8(void *res, int64_t at, int64_t p, int64_t cols, const float *y, float inv) {
+    Vec<__nv_fp8_storage_t, N> q;
+#pragma unroll
+    for (int k = 0; k < N; k++)
+        q.v[k] = __nv_cvt_float_to_fp8(y[k] * inv, __NV_SATFINITE, __NV_E4M3);
+    store_packet<__nv_fp8_storage_t, N>(static_cast<__nv_fp8_storage_t *>(res) + at, p, cols, q);
+}
+
+// Rows of up to tpr * PPT packets: a thread holds packets tx, tx + tpr, ... of its row.
+template <typename T, int N, int PPT, bool Q8, int BLOCK>
+__global__ void __launch_bounds__(BLOCK) norm_rows_kernel(NormArgs<T> a, int log_tpr) {
+    using W = wide_t<T>;
+    __shared__ W red[2 * (BLOCK / 32)];
+    extern __shared__ unsigned group_max[]; // rows of the CTA x groups (8-bit results whose groups span warps)
+    const int tpr = 1 << log_tpr, tx = threadIdx.x & (tpr - 1), ty = threadIdx.x >> log_tpr, at_once = BLOCK >> log_tpr;
+    const int64_t packets = (a.cols + N - 1) / N;
+    RowSum<W, BLOCK> row_sum{red};
+    for (int64_t r0 = (int64_t)blockIdx.x * at_once; r0 < a.rows; r0 += (int64_t)gridDim.x * at_once) {
+        const int64_t r = r0 + ty;
+        const bool live = r < a.rows;
+        Vec<T, N> s[PPT];
+        if (live) {
+            const T *x = a.x + r * a.x_ld;
+#pragma unroll
+            for (int k = 0; k < PPT; k++)
+                if (tx + k * tpr < packets)
+                    s[k] = load_packet<T, N>(x, tx + k * tpr, a.cols);
+            if (a.residual) {
+                const T *res = a.residual + r * a.residual_ld;
+                Vec<T, N> y[PPT];
+#pragma unroll
+                for (int k = 0; k < PPT; k++)
+                    if (tx + k * tpr < packets)
+                        y[k] = load_packet<T, N>(res, tx + k * tpr, a.cols);
+#pragma unroll
+                for (int k = 0; k < PPT; k++)
+                    s[k] = add_residual(s[k], y[k]);
+            }
+            if (a.sum) {
+                T *sum = a.sum + r * a.sum_ld;
+#pragma unroll
+                for (int k = 0; k < PPT; k++)
+                    if (tx + k * tpr < packets)
+                        store_packet<T, N>(sum, tx + k * tpr, a.cols, s[k]);
+            }
+        }
+        W ss = 0;
+#pragma unroll
+        for (int k = 0; k < PPT; k++)
+            if (live && tx + k * tpr < packets)
+                squares(s[k], &ss);
+        const W rstd = W(1) / sqrt(row_sum(ss, tpr) / W(a.cols) + a.eps);
+        if (live && tx == 0 && a.rstd)
+            a.rstd[r] = rstd;
+        if constexpr (!Q8) {
+            if (live) {
+                T *res = static_cast<T *>(a.res) + r * a.res_ld;
+#pragma unroll
+                for (int k = 0; k < PPT; k++)
+                    if (tx + k * tpr < packets) {
+                        W y[N];
+                        normalised<T, N>(s[k], a.weight, tx + k * tpr, a.cols, rstd, y);
+                        Vec<T, N> z;
+#pragma unroll
+                        for (int j = 0; j < N; j++)
+                            z.v[j] = narrow<T>(y[j]);
+                        store_packet<T, N>(res, tx + k * tpr, a.cols, z);
+                    }
+            }
+        } else {
+            float y[PPT][N];
+            unsigned most[PPT];
+#pragma unroll
+            for (int k = 0; k < PPT; k++) {
+                most[k] = 0;
+                if (live && tx + k * tpr < packets) {
+                    normalised<T, N>(s[k], a.weight, tx + k * tpr, a.cols, rstd, y[k]);
+                    most[k] = largest<N>(y[k]);
+                }
+            }
+            if (a.group == 0) {
+#pragma unroll
+                for (int k = 1; k < PPT; k++)
+                    most[0] = max(most[0], most[k]);
+#pragma unroll
+                for (int k = 1; k < PPT; k++)
+                    most[k] = most[0];
+            }
+            // threads that hold one group side by side, and whether a warp holds all of it
+            const int64_t lanes64 = a.group == 0 ? tpr : a.group / N;
+            const bool in_warp = lanes64 <= 32 && lanes64 <= tpr;
+            const int lanes = (int)(in_warp ? lanes64 : (tpr < 32 ? tpr : 32));
+#pragma unroll
+            for (int k = 0; k < PPT; k++)
+                for (int o = lanes >> 1; o >= 1; o >>= 1)
+                    most[k] = max(most[k], __shfl_xor_sync(0xffffffffu, most[k], o));
+            if (!in_warp) {
+                unsigned *gm = group_max + ty * a.groups;
+                for (int64_t g = tx; g < a.groups; g += tpr)
+                    gm[g] = 0;
+                __syncthreads();
+#pragma unroll
+                for (int k = 0; k < PPT; k++)
+                    if (live && tx + k * tpr < packets && (tx & (lanes - 1)) == 0)
+                        atomicMax(&gm[a.group == 0 ? 0 : (int64_t)(tx + k * tpr) * N / a.group], most[k]);
+                __syncthreads();
+#pragma unroll
+                for (int k = 0; k < PPT; k++)
+                    if (tx + k * tpr < packets)
+                        most[k] = gm[a.group == 0 ? 0 : (int64_t)(tx + k * tpr) * N / a.group];
+                __syncthreads();
+            }
+            if (live) {
+#pragma unroll
+                for (int k = 0; k < PPT; k++)
+                    if (tx + k * tpr < packets) {
+                        const float scale = scale_of(most[k]);
+                        const int64_t c = (int64_t)(tx + k * tpr) * N;
+                        if (a.group == 0 ? c == 0 : c % a.group == 0)
+                            a.scales[r * a.scales_ld + (a.group == 0 ? 0 : c / a.group)] = scale;
+                        store_q8<N>(a.res, r * a.res_ld, tx + k * tpr, a.cols, y[k], 1.0f / scale);
+                    }
+            }
+        }
+    }
+}
+
+// Rows that registers do not hold: one CTA per row, which is read again for every pass.  The sum is read back from where
+// it was stored (the thread that stored a packet reads it), so x and residual may be overwritten by it.
+constexpr int LONG_BLOCK = 512;
+template <typename T, int N, bool Q8>
+__global__ void __launch_bounds__(LONG_BLOCK) norm_long_kernel(NormArgs<T> a) {
+    using W = wide_t<T>;
+    __shared__ W red[2 * (LONG_BLOCK / 32)];
+    __shared__ unsigned group_max[LONG_BLOCK * N / 16 + 1];
+    const int64_t packets = (a.cols + N - 1) / N;
+    RowSum<W, LONG_BLOCK> row_sum{red};
+    for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
+        const T *x = a.x + r * a.x_ld, *residual = a.residual ? a.residual + r * a.residual_ld : nullptr;
+        auto stream = [&](int64_t p) {
+            const Vec<T, N> v = load_packet<T, N>(x, p, a.cols);
+            return residual ? add_residual(v, load_packet<T, N>(residual, p, a.cols)) : v;
+        };
+        auto again = [&](int64_t p) {
+            return a.sum ? load_packet<T, N>(a.sum + r * a.sum_ld, p, a.cols) : stream(p);
+        };
+        W ss = 0;
+        for (int64_t p = threadIdx.x; p < packets; p += LONG_BLOCK) {
+            const Vec<T, N> s = stream(p);
+            if (a.sum)
+                store_packet<T, N>(a.sum + r * a.sum_ld, p, a.cols, s);
+            squares(s, &ss);
+        }
+        const W rstd = W(1) / sqrt(row_sum(ss, LONG_BLOCK) / W(a.cols) + a.eps);
+        if (threadIdx.x == 0 && a.rstd)
+            a.rstd[r] = rstd;
+        if constexpr (!Q8) {
+            for (int64_t p = threadIdx.x; p < packets; p += LONG_BLOCK) {
+                W y[N];
+                normalised<T, N>(again(p), a.weight, p, a.cols, rstd, y);
+                Vec<T, N> z;
+#pragma unroll
+                for (int k = 0; k < N; k++)
+                    z.v[k] = narrow<T>(y[k]);
+                store_packet<T, N>(static_cast<T *>(a.res) + r * a.res_ld, p, a.cols, z);
+            }
+        } else {
+            // turns of LONG_BLOCK packets, which hold whole groups (a group has at most 512 columns)
+            unsigned row_most = 0;
+            if (a.group == 0) {
+                if (threadIdx.x == 0)
+                    group_max[0] = 0;
+                __syncthreads();
+                for (int64_t p = threadIdx.x; p < packets; p += LONG_BLOCK) {
+                    float y[N];
+                    normalised<T, N>(again(p), a.weight, p, a.cols, rstd, y);
+                    row_most = max(row_most, largest<N>(y));
+                }
+                atomicMax(&group_max[0], row_most);
+                __syncthreads();
+                row_most = group_max[0];
+                __syncthreads();
+            }
+            for (int64_t p0 = 0; p0 < packets; p0 += LONG_BLOCK) {
+                const int64_t p = p0 + threadIdx.x;
+                float y[N];
+                unsigned most = row_most;
+                if (p < packets)
+                    normalised<T, N>(again(p), a.weight, p, a.cols, rstd, y);
+                if (a.group) {
+                    const int g = (int)((int64_t)threadIdx.x * N / a.group);
+                    for (int i = threadIdx.x; i < (int)(LONG_BLOCK * N / a.group) + 1; i += LONG_BLOCK)
+                        group_max[i] = 0;
+                    __syncthreads();
+                    if (p < packets)
+                        atomicMax(&group_max[g], largest<N>(y));
+                    __syncthreads();
+                    most = group_max[g];
+                    __syncthreads();
+                }
+                if (p < packets) {
+                    const float scale = scale_of(most);
+                    if (a.group == 0 ? p == 0 : p * N % a.group == 0)
+                        a.scales[r * a.scales_ld + (a.group == 0 ? 0 : p * N / a.group)] = scale;
+                    store_q8<N>(a.res, r * a.res_ld, p, a.cols, y, 1.0f / scale);
+                }
+            }
+        }
+    }
+}
+
+template <typename T> struct NormGradArgs { // dx may be the same matrix as grad, sum or dsum
+    const T *grad, *sum, *weight, *dsum;
+    const wide_t<T> *rstd;
+    T *dx;
+    wide_t<T> *part; // CTAs x part_ld column sums, or null
+    int64_t rows, cols, grad_ld, sum_ld, dsum_ld, dx_ld, part_ld;
+};
+
+// dx of the rows, and the CTA's column sums of dy * s * rstd: a thread keeps the sums of its columns in registers over
+// all rows that the CTA visits; the rows that a CTA holds at once are joined through shared memory in order.
+template <typename T, int N, int PPT, int BLOCK>
+__global__ void __launch_bounds__(BLOCK) norm_grad_rows_kernel(NormGradArgs<T> a, int log_tpr) {
+    using W = wide_t<T>;
+    __shared__ W red[2 * (BLOCK / 32)];
+    __shared__ W join[BLOCK * N];
+    const int tpr = 1 << log_tpr, tx = threadIdx.x & (tpr - 1), ty = threadIdx.x >> log_tpr, at_once = BLOCK >> log_tpr;
+    const int64_t packets = (a.cols + N - 1) / N;
+    RowSum<W, BLOCK> row_sum{red};
+    W dw[PPT][N];
+#pragma unroll
+    for (int k = 0; k < PPT; k++)
+#pragma unroll
+        for (int j = 0; j < N; j++)
+            dw[k][j] = 0;
+    for (int64_t r0 = (int64_t)blockIdx.x * at_once; r0 < a.rows; r0 += (int64_t)gridDim.x * at_once) {
+        const int64_t r = r0 + ty;
+        const bool live = r < a.rows;
+        Vec<T, N> g[PPT], s[PPT], d[PPT];
+        W rstd = 0;
+        if (live) {
+#pragma unroll
+            for (int k = 0; k < PPT; k++)
+                if (tx + k * tpr < packets) {
+                    g[k] = load_packet<T, N>(a.grad + r * a.grad_ld, tx + k * tpr, a.cols);
+                    s[k] = load_packet<T, N>(a.sum + r * a.sum_ld, tx + k * tpr, a.cols);
+                    if (a.dsum)
+                        d[k] = load_packet<T, N>(a.dsum + r * a.dsum_ld, tx + k * tpr, a.cols);
+                }
+            rstd = a.rstd[r];
+        }
+        W dot = 0;
+#pragma unroll
+        for (int k = 0; k < PPT; k++)
+            if (live && tx + k * tpr < packets) {
+                Vec<T, N> w;
+                if (a.weight)
+                    w = load_packet<T, N>(a.weight, tx + k * tpr, a.cols);
+#pragma unroll
+                for (int j = 0; j < N; j++) {
+                    const W t = a.weight ? widen(g[k].v[j]) * widen(w.v[j]) : W(widen(g[k].v[j]));
+                    dot += t * widen(s[k].v[j]);
+                    dw[k][j] += widen(g[k].v[j]) * (widen(s[k].v[j]) * rstd);
+                }
+            }
+        const W factor = row_sum(dot, tpr) / W(a.cols) * rstd * rstd;
+        if (live) {
+#pragma unroll
+            for (int k = 0; k < PPT; k++)
+                if (tx + k * tpr < packets) {
+                    Vec<T, N> w, z;
+                    if (a.weight)
+                        w = load_packet<T, N>(a.weight, tx + k * tpr, a.cols);
+#pragma unroll
+                    for (int j = 0; j < N; j++) {
+                        const W t = a.weight ? widen(g[k].v[j]) * widen(w.v[j]) : W(widen(g[k].v[j]));
+                        W v = rstd * (t - widen(s[k].v[j]) * factor);
+                        if (a.dsum)
+                            v += widen(d[k].v[j]);
+                        z.v[j] = narrow<T>(v);
+                    }
+                    store_packet<T, N>(a.dx + r * a.dx_ld, tx + k * tpr, a.cols, z);
+                }
+        }
+    }
+    if (!a.part)
+        return;
+#pragma unroll
+    for (int k = 0; k < PPT; k++) {
+#pragma unroll
+        for (int j = 0; j < N; j++)
+            join[threadIdx.x * N + j] = dw[k][j];
+        __syncthreads();
+        if (ty == 0 && tx + k * tpr < packets) {
+#pragma unroll
+            for (int j = 0; j < N; j++) {
+                W v = join[tx * N + j];
+                for (int i = 1; i < at_once; i++)
+                    v += join[(i * tpr + tx) * N + j];
+                const int64_t c = (int64_t)(tx + k * tpr) * N + j;
+                if (c < a.cols)
+                    a.part[(int64_t)blockIdx.x * a.part_ld + c] = v;
+            }
+        }
+        __syncthreads();
+    }
+}
+
+template <typename T, int N>
+__global__ void __launch_bounds__(LONG_BLOCK) norm_grad_long_kernel(NormGradArgs<T> a) {
+    using W = wide_t<T>;
+    __shared__ W red[2 * (LONG_BLOCK / 32)];
+    const int64_t packets = (a.cols + N - 1) / N;
+    RowSum<W, LONG_BLOCK> row_sum{red};
+    for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
+        const T *g = a.grad + r * a.grad_ld, *s = a.sum + r * a.sum_ld;
+        const W rstd = a.rstd[r];
+        W dot = 0;
+        for (int64_t p = threadIdx.x; p < packets; p += LONG_BLOCK) {
+            const Vec<T, N> gv = load_packet<T, N>(g, p, a.cols), sv = load_packet<T, N>(s, p, a.cols);
+            Vec<T, N> w;
+            if (a.weight)
+                w = load_packet<T, N>(a.weight, p, a.cols);
+#pragma unroll
+            for (int j = 0; j < N; j++)
+                dot += (a.weight ? widen(gv.v[j]) * widen(w.v[j]) : W(widen(gv.v[j]))) * widen(sv.v[j]);
+        }
+        const W factor = row_sum(dot, LONG_BLOCK) / W(a.cols) * rstd * rstd;
+        for (int64_t p = threadIdx.x; p < packets; p += LONG_BLOCK) {
+            const Vec<T, N> gv = load_packet<T, N>(g, p, a.cols), sv = load_packet<T, N>(s, p, a.cols);
+            Vec<T, N> w, d, z;
+            if (a.weight)
+                w = load_packet<T, N>(a.weight, p, a.cols);
+            if (a.dsum)
+                d = load_packet<T, N>(a.dsum + r * a.dsum_ld, p, a.cols);
+#pragma unroll
+            for (int j = 0; j < N; j++) {
+                W v = rstd * ((a.weight ? widen(gv.v[j]) * widen(w.v[j]) : W(widen(gv.v[j]))) - widen(sv.v[j]) * factor);
+                if (a.dsum)
+                    v += widen(d.v[j]);
+                z.v[j] = narrow<T>(v);
+            }
+            store_packet<T, N>(a.dx + r * a.dx_ld, p, a.cols, z);
+        }
+    }
+}
+
+// column sums of dy * s * rstd for the long rows: CTA (x, y) takes 32 columns and every gridDim.y-th group of 8 rows
+// (launched before dx is written, which may be the same matrix as grad or sum)
+template <typename T> __global__ void __launch_bounds__(256) norm_dweight_kernel(NormGradArgs<T> a) {
+    using W = wide_t<T>;
+    __shared__ W sums[8][33];
+    const int tx = threadIdx.x % 32, ty = threadIdx.x / 32;
+    const int64_t c = (int64_t)blockIdx.x * 32 + tx;
+    W v = 0;
+    if (c < a.cols)
+        for (int64_t r = (int64_t)blockIdx.y * 8 + ty; r < a.rows; r += (int64_t)gridDim.y * 8)
+            v += widen(a.grad[r * a.grad_ld + c]) * (widen(a.sum[r * a.sum_ld + c]) * a.rstd[r]);
+    sums[ty][tx] = v;
+    __syncthreads();
+    if (ty == 0 && c < a.cols) {
+        for (int k = 1; k < 8; k++)
+            v += sums[k][tx];
+        a.part[(int64_t)blockIdx.y * a.part_ld + c] = v;
+    }
+}
+
+// dweight[c] = sum over the parts, in order within eight shares and over the shares
+template <typename W>
+__global__ void __launch_bounds__(256)
+    norm_join_kernel(const W *__restrict__ part, int parts, int64_t cols, int64_t part_ld, W *__restrict__ res) {
+    __shared__ W sums[8][33];
+    const int tx = threadIdx.x % 32, ty = threadIdx.x / 32;
+    const int64_t c = (int64_t)blockIdx.x * 32 + tx;
+    const int share = (parts + 7) / 8, first = ty * share, last = first + share < parts ? first + share : parts;
+    W v = 0;
+    if (c < cols) {
+#pragma unroll 8
+        for (int i = first; i < last; i++)
+            v += part[(int64_t)i * part_ld + c];
+    }
+    sums[ty][tx] = v;
+    __syncthreads();
+    if (ty == 0 && c < cols) {
+        for (int k = 1; k < 8; k++)
+            v += sums[k][tx];
+        res[c] = v;
+    }
+}
+
+// How many threads share a row and how many packets each holds.  Many rows: as few threads as hold the row in `most`
+// packets each, since every thread then has more loads in flight; few rows (fewer than SMs): one packet each, which
+// shortens the way of the single row.
+struct RowPlan {
+    int log_tpr, ppt;
+    bool fits;
+};
+RowPlan row_plan(int64_t packets, int64_t rows, int most, int max_log) {
+    const int64_t want = rows < sm_count() ? packets : (packets + most - 1) / most;
+    RowPlan p{3, 1, true};
+    while (p.log_tpr < max_log && ((int64_t)1 << p.log_tpr) < want)
+        p.log_tpr++;
+    while (p.ppt < most && ((int64_t)p.ppt << p.log_tpr) < packets)
+        p.ppt *= 2;
+    p.fits = ((int64_t)p.ppt << p.log_tpr) >= packets;
+    return p;
+}
+
+template <typename T, int N, bool Q8> int norm_launch(const NormArgs<T> &a, cudaStream_t st) {
+    constexpr int MOST = N == 1 ? 8 : 4;
+    const RowPlan p = row_plan((a.cols + N - 1) / N, a.rows, MOST, 10);
+    const int64_t max_grid = (int64_t)1 << 30;
+    if (!p.fits) {
+        norm_long_kernel<T, N, Q8><<<(unsigned)(a.rows < max_grid ? a.rows : max_grid), LONG_BLOCK, 0, st>>>(a);
+        return after_launch("norm_long_kernel");
+    }
+    const int block = p.log_tpr > 8 ? 1 << p.log_tpr : 256, at_once = block >> p.log_tpr;
+    const int64_t blocks = (a.rows + at_once - 1) / at_once;
+    const unsigned grid = (unsigned)(blocks < max_grid ? blocks : max_grid);
+    const size_t smem = Q8 ? (size_t)at_once * a.groups * sizeof(unsigned) : 0;
+#define DB2_NORM(PPT, BLOCK) norm_rows_kernel<T, N, PPT, Q8, BLOCK><<<grid, BLOCK, smem, st>>>(a, p.log_tpr)
+#define DB2_NORM_PPT(BLOCK)                                                                                            \
+    switch (p.ppt) {                                                                                                   \
+    case 1: DB2_NORM(1, BLOCK); break;                                                                                 \
+    case 2: DB2_NORM(2, BLOCK); break;                                                                                 \
+    case 4: DB2_NORM(4, BLOCK); break;                                                                                 \
+    default: DB2_NORM(MOST, BLOCK); break;                                                                             \
+    }
+    if (block == 256)
+        DB2_NORM_PPT(256)
+    else if (block == 512)
+        DB2_NORM_PPT(512)
+    else
+        DB2_NORM_PPT(1024)
+#undef DB2_NORM_PPT
+#undef DB2_NORM
+    return after_launch("norm_rows_kernel");
+}
+
+// CTAs of the gradient kernel: each keeps its own column sums
+int64_t grad_ctas(int64_t rows) {
+    const int64_t cap = (int64_t)sm_count() * 4;
+    return rows < 1 ? 1 : (rows < cap ? rows : cap);
+}
+
+template <typename T, int N> int norm_grad_launch(NormGradArgs<T> a, wide_t<T> *dweight, cudaStream_t st) {
+    constexpr int MOST = N == 1 ? 8 : 4;
+    const RowPlan p = row_plan((a.cols + N - 1) / N, a.rows, MOST, 9); // 512 threads: 128 registers each
+    const int64_t ctas = grad_ctas(a.rows);
+    int parts;
+    if (!p.fits) {
+        parts = (int)(ctas < 16 ? ctas : 16);
+        if (a.part) {
+            norm_dweight_kernel<T><<<dim3((unsigned)((a.cols + 31) / 32), (unsigned)parts), 256, 0, st>>>(a);
+            DB2_TRY(after_launch("norm_dweight_kernel"));
+        }
+        norm_grad_long_kernel<T, N><<<(unsigned)ctas, LONG_BLOCK, 0, st>>>(a);
+        DB2_TRY(after_launch("norm_grad_long_kernel"));
+    } else {
+        const int block = p.log_tpr > 8 ? 512 : 256, at_once = block >> p.log_tpr;
+        const int64_t blocks = (a.rows + at_once - 1) / at_once;
+        parts = (int)(blocks < ctas ? blocks : ctas);
+#define DB2_NORM_GRAD(PPT, BLOCK) norm_grad_rows_kernel<T, N, PPT, BLOCK><<<parts, BLOCK, 0, st>>>(a, p.log_tpr)
+#define DB2_NORM_GRAD_PPT(BLOCK)                                                                                       \
+    switch (p.ppt) {                                                                                                   \
+    case 1: DB2_NORM_GRAD(1, BLOCK); break;                                                                            \
+    case 2: DB2_NORM_GRAD(2, BLOCK); break;                                                                            \
+    case 4: DB2_NORM_GRAD(4, BLOCK); break;                                                                            \
+    default: DB2_NORM_GRAD(MOST, BLOCK); break;                                                                        \
+    }
+        if (block == 256)
+            DB2_NORM_GRAD_PPT(256)
+        else
+            DB2_NORM_GRAD_PPT(512)
+#undef DB2_NORM_GRAD_PPT
+#undef DB2_NORM_GRAD
+        DB2_TRY(after_launch("norm_grad_rows_kernel"));
+    }
+    if (a.part) {
+        norm_join_kernel<wide_t<T>><<<(unsigned)((a.cols + 31) / 32), 256, 0, st>>>(a.part, parts, a.cols, a.part_ld,
+                                                                                   dweight);
+        DB2_TRY(after_launch("norm_join_kernel"));
+    }
+    return DB2_OK;
+}
+
+int64_t part_ld_of(int64_t cols) { return (cols + 7) / 8 * 8; }
+
+bool seq_type(int dtype) {
+    return dtype == DB2_F64 || dtype == DB2_F32 || dtype == DB2_F16 || dtype == DB2_BF16;
+}
+
+// the arguments that both forms of the norm share
+int check_norm(const char *what, const void *x, int64_t rows, int64_t cols, int64_t x_ld, const void *residual,
+               int64_t residual_ld, double eps, const void *sum, int64_t sum_ld, const void *res, int64_t res_ld) {
+    DB2_CHECK(eps >= 0.0, DB2_EINVAL, "%s: eps must not be negative", what);
+    DB2_CHECK(cols > 0, DB2_EINVAL, "%s: rows without columns have no mean", what);
+    DB2_CHECK(x && res, DB2_EINVAL, "%s: null operand", what);
+    DB2_CHECK(ld_ok(x_ld, rows, cols) && (!residual || ld_ok(residual_ld, rows, cols)) &&
+                  (!sum || ld_ok(sum_ld, rows, cols)) && ld_ok(res_ld, rows, cols),
+              DB2_EINVAL, "%s: a leading dimension is smaller than the number of columns", what);
+    return DB2_OK;
+}
+
+void count(db2_context *ctx, uint64_t before) {
+    std::lock_guard<std::mutex> lock(ctx->mu);
+    ctx->stats.launches += g_launches.load(std::memory_order_relaxed) - before;
+}
+
+// checks of the handle forms that compare matrices with one another
+int check_operands(const char *what, const db2_matrix *x, const db2_matrix *other, const char *name) {
+    DB2_CHECK(!other || (other->dtype == x->dtype && other->rows == x->rows && other->cols == x->cols), DB2_EINVAL,
+              "%s: %s must have the shape and value type of the first argument", what, name);
+    return DB2_OK;
+}
+int check_weight(const char *what, const db2_matrix *x, const db2_matrix *weight) {
+    DB2_CHECK(!weight || (weight->dtype == x->dtype && weight->rows == 1 && weight->cols == x->cols), DB2_EINVAL,
+              "%s: weight must be a row matrix of %lld columns and of the same value type", what, (long long)x->cols);
+    return DB2_OK;
+}
+int wide_dtype(int dtype) { return dtype == DB2_F64 ? DB2_F64 : DB2_F32; }
+
+// rmsNorm (scales == nullptr) and rmsNormQ8 on handles
+int norm_on_handles(db2_context *ctx, const char *what, db2_matrix **res, db2_matrix **scales, db2_matrix **sum,
+                    db2_matrix **rstd, db2_matrix *x, db2_matrix *residual, db2_matrix *weight, double eps,
+                    int64_t group) {
+    DB2_CHECK(seq_type(x->dtype) && (!scales || x->dtype != DB2_F64), DB2_EUNSUPPORTED,
+              "%s: unsupported value type code %d", what, x->dtype);
+    DB2_CHECK(eps >= 0.0, DB2_EINVAL, "%s: eps must not be negative", what);
+    DB2_CHECK(x->cols > 0 || x->rows == 0, DB2_EINVAL, "%s: rows without columns have no mean", what);
+    DB2_TRY(check_operands(what, x, residual, "residual"));
+    DB2_TRY(check_weight(what, x, weight));
+    db2_matrix *slots[4] = {*res, scales ? *scales : nullptr, sum ? *sum : nullptr, rstd ? *rstd : nullptr};
+    for (int i = 0; i < 4; i++)
+        for (int j = 0; j < i; j++)
+            DB2_CHECK(!slots[i] || slots[i] != slots[j], DB2_EINVAL, "%s: two results are to go to one matrix", what);
+    DB2_CHECK(!scales || group == 0 || (group >= 16 && group <= 512 && (group & (group - 1)) == 0), DB2_EINVAL,
+              "%s: groups of 16, 32, 64, 128, 256 or 512 columns, or 0 for the whole row (got %lld)", what,
+              (long long)group);
+    bind_device(ctx);
+    const uint64_t before = g_launches.load();
+    const DeviceOperand dx(x), dres(residual), dw(weight);
+    DB2_TRY(prepare_result(ctx, res, scales ? DB2_F8E4M3 : x->dtype, x->rows, x->cols));
+    if (scales)
+        DB2_TRY(prepare_result(ctx, scales, DB2_F32, x->rows, group ? (x->cols + group - 1) / group : 1));
+    if (sum)
+        DB2_TRY(prepare_result(ctx, sum, x->dtype, x->rows, x->cols));
+    if (rstd) {
+        DB2_TRY(prepare_result(ctx, rstd, wide_dtype(x->dtype), x->rows, 1));
+        DB2_CHECK((*rstd)->dev_ld == 1 || x->rows <= 1, DB2_EUNSUPPORTED, "%s: rstd into a strided result view", what);
+    }
+    if (x->rows > 0) {
+        void *sp = sum ? (*sum)->dev_ptr() : nullptr, *tp = rstd ? (*rstd)->dev_ptr() : nullptr;
+        const int64_t sld = sum ? (*sum)->dev_ld : 0;
+        if (scales)
+            DB2_TRY(db2k_rms_norm_q8(x->dtype, dx.ptr, x->rows, x->cols, dx.ld, dres.ptr, dres.ld, dw.ptr, eps, sp, sld,
+                                     (*res)->dev_ptr(), (*res)->dev_ld, (*scales)->dev_ptr(), (*scales)->dev_ld, group,
+                                     tp, ctx->stream));
+        else
+            DB2_TRY(db2k_rms_norm(x->dtype, dx.ptr, x->rows, x->cols, dx.ld, dres.ptr, dres.ld, dw.ptr, eps, sp, sld,
+                                  (*res)->dev_ptr(), (*res)->dev_ld, tp, ctx->stream));
+    }
+    count(ctx, before);
+    return DB2_OK;
+}
+
+} // namespace
+} // namespace db2
+
+using namespace db2;
+
+extern "C" {
+
+int db2k_rms_norm(int dtype, const void *x, int64_t rows, int64_t cols, int64_t x_ld, const void *residual,
+                  int64_t residual_ld, const void *weight, double eps, void *sum, int64_t sum_ld, void *res,
+                  int64_t res_ld, void *rstd, void *stream) {
+    DB2_CHECK(seq_type(dtype), DB2_EUNSUPPORTED, "rmsNorm: unsupported value type code %d", dtype);
+    DB2_CHECK(rows >= 0 && cols >= 0, DB2_EINVAL, "rmsNorm: negative shape");
+    if (rows == 0)
+        return DB2_OK;
+    DB2_TRY(check_norm("rmsNorm", x, rows, cols, x_ld, residual, residual_ld, eps, sum, sum_ld, res, res_ld));
+    DB2_DISPATCH_SEQ(dtype, T, {
+        constexpr int N = 16 / sizeof(T);
+        NormArgs<T> a{static_cast<const T *>(x), static_cast<const T *>(residual), static_cast<const T *>(weight),
+                      static_cast<T *>(sum), res, nullptr, static_cast<wide_t<T> *>(rstd), rows, cols, x_ld,
+                      residual_ld, sum_ld, res_ld, 0, 0, 0, (wide_t<T>)eps};
+        const bool packed = rows_aligned(x, x_ld, sizeof(T), 16) && rows_aligned(residual, residual_ld, sizeof(T), 16) &&
+                            rows_aligned(weight, 0, sizeof(T), 16) && rows_aligned(sum, sum_ld, sizeof(T), 16) &&
+                            rows_aligned(res, res_ld, sizeof(T), 16);
+        return packed ? norm_launch<T, N, false>(a, as_stream(stream)) : norm_launch<T, 1, false>(a, as_stream(stream));
+    });
+    return DB2_OK;
+}
+
+int db2k_rms_norm_q8(int dtype, const void *x, int64_t rows, int64_t cols, int64_t x_ld, const void *residual,
+                     int64_t residual_ld, const void *weight, double eps, void *sum, int64_t sum_ld, void *res,
+                     int64_t res_ld, void *scales, int64_t scales_ld, int64_t group, void *rstd, void *stream) {
+    DB2_CHECK(seq_type(dtype) && dtype != DB2_F64, DB2_EUNSUPPORTED, "rmsNormQ8: unsupported value type code %d", dtype);
+    DB2_CHECK(rows >= 0 && cols >= 0, DB2_EINVAL, "rmsNormQ8: negative shape");
+    DB2_CHECK(group == 0 || (group >= 16 && group <= 512 && (group & (group - 1)) == 0), DB2_EINVAL,
+              "rmsNormQ8: groups of 16, 32, 64, 128, 256 or 512 columns, or 0 for the whole row (got %lld)",
+              (long long)group);
+    if (rows == 0)
+        return DB2_OK;
+    DB2_TRY(check_norm("rmsNormQ8", x, rows, cols, x_ld, residual, residual_ld, eps, sum, sum_ld, res, res_ld));
+    const int64_t groups = group ? (cols + group - 1) / group : 1;
+    DB2_CHECK(scales && ld_ok(scales_ld, rows, groups), DB2_EINVAL,
+              "rmsNormQ8: null scales or their leading dimension smaller than the number of groups");
+    auto go = [&](auto tag) {
+        using T = decltype(tag);
+        constexpr int N = 16 / sizeof(T);
+        NormArgs<T> a{static_cast<const T *>(x), static_cast<const T *>(residual), static_cast<const T *>(weight),
+                      static_cast<T *>(sum), res, static_cast<float *>(scales), static_cast<float *>(rstd), rows, cols,
+                      x_ld, residual_ld, sum_ld, res_ld, scales_ld, group, groups, (float)eps};
+        const bool packed = rows_aligned(x, x_ld, sizeof(T), 16) && rows_aligned(residual, residual_ld, sizeof(T), 16) &&
+                            rows_aligned(weight, 0, sizeof(T), 16) && rows_aligned(sum, sum_ld, sizeof(T), 16) &&
+                            rows_aligned(res, res_ld, 1, N);
+        return packed ? norm_launch<T, N, true>(a, as_stream(stream)) : norm_launch<T, 1, true>(a, as_stream(stream));
+    };
+    return dtype == DB2_F32 ? go(float()) : dtype == DB2_F16 ? go(__half()) : go(__nv_bfloat16());
+}
+
+size_t db2k_rms_norm_grad_scratch_bytes(int dtype, int64_t rows, int64_t cols) {
+    if (rows <= 0 || cols <= 0)
+        return 0;
+    return (size_t)grad_ctas(rows) * part_ld_of(cols) * (dtype == DB2_F64 ? 8 : 4);
+}
+
+int db2k_rms_norm_grad(int dtype, const void *grad, int64_t grad_ld, int64_t rows, int64_t cols, const void *sum,
+                       int64_t sum_ld, const void *weight, const void *rstd, const void *dsum, int64_t dsum_ld, void *dx,
+                       int64_t dx_ld, void *dweight, void *scratch, size_t scratch_bytes, void *stream) {
+    DB2_CHECK(seq_type(dtype), DB2_EUNSUPPORTED, "rmsNormGrad: unsupported value type code %d", dtype);
+    DB2_CHECK(rows >= 0 && cols >= 0, DB2_EINVAL, "rmsNormGrad: negative shape");
+    if (cols == 0)
+        return DB2_OK;
+    if (rows == 0) {
+        if (dweight)
+            DB2_CUDA(cudaMemsetAsync(dweight, 0, (size_t)cols * (dtype == DB2_F64 ? 8 : 4), as_stream(stream)));
+        return DB2_OK;
+    }
+    DB2_CHECK(grad && sum && rstd && dx, DB2_EINVAL, "rmsNormGrad: null operand");
+    DB2_CHECK(ld_ok(grad_ld, rows, cols) && ld_ok(sum_ld, rows, cols) && (!dsum || ld_ok(dsum_ld, rows, cols)) &&
+                  ld_ok(dx_ld, rows, cols),
+              DB2_EINVAL, "rmsNormGrad: a leading dimension is smaller than the number of columns");
+    DB2_CHECK(!dweight || (scratch && scratch_bytes >= db2k_rms_norm_grad_scratch_bytes(dtype, rows, cols) &&
+                           aligned16(scratch)),
+              DB2_EINVAL, "rmsNormGrad: scratch smaller than db2k_rms_norm_grad_scratch_bytes, or not 16-byte aligned");
+    DB2_DISPATCH_SEQ(dtype, T, {
+        constexpr int N = 16 / sizeof(T);
+        NormGradArgs<T> a{static_cast<const T *>(grad), static_cast<const T *>(sum), static_cast<const T *>(weight),
+                          static_cast<const T *>(dsum), static_cast<const wide_t<T> *>(rstd), static_cast<T *>(dx),
+                          dweight ? static_cast<wide_t<T> *>(scratch) : nullptr, rows, cols, grad_ld, sum_ld, dsum_ld,
+                          dx_ld, part_ld_of(cols)};
+        const bool packed = rows_aligned(grad, grad_ld, sizeof(T), 16) && rows_aligned(sum, sum_ld, sizeof(T), 16) &&
+                            rows_aligned(weight, 0, sizeof(T), 16) && rows_aligned(dsum, dsum_ld, sizeof(T), 16) &&
+                            rows_aligned(dx, dx_ld, sizeof(T), 16);
+        wide_t<T> *dw = static_cast<wide_t<T> *>(dweight);
+        return packed ? norm_grad_launch<T, N>(a, dw, as_stream(stream)) : norm_grad_launch<T, 1>(a, dw, as_stream(stream));
+    });
+    return DB2_OK;
+}
+
+int db2_rmsNorm(db2_context *ctx, db2_matrix **res, db2_matrix **sum, db2_matrix **rstd, db2_matrix *x,
+                db2_matrix *residual, db2_matrix *weight, double eps) {
+    DB2_API_BEGIN
+    DB2_CHECK(ctx && res && x, DB2_EINVAL, "null argument");
+    return norm_on_handles(ctx, "rmsNorm", res, nullptr, sum, rstd, x, residual, weight, eps, 0);
+    DB2_API_END
+}
+
+int db2_rmsNormQ8(db2_context *ctx, db2_matrix **res, db2_matrix **scales, db2_matrix **sum, db2_matrix **rstd,
+                  db2_matrix *x, db2_matrix *residual, db2_matrix *weight, double eps, int64_t group) {
+    DB2_API_BEGIN
+    DB2_CHECK(ctx && res && scales && x, DB2_EINVAL, "null argument");
+    return norm_on_handles(ctx, "rmsNormQ8", res, scales, sum, rstd, x, residual, weight, eps, group);
+    DB2_API_END
+}
+
+int db2_rmsNormGrad(db2_context *ctx, db2_matrix **dx, db2_matrix **dweight, db2_matrix *grad, db2_matrix *sum,
+                    db2_matrix *weight, db2_matrix *rstd, db2_matrix *dsum) {
+    DB2_API_BEGIN
+    DB2_CHECK(ctx && dx && grad && sum && rstd, DB2_EINVAL, "null argument");
+    DB2_CHECK(seq_type(grad->dtype), DB2_EUNSUPPORTED, "rmsNormGrad: unsupported value type code %d", grad->dtype);
+    DB2_TRY(check_operands("rmsNormGrad", grad, sum, "sum"));
+    DB2_TRY(check_operands("rmsNormGrad", grad, dsum, "dsum"));
+    DB2_TRY(check_weight("rmsNormGrad", grad, weight));
+    DB2_CHECK(rstd->dtype == wide_dtype(grad->dtype) && rstd->rows == grad->rows && rstd->cols == 1, DB2_EINVAL,
+              "rmsNormGrad: rstd must be the column matrix that rmsNorm gave");
+    DB2_CHECK(!dweight || !*dweight || *dweight != *dx, DB2_EINVAL,
+              "rmsNormGrad: two results are to go to one matrix");
+    bind_device(ctx);
+    const uint64_t before = g_launches.load();
+    const DeviceOperand dg(grad), ds(sum), dw(weight), dr(rstd), dd(dsum);
+    DB2_CHECK(dr.ld == 1 || grad->rows <= 1, DB2_EUNSUPPORTED, "rmsNormGrad: rstd is a strided view");
+    DB2_TRY(prepare_result(ctx, dx, grad->dtype, grad->rows, grad->cols));
+    if (dweight)
+        DB2_TRY(prepare_result(ctx, dweight, wide_dtype(grad->dtype), 1, grad->cols));
+    const size_t sb = db2k_rms_norm_grad_scratch_bytes(grad->dtype, grad->rows, grad->cols);
+    void *scratch = nullptr;
+    DB2_TRY(ctx_scratch(ctx, sb, &scratch));
+    DB2_TRY(db2k_rms_norm_grad(grad->dtype, dg.ptr, dg.ld, grad->rows, grad->cols, ds.ptr, ds.ld, dw.ptr, dr.ptr, dd.ptr,
+                               dd.ld, (*dx)->dev_ptr(), (*dx)->dev_ld, dweight ? (*dweight)->dev_ptr() : nullptr,
+                               scratch, ctx->scratch_bytes, ctx->stream));
+    count(ctx, before);
+    return DB2_OK;
+    DB2_API_END
+}
+
+} // extern "C"

@@ -274,6 +274,14 @@ int nccl_allreduce_group(const std::vector<db2_context *> &ctxs, const std::vect
 int ensure_device(db2_matrix *m);
 // result allocation following the reference's "*res == nullptr means allocate" convention; checks shape/type otherwise
 int prepare_result(db2_context *ctx, db2_matrix **res, int dtype, int64_t rows, int64_t cols);
+// A device-resident operand (or none, for a null handle) that keeps its buffer: a result that is prepared afterwards and
+// names the same matrix gets a buffer of its own instead of the operand's values.  Views are written in place.
+struct DeviceOperand {
+    std::shared_ptr<DevBuf> keep;
+    const void *ptr = nullptr;
+    int64_t ld = 0;
+    explicit DeviceOperand(db2_matrix *m); // throws Error (embed.cu)
+};
 // makes m the target of an update in place: current on the device, in a buffer that no other handle reads (embed.cu)
 int prepare_update(db2_matrix *m);
 } // namespace db2

@@ -471,6 +471,43 @@ def embedGrad(grad: DenseMatrix, tokens: DenseMatrix, vocab: int, scale: float =
     return _res(ctx, h)
 
 
+def _handle(m: Optional[DenseMatrix]):
+    return m.handle if m is not None else None
+
+
+def rmsNorm(x: DenseMatrix, weight: Optional[DenseMatrix] = None, eps: float = 1e-6,
+            residual: Optional[DenseMatrix] = None, ctx: Optional[Context] = None):
+    """Rows of s = x + residual divided by their root mean square, times the row matrix `weight`: (result, s, rstd);
+    s is x itself without a residual, rstd (rows x 1) is what rmsNormGrad asks for."""
+    ctx = ctx or x.ctx
+    y, s, rstd = C.c_void_p(), C.c_void_p(), C.c_void_p()
+    check(lib.db2_rmsNorm(ctx.handle, C.byref(y), C.byref(s) if residual is not None else None, C.byref(rstd), x.handle,
+                          _handle(residual), _handle(weight), float(eps)))
+    return _res(ctx, y), (_res(ctx, s) if residual is not None else x), _res(ctx, rstd)
+
+
+def rmsNormQ8(x: DenseMatrix, weight: Optional[DenseMatrix] = None, eps: float = 1e-6,
+              residual: Optional[DenseMatrix] = None, group: int = 0, ctx: Optional[Context] = None):
+    """rmsNorm with a result in 8 bits (FLOAT8_E4M3) and one float scale per row and `group` columns (0: per row):
+    (result, scales, s, rstd)."""
+    ctx = ctx or x.ctx
+    y, sc, s, rstd = C.c_void_p(), C.c_void_p(), C.c_void_p(), C.c_void_p()
+    check(lib.db2_rmsNormQ8(ctx.handle, C.byref(y), C.byref(sc), C.byref(s) if residual is not None else None,
+                            C.byref(rstd), x.handle, _handle(residual), _handle(weight), float(eps), int(group)))
+    return _res(ctx, y), _res(ctx, sc), (_res(ctx, s) if residual is not None else x), _res(ctx, rstd)
+
+
+def rmsNormGrad(grad: DenseMatrix, s: DenseMatrix, rstd: DenseMatrix, weight: Optional[DenseMatrix] = None,
+                dsum: Optional[DenseMatrix] = None, ctx: Optional[Context] = None):
+    """(gradient of x and of the residual, gradient of the weight) from the s and rstd of rmsNorm; `dsum` is the gradient
+    that reaches s directly."""
+    ctx = ctx or grad.ctx
+    dx, dw = C.c_void_p(), C.c_void_p()
+    check(lib.db2_rmsNormGrad(ctx.handle, C.byref(dx), C.byref(dw), grad.handle, s.handle, _handle(weight), rstd.handle,
+                              _handle(dsum)))
+    return _res(ctx, dx), _res(ctx, dw)
+
+
 class CSRMatrix:
     """Handle to a db2_csr.  The host arrays follow the reference's CSRMatrix layout (values, colIdxs and rowOffsets
     with 64-bit indices)."""

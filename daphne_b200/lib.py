@@ -96,6 +96,10 @@ _SIGS = {
     "db2k_embed_grad_scratch_bytes": (sz, [i32, i64, i64, i64]),
     "db2k_embed_grad": (i32, [i32, vp, i64, i64, i64, i32, vp, i64, C.c_double, i32, vp, i64, i64, i32, vp, sz, vp,
                               vp]),
+    "db2k_rms_norm": (i32, [i32, vp, i64, i64, i64, vp, i64, vp, C.c_double, vp, i64, vp, i64, vp, vp]),
+    "db2k_rms_norm_q8": (i32, [i32, vp, i64, i64, i64, vp, i64, vp, C.c_double, vp, i64, vp, i64, vp, i64, i64, vp, vp]),
+    "db2k_rms_norm_grad_scratch_bytes": (sz, [i32, i64, i64]),
+    "db2k_rms_norm_grad": (i32, [i32, vp, i64, i64, i64, vp, i64, vp, vp, vp, i64, vp, i64, vp, vp, sz, vp]),
     # runtime
     "db2_context_create": (i32, [i32, _P(vp)]),
     "db2_context_destroy": (i32, [vp]),
@@ -184,6 +188,9 @@ _SIGS = {
     "db2_castObj": (i32, [vp, _P(vp), vp, i32]),
     "db2_embed": (i32, [vp, _P(vp), vp, vp, C.c_double]),
     "db2_embedGrad": (i32, [vp, _P(vp), vp, vp, i64, C.c_double, i32, i32]),
+    "db2_rmsNorm": (i32, [vp, _P(vp), _P(vp), _P(vp), vp, vp, vp, C.c_double]),
+    "db2_rmsNormQ8": (i32, [vp, _P(vp), _P(vp), _P(vp), _P(vp), vp, vp, vp, C.c_double, i64]),
+    "db2_rmsNormGrad": (i32, [vp, _P(vp), _P(vp), vp, vp, vp, vp, vp]),
     "db2_readDaphne": (i32, [vp, _P(vp), C.c_char_p]),
     "db2_writeDaphne": (i32, [vp, vp, C.c_char_p]),
     "db2_vectorizedPipeline": (i32, [vp, _P(vp), sz, _P(i32), _P(vp), sz, _P(i64), _P(i64), _P(i64), _P(i64), vp, i64]),

@@ -281,6 +281,30 @@ int db2k_embed_grad(int dtype, const void *grad, int64_t grad_ld, int64_t n, int
                     int64_t res_ld, int accumulate, void *scratch, size_t scratch_bytes, int32_t *dev_status,
                     void *stream);
 
+/* Root-mean-square norm of the rows: s = x + residual, rounded to dtype (s = x without a residual);
+ * rstd = 1 / sqrt(mean(s^2) + eps); res = s * rstd * weight.  residual, weight (cols contiguous values of dtype; NULL
+ * stands for ones), sum (receives s) and rstd (receives rows contiguous wide values) may be NULL.  sum may be x or
+ * residual itself, and res may be x or residual itself (same pointer and leading dimension); no other overlap. */
+int db2k_rms_norm(int dtype, const void *x, int64_t rows, int64_t cols, int64_t x_ld, const void *residual,
+                  int64_t residual_ld, const void *weight, double eps, void *sum, int64_t sum_ld, void *res,
+                  int64_t res_ld, void *rstd, void *stream);
+/* The same with an 8-bit result (DB2_F8E4M3): per row and group of `group` columns (16, 32, ..., 512; 0: the whole row;
+ * the last group may be narrower) scale = max|y| / 448 and res = y / scale, rounded to nearest; scale is 1 where all y
+ * are zero and never below the smallest normal float.  scales: rows x ceil(cols / group) floats (rows x 1 for group 0).
+ * A group with a NaN gets a NaN scale.  Not for DB2_F64.  res overlaps nothing. */
+int db2k_rms_norm_q8(int dtype, const void *x, int64_t rows, int64_t cols, int64_t x_ld, const void *residual,
+                     int64_t residual_ld, const void *weight, double eps, void *sum, int64_t sum_ld, void *res,
+                     int64_t res_ld, void *scales, int64_t scales_ld, int64_t group, void *rstd, void *stream);
+/* Gradient, from the sum s and the rstd of the forward call: t = grad * weight;
+ * dx = rstd * (t - s * rstd^2 * mean(t * s)) + dsum, which is the gradient of x and of residual alike; dsum (the gradient
+ * that reaches s on its other way, along the residual) may be NULL.  dweight: cols contiguous wide values, the column
+ * sums of grad * s * rstd in a fixed order; NULL: not wanted (and no scratch needed).  dx may be grad, sum or dsum
+ * itself; no other overlap. */
+size_t db2k_rms_norm_grad_scratch_bytes(int dtype, int64_t rows, int64_t cols);
+int db2k_rms_norm_grad(int dtype, const void *grad, int64_t grad_ld, int64_t rows, int64_t cols, const void *sum,
+                       int64_t sum_ld, const void *weight, const void *rstd, const void *dsum, int64_t dsum_ld, void *dx,
+                       int64_t dx_ld, void *dweight, void *scratch, size_t scratch_bytes, void *stream);
+
 /* ------------------------------------------------------------------------- */
 /* db2_*: runtime -- context, matrix handles with residency, operator calls   */
 /* ------------------------------------------------------------------------- */
@@ -440,6 +464,15 @@ int db2_castObj(db2_context *ctx, db2_matrix **res, db2_matrix *arg, int dtype);
 int db2_embed(db2_context *ctx, db2_matrix **res, db2_matrix *table, db2_matrix *tokens, double scale);
 int db2_embedGrad(db2_context *ctx, db2_matrix **res, db2_matrix *grad, db2_matrix *tokens, int64_t vocab, double scale,
                   int res_dtype, int accumulate);
+/* db2k_rms_norm, db2k_rms_norm_q8, db2k_rms_norm_grad on handles.  weight: 1 x cols; residual, weight, dsum may be NULL;
+ * sum, rstd and dweight are not computed when their slot pointer is NULL; rstd: rows x 1, dweight: 1 x cols, both of
+ * the wide type. */
+int db2_rmsNorm(db2_context *ctx, db2_matrix **res, db2_matrix **sum, db2_matrix **rstd, db2_matrix *x,
+                db2_matrix *residual, db2_matrix *weight, double eps);
+int db2_rmsNormQ8(db2_context *ctx, db2_matrix **res, db2_matrix **scales, db2_matrix **sum, db2_matrix **rstd,
+                  db2_matrix *x, db2_matrix *residual, db2_matrix *weight, double eps, int64_t group);
+int db2_rmsNormGrad(db2_context *ctx, db2_matrix **dx, db2_matrix **dweight, db2_matrix *grad, db2_matrix *sum,
+                    db2_matrix *weight, db2_matrix *rstd, db2_matrix *dsum);
 
 /* ------------------------------------------------------------------------- */
 /* row-partition scheduler                                                    */
