@@ -508,6 +508,42 @@ def rmsNormGrad(grad: DenseMatrix, s: DenseMatrix, rstd: DenseMatrix, weight: Op
     return _res(ctx, dx), _res(ctx, dw)
 
 
+class Gate(enum.IntEnum):
+    """h[t] = f[t] * h[t-1] + u[t]; DECAY: f = g, u = x; SIGMOID: f = sigmoid(g), u = (1 - f) * x."""
+    DECAY = _l.GATE_DECAY
+    SIGMOID = _l.GATE_SIGMOID
+
+
+def gatedScan(gate, g: DenseMatrix, x: DenseMatrix, offsets: Optional[DenseMatrix] = None,
+              h0: Optional[DenseMatrix] = None, ctx: Optional[Context] = None):
+    """The gated recurrence down the rows of every column: (h, the state behind every sequence).  `offsets` (int64 column)
+    says where the packed sequences start and where the last one ends; None: one sequence."""
+    ctx = ctx or g.ctx
+    h, last = C.c_void_p(), C.c_void_p()
+    check(lib.db2_gatedScan(ctx.handle, int(gate), C.byref(h), C.byref(last), g.handle, x.handle, _handle(offsets),
+                            _handle(h0)))
+    return _res(ctx, h), _res(ctx, last)
+
+
+def gatedScanGrad(gate, g: DenseMatrix, x: Optional[DenseMatrix], h: DenseMatrix, grad: DenseMatrix,
+                  offsets: Optional[DenseMatrix] = None, h0: Optional[DenseMatrix] = None,
+                  grad_last: Optional[DenseMatrix] = None, ctx: Optional[Context] = None):
+    """(gradient of g, of x, of h0) from the result h of gatedScan, the gradient of h and that of the last states."""
+    ctx = ctx or g.ctx
+    dg, dx, dh0 = C.c_void_p(), C.c_void_p(), C.c_void_p()
+    check(lib.db2_gatedScanGrad(ctx.handle, int(gate), C.byref(dg), C.byref(dx), C.byref(dh0), g.handle, _handle(x),
+                                h.handle, grad.handle, _handle(offsets), _handle(h0), _handle(grad_last)))
+    return _res(ctx, dg), _res(ctx, dx), _res(ctx, dh0)
+
+
+def gatedStep(gate, g: DenseMatrix, x: DenseMatrix, state: DenseMatrix, ctx: Optional[Context] = None) -> DenseMatrix:
+    """One new row per sequence: `state` (one row each) is brought up to date in place; returns h."""
+    ctx = ctx or g.ctx
+    h = C.c_void_p()
+    check(lib.db2_gatedStep(ctx.handle, int(gate), C.byref(h), C.byref(state._h), g.handle, x.handle, state.handle))
+    return _res(ctx, h)
+
+
 class CSRMatrix:
     """Handle to a db2_csr.  The host arrays follow the reference's CSRMatrix layout (values, colIdxs and rowOffsets
     with 64-bit indices)."""

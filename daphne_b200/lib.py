@@ -14,6 +14,9 @@ LIB_PATH = _PKG / "libdaphne_b200.so"
 # value type codes (include/daphne_b200.h)
 F64, F32, I64, U64, I32, U32, U8, F16, BF16, F8E4M3 = 0, 1, 2, 3, 4, 5, 6, 7, 8, 9
 
+# gates of the linear recurrence
+GATE_DECAY, GATE_SIGMOID = 0, 1
+
 
 class Db2Error(RuntimeError):
     """A non-zero status from the C-ABI; mirrors the std::runtime_error the reference's kernels throw."""
@@ -100,6 +103,11 @@ _SIGS = {
     "db2k_rms_norm_q8": (i32, [i32, vp, i64, i64, i64, vp, i64, vp, C.c_double, vp, i64, vp, i64, vp, i64, i64, vp, vp]),
     "db2k_rms_norm_grad_scratch_bytes": (sz, [i32, i64, i64]),
     "db2k_rms_norm_grad": (i32, [i32, vp, i64, i64, i64, vp, i64, vp, vp, vp, i64, vp, i64, vp, vp, sz, vp]),
+    "db2k_gated_scan_scratch_bytes": (sz, [i32, i64, i64, i64]),
+    "db2k_gated_scan": (i32, [i32, i32, vp, i64, vp, i64, i64, i64, vp, i64, vp, i64, vp, i64, vp, i64, vp, sz, vp]),
+    "db2k_gated_scan_grad": (i32, [i32, i32, vp, i64, vp, i64, vp, i64, vp, i64, i64, i64, vp, i64, vp, i64, vp, i64, vp,
+                                   i64, vp, i64, vp, i64, vp, sz, vp]),
+    "db2k_gated_step": (i32, [i32, i32, vp, i64, vp, i64, i64, i64, vp, i64, vp, i64, vp, i64, vp]),
     # runtime
     "db2_context_create": (i32, [i32, _P(vp)]),
     "db2_context_destroy": (i32, [vp]),
@@ -191,6 +199,9 @@ _SIGS = {
     "db2_rmsNorm": (i32, [vp, _P(vp), _P(vp), _P(vp), vp, vp, vp, C.c_double]),
     "db2_rmsNormQ8": (i32, [vp, _P(vp), _P(vp), _P(vp), _P(vp), vp, vp, vp, C.c_double, i64]),
     "db2_rmsNormGrad": (i32, [vp, _P(vp), _P(vp), vp, vp, vp, vp, vp]),
+    "db2_gatedScan": (i32, [vp, i32, _P(vp), _P(vp), vp, vp, vp, vp]),
+    "db2_gatedScanGrad": (i32, [vp, i32, _P(vp), _P(vp), _P(vp), vp, vp, vp, vp, vp, vp, vp]),
+    "db2_gatedStep": (i32, [vp, i32, _P(vp), _P(vp), vp, vp, vp]),
     "db2_readDaphne": (i32, [vp, _P(vp), C.c_char_p]),
     "db2_writeDaphne": (i32, [vp, vp, C.c_char_p]),
     "db2_vectorizedPipeline": (i32, [vp, _P(vp), sz, _P(i32), _P(vp), sz, _P(i64), _P(i64), _P(i64), _P(i64), vp, i64]),

@@ -305,6 +305,37 @@ int db2k_rms_norm_grad(int dtype, const void *grad, int64_t grad_ld, int64_t row
                        int64_t sum_ld, const void *weight, const void *rstd, const void *dsum, int64_t dsum_ld, void *dx,
                        int64_t dx_ld, void *dweight, void *scratch, size_t scratch_bytes, void *stream);
 
+/* Gated linear recurrence down the rows, column by column: h[t] = f[t] * h[t-1] + u[t] with
+ *   DB2_GATE_DECAY:    f = g,           u = x
+ *   DB2_GATE_SIGMOID:  f = sigmoid(g),  u = (1 - f) * x
+ * over `seqs` sequences of consecutive rows: sequence s is the rows row_off[s] .. row_off[s + 1] - 1 (device int64, seqs + 1
+ * ascending values within [0, rows]; values that break this give some other rows of the same matrices, never memory
+ * outside them), or, with row_off == NULL, rows / seqs rows each.  Rows of no sequence (in front of the first, behind the last)
+ * are left as they are, in h as in the gradients.  A sequence may be empty.  h0 (seqs x cols wide values, NULL: zeros) is the
+ * state in front of every sequence; last (seqs x cols wide values, may be NULL, may be h0 itself) receives the state behind
+ * it, unrounded.  h may be g or x itself (same pointer and leading dimension); no other overlap.
+ * A NaN or an infinity stays within its column and sequence; what follows it there is not finite, but which of the
+ * non-finite values is not specified.  Gates are expected within [-1, 1]: products of larger ones over many rows may
+ * overflow where the recurrence itself does not. */
+enum { DB2_GATE_DECAY = 0, DB2_GATE_SIGMOID = 1 };
+size_t db2k_gated_scan_scratch_bytes(int dtype, int64_t rows, int64_t cols, int64_t seqs); /* of both directions */
+int db2k_gated_scan(int dtype, int gate, const void *g, int64_t g_ld, const void *x, int64_t x_ld, int64_t rows,
+                    int64_t cols, const int64_t *row_off, int64_t seqs, const void *h0, int64_t h0_ld, void *h,
+                    int64_t h_ld, void *last, int64_t last_ld, void *scratch, size_t scratch_bytes, void *stream);
+/* Its gradient: from g, x (not read for DB2_GATE_DECAY), the result h, the gradient `grad` of h and that of the last states
+ * (grad_last, seqs x cols wide values, NULL: zeros) to dg, dx and dh0 (seqs x cols wide values, may be NULL).  Nothing
+ * overlaps. */
+int db2k_gated_scan_grad(int dtype, int gate, const void *g, int64_t g_ld, const void *x, int64_t x_ld, const void *h,
+                         int64_t h_ld, const void *grad, int64_t grad_ld, int64_t rows, int64_t cols,
+                         const int64_t *row_off, int64_t seqs, const void *h0, int64_t h0_ld, const void *grad_last,
+                         int64_t grad_last_ld, void *dg, int64_t dg_ld, void *dx, int64_t dx_ld, void *dh0,
+                         int64_t dh0_ld, void *scratch, size_t scratch_bytes, void *stream);
+/* One new row for each of n sequences: new_state = f * state + u (wide values; new_state may be state itself), h = the same
+ * rounded to dtype (may be NULL; may be g or x itself). */
+int db2k_gated_step(int dtype, int gate, const void *g, int64_t g_ld, const void *x, int64_t x_ld, int64_t n, int64_t cols,
+                    const void *state, int64_t state_ld, void *new_state, int64_t new_state_ld, void *h, int64_t h_ld,
+                    void *stream);
+
 /* ------------------------------------------------------------------------- */
 /* db2_*: runtime -- context, matrix handles with residency, operator calls   */
 /* ------------------------------------------------------------------------- */
@@ -473,6 +504,18 @@ int db2_rmsNormQ8(db2_context *ctx, db2_matrix **res, db2_matrix **scales, db2_m
                   db2_matrix *x, db2_matrix *residual, db2_matrix *weight, double eps, int64_t group);
 int db2_rmsNormGrad(db2_context *ctx, db2_matrix **dx, db2_matrix **dweight, db2_matrix *grad, db2_matrix *sum,
                     db2_matrix *weight, db2_matrix *rstd, db2_matrix *dsum);
+/* db2k_gated_scan, db2k_gated_scan_grad, db2k_gated_step on handles.  offsets: column matrix of int64 (NULL: one sequence of
+ * all rows); offsets that do not ascend within the rows are DB2_EDOMAIN (they are looked at on the host).  h0, grad_last
+ * may be NULL; last and dh0 are not computed when their slot pointer is NULL.  Rows of no sequence are zero in a result
+ * that the call allocates and keep their values in one that is given. */
+int db2_gatedScan(db2_context *ctx, int gate, db2_matrix **h, db2_matrix **last, db2_matrix *g, db2_matrix *x,
+                  db2_matrix *offsets, db2_matrix *h0);
+int db2_gatedScanGrad(db2_context *ctx, int gate, db2_matrix **dg, db2_matrix **dx, db2_matrix **dh0, db2_matrix *g,
+                      db2_matrix *x, db2_matrix *h, db2_matrix *grad, db2_matrix *offsets, db2_matrix *h0,
+                      db2_matrix *grad_last);
+/* *new_state may be state: it is then updated in place */
+int db2_gatedStep(db2_context *ctx, int gate, db2_matrix **h, db2_matrix **new_state, db2_matrix *g, db2_matrix *x,
+                  db2_matrix *state);
 
 /* ------------------------------------------------------------------------- */
 /* row-partition scheduler                                                    */
