@@ -17,11 +17,18 @@
 #include "runtime.h"
 #include "seq.cuh"
 
+#include <cooperative_groups.h>
+
 namespace db2 {
 
 namespace {
 
-constexpr int SCAN_WARPS = 8, SCAN_R = 8, SCAN_TILE = SCAN_WARPS * SCAN_R;
+constexpr int SCAN_WARPS = 4, SCAN_THREADS = SCAN_WARPS * 32;
+// Rows that a warp holds at once.  More rows spread the exchange between the warps over more work; the registers of a
+// thread (gates, inputs and the rows on their way, for VEC columns) set the limit at 128, four CTAs on an SM.
+template <typename T, bool BACK> constexpr int scan_rows() { return (BACK ? 8 : 16) / (sizeof(T) == 8 ? 2 : 1); }
+template <typename T, bool BACK> constexpr int scan_tile() { return SCAN_WARPS * scan_rows<T, BACK>(); }
+constexpr int SCAN_CLUSTER = 8; // most CTAs of a cluster
 
 template <typename T> struct ScanArgs {
     using W = wide_t<T>;
@@ -29,11 +36,12 @@ template <typename T> struct ScanArgs {
     T *h, *dg, *dx;
     const W *h0, *init; // init: the state that enters (forward: h0; gradient: the gradient of the last state)
     W *last;            // the state that leaves (forward: last state; gradient: dh0)
-    W *part;            // split sequences: (A, B) per block, later the state that enters the block
+    W *part;            // split sequences: (A, B) per block
     const int64_t *off;
     int64_t g_ld, x_ld, grad_ld, above_ld, h_ld, dg_ld, dx_ld, h0_ld, init_ld, last_ld, part_ld;
     int64_t rows, cols, seqs, strips;
-    int blocks; // blocks that a sequence is cut into
+    int blocks;  // blocks that a sequence is cut into, by a pass of its own
+    int cluster; // CTAs that take turns on the tiles of a block
 };
 
 // rows of sequence s; offsets outside [0, rows] or that go back give fewer rows, never others' memory
@@ -51,20 +59,20 @@ __device__ __forceinline__ void sequence(const ScanArgs<T> &a, int64_t s, int64_
 }
 
 // f = sigmoid(g) and 1 - f, each accurate relative to itself: e = exp(-|g|) lies in [0, 1], and the two are 1 / (1 + e) and
-// e / (1 + e).  In float the fast exponential and division cost a few units in the last place of f.
+// e / (1 + e).  In float the approximate base-2 exponential and reciprocal cost a few units in the last place of f; a
+// NaN passes through all of it.
 __device__ __forceinline__ void gate_pair(float g, float *f, float *o) {
-    const float e = __expf(-fabsf(g)), r = __fdividef(1.0f, 1.0f + e), q = e * r;
+    float e, r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(fabsf(g) * -1.44269504f));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
+    const float q = e * r;
     *f = g >= 0.0f ? r : q;
     *o = g >= 0.0f ? q : r;
-    if (g != g)
-        *f = *o = g;
 }
 __device__ __forceinline__ void gate_pair(double g, double *f, double *o) {
     const double e = exp(-fabs(g)), r = 1.0 / (1.0 + e), q = e * r;
     *f = g >= 0.0 ? r : q;
     *o = g >= 0.0 ? q : r;
-    if (g != g)
-        *f = *o = g;
 }
 
 // a * v + b for a state v and a composed step: a state of zero stays out of it, so that a product of large gates that
@@ -73,180 +81,258 @@ template <typename W> __device__ __forceinline__ W step_state(W a, W v, W b) {
     return v == W(0) ? b : a * v + b;
 }
 
-// CTA (sequence, strip of columns, block of rows).  AGGREGATE: only (A, B) of the block, into part.  Otherwise the
-// results; the state that enters is init, or part when sequences are cut into several blocks.
+// A composed step per channel of a strip, as it lies in shared memory.
+template <typename W, int VEC> struct Steps {
+    W a[32 * VEC], b[32 * VEC];
+};
+template <typename W, int VEC> __device__ __forceinline__ void put(Steps<W, VEC> &s, int lane, const W *A, const W *B) {
+    Vec<W, VEC> x, y;
+#pragma unroll
+    for (int k = 0; k < VEC; k++) {
+        x.v[k] = A[k];
+        y.v[k] = B[k];
+    }
+    st_vec<W, VEC>(s.a + lane * VEC, x);
+    st_vec<W, VEC>(s.b + lane * VEC, y);
+}
+
+// CTA (sequence, strip of 32 x VEC columns, block of rows, rank within its cluster).  AGGREGATE: only (A, B) of the
+// block, into part.  Otherwise the results; the state that enters a block is init, advanced by part of the blocks in
+// front of it.  The CTAs of a cluster take the tiles of their block in turns: rank k has tile k, k + cluster, ...; in
+// every round each of them sends the composed step of its tile to all of them, so that all know the state that enters
+// each tile, and the data is still read once.
 template <typename T, int VEC, bool BACK, bool SIGMOID, bool AGGREGATE>
-__global__ void __launch_bounds__(SCAN_WARPS * 32) gated_scan_kernel(ScanArgs<T> a) {
+__global__ void __launch_bounds__(SCAN_THREADS, sizeof(T) == 8 ? 3 : 4) gated_scan_kernel(ScanArgs<T> a) {
     using W = wide_t<T>;
     using V = Vec<T, VEC>;
-    __shared__ W agg[2][SCAN_WARPS][2][32 * VEC];
+    constexpr int R = scan_rows<T, BACK>(), TILE = scan_tile<T, BACK>();
+    __shared__ Steps<W, VEC> agg[2][SCAN_WARPS];
+    __shared__ Steps<W, VEC> tiles[2][SCAN_CLUSTER];
     const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-    const int64_t strip = blockIdx.x % a.strips, rest = blockIdx.x / a.strips;
+    const int rank = (int)(blockIdx.x % a.cluster);
+    const int64_t id = blockIdx.x / a.cluster, strip = id % a.strips, rest = id / a.strips;
     const int64_t blk = rest % a.blocks, seq = rest / a.blocks;
     const int64_t c = (strip * 32 + lane) * VEC;
     const bool in = c < a.cols; // cols is a multiple of VEC
     int64_t begin, end;
     sequence(a, seq, &begin, &end);
     // rows of the block, a multiple of the tile each: n rows from `first` on, in the direction of the recurrence
-    const int64_t len = end - begin, per = ((len + a.blocks - 1) / a.blocks + SCAN_TILE - 1) / SCAN_TILE * SCAN_TILE;
+    const int64_t len = end - begin, per = ((len + a.blocks - 1) / a.blocks + TILE - 1) / TILE * TILE;
     const int64_t skip = blk * per < len ? blk * per : len, n = len - skip < per ? len - skip : per;
     const int64_t first = BACK ? end - 1 - skip : begin + skip;
-    W *my_part = a.part + (seq * a.blocks + blk) * 2 * a.part_ld;
 
     W state[VEC], prod[VEC]; // AGGREGATE: (prod, state) is the step composed so far
 #pragma unroll
     for (int k = 0; k < VEC; k++) {
         prod[k] = W(1);
-        state[k] = W(0);
-        if (!AGGREGATE && in) {
-            if (a.blocks > 1)
-                state[k] = my_part[c + k];
-            else if (a.init)
-                state[k] = a.init[seq * a.init_ld + c + k];
-        }
+        state[k] = !AGGREGATE && in && a.init ? a.init[seq * a.init_ld + c + k] : W(0);
     }
-    V rg[SCAN_R], rb[SCAN_R], rx[SCAN_R], ra[SCAN_R]; // g; x or grad; (gradient) x; (gradient) h of the row above
-    auto row_at = [&](int64_t q) { return BACK ? first - q : first + q; };
-    auto load = [&](int64_t q0) {
-#pragma unroll
-        for (int i = 0; i < SCAN_R; i++)
-            if (in && q0 + i < n) {
-                const int64_t r = row_at(q0 + i);
-                rg[i] = ld_vec<T, VEC>(a.g + r * a.g_ld + c);
-                rb[i] = BACK ? ld_vec<T, VEC>(a.grad + r * a.grad_ld + c) : ld_vec<T, VEC>(a.x + r * a.x_ld + c);
-                if constexpr (BACK && !AGGREGATE) {
-                    if constexpr (SIGMOID)
-                        rx[i] = ld_vec<T, VEC>(a.x + r * a.x_ld + c);
-                    if (r > begin)
-                        ra[i] = ld_vec<T, VEC>(a.above + (r - 1) * a.above_ld + c);
-                }
-            }
-    };
-    load(warp * SCAN_R);
-    int turn = 0;
-    for (int64_t tile = 0; tile < n; tile += SCAN_TILE, turn ^= 1) {
-        const int64_t q0 = tile + warp * SCAN_R;
-        W f[SCAN_R][VEC], o[SCAN_R][VEC], b[SCAN_R][VEC]; // gate, 1 - gate, u or dh
+    if (!AGGREGATE && blk > 0) { // the blocks in front: a quarter for each warp, then the four quarters in order
+        const int64_t share = (blk + SCAN_WARPS - 1) / SCAN_WARPS, b0 = warp * share, b1 = b0 + share < blk ? b0 + share : blk;
+        const W *p = a.part + (seq * a.blocks + b0) * 2 * a.part_ld + c;
         W A[VEC], B[VEC];
 #pragma unroll
         for (int k = 0; k < VEC; k++) {
             A[k] = W(1);
             B[k] = W(0);
         }
+        if (in) {
+#pragma unroll 8
+            for (int64_t b = b0; b < b1; b++, p += 2 * a.part_ld)
 #pragma unroll
-        for (int i = 0; i < SCAN_R; i++)
+                for (int k = 0; k < VEC; k++) {
+                    B[k] = step_state(p[k], B[k], p[a.part_ld + k]);
+                    A[k] *= p[k];
+                }
+        }
+        put(agg[1][warp], lane, A, B); // the first tile uses the other half
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < SCAN_WARPS; w++)
+#pragma unroll
+            for (int k = 0; k < VEC; k++)
+                state[k] = step_state(agg[1][w].a[lane * VEC + k], state[k], agg[1][w].b[lane * VEC + k]);
+    }
+    // Row q of the block lies q * ld elements behind the first one, or in front of it.
+    const int64_t sg = BACK ? -a.g_ld : a.g_ld, sx = BACK ? -a.x_ld : a.x_ld;
+    const int64_t base = first, q_first = (int64_t)rank * TILE + warp * R;
+    const T *pg = a.g + (base + (BACK ? -q_first : q_first)) * a.g_ld + c;
+    const T *px = a.x + (base + (BACK ? -q_first : q_first)) * a.x_ld + c;
+    const T *pd = BACK ? a.grad + (base - q_first) * a.grad_ld + c : nullptr;
+    const T *pa = BACK ? a.above + (base - q_first - 1) * a.above_ld + c : nullptr;
+    V rg[R], rx[R], rd[R], ra[R];
+    // rows that are there of the R from row q on (for this lane)
+    auto rows_from = [&](int64_t q) { return !in || q >= n ? 0 : (n - q < R ? (int)(n - q) : R); };
+    auto load = [&](int64_t q) {
+        const int m = rows_from(q);
+        const int above = BACK && first - q - (m - 1) == begin ? m - 1 : m; // the sequence's first row has none above
+#pragma unroll
+        for (int i = 0; i < R; i++) {
+            if (i < m) {
+                rg[i] = ld_vec<T, VEC>(pg + i * sg);
+                if constexpr (!BACK || (SIGMOID && !AGGREGATE))
+                    rx[i] = ld_vec<T, VEC>(px + i * sx);
+                if constexpr (BACK)
+                    rd[i] = ld_vec<T, VEC>(pd - i * a.grad_ld);
+            }
+            if constexpr (BACK && !AGGREGATE)
+                if (i < above)
+                    ra[i] = ld_vec<T, VEC>(pa - i * a.above_ld);
+        }
+        const int64_t step = (int64_t)TILE * a.cluster;
+        pg += step * sg;
+        if constexpr (!BACK || (SIGMOID && !AGGREGATE))
+            px += step * sx;
+        if constexpr (BACK)
+            pd -= step * a.grad_ld;
+        if constexpr (BACK && !AGGREGATE)
+            pa -= step * a.above_ld;
+    };
+    load(q_first);
+    int turn = 0;
+    for (int64_t round = 0; round < n; round += (int64_t)TILE * a.cluster, turn ^= 1) {
+        const int64_t q = round + q_first;
+        const int m = rows_from(q);
+        W f[R][VEC], o[R][VEC], b[R][VEC]; // gate, 1 - gate, u or dh
+        W A[VEC], B[VEC];
+#pragma unroll
+        for (int k = 0; k < VEC; k++) {
+            A[k] = W(1);
+            B[k] = W(0);
+        }
+        V kx[R], ka[R];
+#pragma unroll
+        for (int i = 0; i < R; i++) {
 #pragma unroll
             for (int k = 0; k < VEC; k++) {
                 f[i][k] = W(1);
                 o[i][k] = b[i][k] = W(0);
-                if (in && q0 + i < n) {
-                    const W g = widen(rg[i].v[k]);
-                    if (SIGMOID)
-                        gate_pair(g, &f[i][k], &o[i][k]);
+            }
+            if (i < m) {
+#pragma unroll
+                for (int k = 0; k < VEC; k++) {
+                    f[i][k] = widen(rg[i].v[k]);
+                    if constexpr (SIGMOID)
+                        gate_pair(f[i][k], &f[i][k], &o[i][k]);
+                    if constexpr (BACK)
+                        b[i][k] = widen(rd[i].v[k]);
                     else
-                        f[i][k] = g;
-                    b[i][k] = widen(rb[i].v[k]);
-                    if (SIGMOID && !BACK)
-                        b[i][k] *= o[i][k];
+                        b[i][k] = SIGMOID ? o[i][k] * widen(rx[i].v[k]) : W(widen(rx[i].v[k]));
                 }
+            }
+#pragma unroll
+            for (int k = 0; k < VEC; k++) {
                 B[k] = BACK ? f[i][k] * (B[k] + b[i][k]) : f[i][k] * B[k] + b[i][k];
                 A[k] *= f[i][k];
             }
-        V px[SCAN_R], pa[SCAN_R];
-        if constexpr (BACK && !AGGREGATE) {
-#pragma unroll
-            for (int i = 0; i < SCAN_R; i++) {
-                px[i] = rx[i];
-                pa[i] = ra[i];
+            if constexpr (BACK && !AGGREGATE) {
+                kx[i] = rx[i];
+                ka[i] = ra[i];
             }
         }
-        load(q0 + SCAN_TILE); // on its way while the warps exchange their steps
+        load(q + (int64_t)TILE * a.cluster); // on its way while the steps are exchanged
+        put(agg[turn][warp], lane, A, B);
+        __syncthreads(); // the halves of agg alternate: nobody writes this one again before the next barrier
+        // the composed step of the warps in front of this one, and of the whole tile
+        W fa[VEC], fb[VEC], va[VEC], v[VEC];
 #pragma unroll
         for (int k = 0; k < VEC; k++) {
-            agg[turn][warp][0][lane * VEC + k] = A[k];
-            agg[turn][warp][1][lane * VEC + k] = B[k];
+            fa[k] = W(1);
+            fb[k] = W(0);
         }
-        __syncthreads(); // the halves of agg alternate: nobody writes this one again before the next barrier
-        W v[VEC];
 #pragma unroll
-        for (int w = 0; w < SCAN_WARPS; w++)
+        for (int w = 0; w < SCAN_WARPS; w++) {
+            const Vec<W, VEC> wa = ld_vec<W, VEC>(agg[turn][w].a + lane * VEC), wb = ld_vec<W, VEC>(agg[turn][w].b + lane * VEC);
 #pragma unroll
             for (int k = 0; k < VEC; k++) {
-                const W wa = agg[turn][w][0][lane * VEC + k], wb = agg[turn][w][1][lane * VEC + k];
-                if (w == warp)
-                    v[k] = state[k];
-                state[k] = step_state(wa, state[k], wb);
-                if (AGGREGATE)
-                    prod[k] *= wa;
-            }
-        if constexpr (!AGGREGATE) {
-#pragma unroll
-            for (int i = 0; i < SCAN_R; i++) {
-                const bool live = in && q0 + i < n;
-                const int64_t r = row_at(q0 + i);
-                V y, z;
-#pragma unroll
-                for (int k = 0; k < VEC; k++) {
-                    if constexpr (!BACK) {
-                        v[k] = f[i][k] * v[k] + b[i][k];
-                        y.v[k] = narrow<T>(v[k]);
-                    } else {
-                        const W delta = b[i][k] + v[k];
-                        W above = W(0);
-                        if (live && r > begin)
-                            above = widen(pa[i].v[k]);
-                        else if (live && a.h0)
-                            above = a.h0[seq * a.h0_ld + c + k];
-                        if constexpr (SIGMOID) {
-                            y.v[k] = narrow<T>(delta * (above - (live ? W(widen(px[i].v[k])) : W(0))) * f[i][k] * o[i][k]);
-                            z.v[k] = narrow<T>(delta * o[i][k]);
-                        } else {
-                            y.v[k] = narrow<T>(delta * above);
-                            z.v[k] = narrow<T>(delta);
-                        }
-                        v[k] = f[i][k] * delta;
-                    }
+                if (w == warp) {
+                    va[k] = fa[k];
+                    v[k] = fb[k];
                 }
-                if (live) {
-                    if constexpr (!BACK)
-                        st_vec<T, VEC>(a.h + r * a.h_ld + c, y);
-                    else {
-                        st_vec<T, VEC>(a.dg + r * a.dg_ld + c, y);
-                        st_vec<T, VEC>(a.dx + r * a.dx_ld + c, z);
-                    }
-                }
+                fb[k] = step_state(wa.v[k], fb[k], wb.v[k]);
+                fa[k] *= wa.v[k];
             }
         }
+        if (a.cluster == 1) {
+#pragma unroll
+            for (int k = 0; k < VEC; k++) {
+                v[k] = step_state(va[k], state[k], v[k]);
+                state[k] = step_state(fa[k], state[k], fb[k]);
+                prod[k] *= fa[k];
+            }
+        } else {
+            for (int t = warp; t < a.cluster; t += SCAN_WARPS) {
+                Steps<W, VEC> *there = cooperative_groups::this_cluster().map_shared_rank(&tiles[turn][rank], t);
+                put(*there, lane, fa, fb);
+            }
+            cooperative_groups::this_cluster().sync();
+            W mine[VEC];
+            for (int t = 0; t < a.cluster; t++) {
+                const Vec<W, VEC> ta = ld_vec<W, VEC>(tiles[turn][t].a + lane * VEC), tb = ld_vec<W, VEC>(tiles[turn][t].b + lane * VEC);
+#pragma unroll
+                for (int k = 0; k < VEC; k++) {
+                    if (t == rank)
+                        mine[k] = state[k];
+                    state[k] = step_state(ta.v[k], state[k], tb.v[k]);
+                    prod[k] *= ta.v[k];
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < VEC; k++)
+                v[k] = step_state(va[k], mine[k], v[k]);
+        }
+        if constexpr (!AGGREGATE) {
+            const int64_t r = BACK ? first - q : first + q;
+#pragma unroll
+            for (int i = 0; i < R; i++)
+                if (i < m) {
+                    V y, z;
+                    if constexpr (!BACK) {
+#pragma unroll
+                        for (int k = 0; k < VEC; k++) {
+                            v[k] = f[i][k] * v[k] + b[i][k];
+                            y.v[k] = narrow<T>(v[k]);
+                        }
+                        st_vec<T, VEC>(a.h + (r + i) * a.h_ld + c, y);
+                    } else {
+                        W above[VEC];
+#pragma unroll
+                        for (int k = 0; k < VEC; k++)
+                            above[k] = widen(ka[i].v[k]);
+                        if (r - i == begin) {
+#pragma unroll
+                            for (int k = 0; k < VEC; k++)
+                                above[k] = a.h0 ? a.h0[seq * a.h0_ld + c + k] : W(0);
+                        }
+#pragma unroll
+                        for (int k = 0; k < VEC; k++) {
+                            const W delta = b[i][k] + v[k];
+                            v[k] = f[i][k] * delta;
+                            if constexpr (SIGMOID) {
+                                y.v[k] = narrow<T>(v[k] * (above[k] - widen(kx[i].v[k])) * o[i][k]);
+                                z.v[k] = narrow<T>(delta * o[i][k]);
+                            } else {
+                                y.v[k] = narrow<T>(delta * above[k]);
+                                z.v[k] = narrow<T>(delta);
+                            }
+                        }
+                        st_vec<T, VEC>(a.dg + (r - i) * a.dg_ld + c, y);
+                        st_vec<T, VEC>(a.dx + (r - i) * a.dx_ld + c, z);
+                    }
+                }
+        }
     }
-    if (warp == 0 && in) {
+    if (warp == 0 && rank == 0 && in) {
+        W *p = a.part + (seq * a.blocks + blk) * 2 * a.part_ld + c;
 #pragma unroll
         for (int k = 0; k < VEC; k++) {
             if (AGGREGATE) {
-                my_part[c + k] = prod[k];
-                my_part[a.part_ld + c + k] = state[k];
-            } else if (a.blocks == 1 && a.last)
+                p[k] = prod[k];
+                p[a.part_ld + k] = state[k];
+            } else if (blk == a.blocks - 1 && a.last)
                 a.last[seq * a.last_ld + c + k] = state[k];
         }
     }
-}
-
-// (A, B) of the blocks of every sequence -> the state that enters each block; the state that leaves the last one
-template <typename T> __global__ void __launch_bounds__(128) gated_carry_kernel(ScanArgs<T> a) {
-    using W = wide_t<T>;
-    const int64_t i = (int64_t)blockIdx.x * 128 + threadIdx.x;
-    if (i >= a.seqs * a.cols)
-        return;
-    const int64_t seq = i / a.cols, c = i % a.cols;
-    W v = a.init ? a.init[seq * a.init_ld + c] : W(0);
-    W *p = a.part + seq * a.blocks * 2 * a.part_ld + c;
-#pragma unroll 8
-    for (int b = 0; b < a.blocks; b++, p += 2 * a.part_ld) {
-        const W A = p[0], B = p[a.part_ld];
-        p[0] = v;
-        v = step_state(A, v, B);
-    }
-    if (a.last)
-        a.last[seq * a.last_ld + c] = v;
 }
 
 template <typename T, bool SIGMOID>
@@ -268,29 +354,51 @@ __global__ void __launch_bounds__(256)
         }
 }
 
-// Blocks that a sequence is cut into: one (a single pass over the data) when the sequences and strips alone keep the SMs
-// busy or when a block would be shorter than four tiles.  Depends on the shape and the number of SMs alone.
+// How a sequence is shared out, from the shape and the number of SMs alone (both directions share the scratch).
+// `ctas` = sequences x strips of columns work independently.  Four CTAs on every SM keep enough loads in flight; with
+// fewer, the CTAs of a cluster take turns on a sequence's tiles, which reads the data once as before.  Where even
+// clusters leave most SMs without work (few columns, one long sequence), sequences are cut into blocks instead: a first
+// pass composes the blocks' steps, the second one has its inputs from L2 when they fit there.
 template <typename T> constexpr int widest() { return sizeof(T) == 2 ? 2 : 1; }
-int scan_blocks(size_t es, int64_t rows, int64_t cols, int64_t seqs) {
+struct ScanPlan {
+    int blocks, cluster;
+};
+ScanPlan scan_plan(size_t es, int64_t rows, int64_t cols, int64_t seqs) {
+    ScanPlan p{1, 1};
     if (rows <= 0 || cols <= 0 || seqs <= 0)
-        return 1;
-    const int64_t strips = (cols + 31) / 32 / (es == 2 ? 2 : 1) + 1, ctas = strips * seqs;
-    const int64_t want = ((int64_t)sm_count() * 4 + ctas - 1) / ctas, most = rows / seqs / (4 * SCAN_TILE);
+        return p;
+    const int64_t columns = es == 2 ? 64 : 32, strips = (cols + columns - 1) / columns, ctas = strips * seqs;
+    const int64_t tile = 64, tiles = rows / seqs / tile, full = (int64_t)sm_count() * 4;
+    if (ctas * SCAN_CLUSTER >= sm_count() * 2 || tiles < 4 * SCAN_CLUSTER) {
+        while (p.cluster < SCAN_CLUSTER && ctas * p.cluster < full && p.cluster * 2 <= tiles)
+            p.cluster *= 2;
+        return p;
+    }
+    const int64_t want = (full + ctas - 1) / ctas, most = tiles / 4;
     const int64_t b = want < most ? want : most;
-    return b < 2 ? 1 : (int)(b > 1024 ? 1024 : b);
+    p.blocks = (int)(b > 1024 ? 1024 : b);
+    return p;
 }
 
 template <typename T, int VEC, bool BACK, bool SIGMOID> int scan_launch(ScanArgs<T> a, cudaStream_t st) {
     a.strips = (a.cols + 32 * VEC - 1) / (32 * VEC);
-    const int64_t ctas = a.strips * a.blocks * a.seqs;
+    const int64_t ctas = a.strips * a.blocks * a.seqs * a.cluster;
     DB2_CHECK(ctas < ((int64_t)1 << 31), DB2_EUNSUPPORTED, "gatedScan: too many sequences and columns for one launch");
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)a.cluster;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)ctas);
+    cfg.blockDim = dim3(SCAN_THREADS);
+    cfg.stream = st;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
     if (a.blocks > 1) {
-        gated_scan_kernel<T, VEC, BACK, SIGMOID, true><<<(unsigned)ctas, SCAN_WARPS * 32, 0, st>>>(a);
+        DB2_CUDA(cudaLaunchKernelEx(&cfg, gated_scan_kernel<T, VEC, BACK, SIGMOID, true>, a));
         DB2_TRY(after_launch("gated_scan_kernel"));
-        gated_carry_kernel<T><<<(unsigned)((a.seqs * a.cols + 127) / 128), 128, 0, st>>>(a);
-        DB2_TRY(after_launch("gated_carry_kernel"));
     }
-    gated_scan_kernel<T, VEC, BACK, SIGMOID, false><<<(unsigned)ctas, SCAN_WARPS * 32, 0, st>>>(a);
+    DB2_CUDA(cudaLaunchKernelEx(&cfg, gated_scan_kernel<T, VEC, BACK, SIGMOID, false>, a));
     return after_launch("gated_scan_kernel");
 }
 
@@ -373,7 +481,7 @@ extern "C" {
 size_t db2k_gated_scan_scratch_bytes(int dtype, int64_t rows, int64_t cols, int64_t seqs) {
     if (rows <= 0 || cols <= 0 || seqs <= 0)
         return 0;
-    const int blocks = scan_blocks(dtype_size(dtype), rows, cols, seqs);
+    const int blocks = scan_plan(dtype_size(dtype), rows, cols, seqs).blocks;
     return blocks < 2 ? 0 : (size_t)seqs * blocks * 2 * scan_part_ld(cols) * (dtype == DB2_F64 ? 8 : 4);
 }
 
@@ -409,7 +517,9 @@ int db2k_gated_scan(int dtype, int gate, const void *g, int64_t g_ld, const void
         a.rows = rows;
         a.cols = cols;
         a.seqs = seqs;
-        a.blocks = scan_blocks(sizeof(T), rows, cols, seqs);
+        const ScanPlan plan = scan_plan(sizeof(T), rows, cols, seqs);
+        a.blocks = plan.blocks;
+        a.cluster = plan.cluster;
         constexpr size_t al = sizeof(T) * widest<T>();
         const bool packed = cols % widest<T>() == 0 && rows_aligned(g, g_ld, sizeof(T), al) &&
                             rows_aligned(x, x_ld, sizeof(T), al) && rows_aligned(h, h_ld, sizeof(T), al);
@@ -463,7 +573,9 @@ int db2k_gated_scan_grad(int dtype, int gate, const void *g, int64_t g_ld, const
         a.rows = rows;
         a.cols = cols;
         a.seqs = seqs;
-        a.blocks = scan_blocks(sizeof(T), rows, cols, seqs);
+        const ScanPlan plan = scan_plan(sizeof(T), rows, cols, seqs);
+        a.blocks = plan.blocks;
+        a.cluster = plan.cluster;
         constexpr size_t al = sizeof(T) * widest<T>();
         const bool packed = cols % widest<T>() == 0 && rows_aligned(g, g_ld, sizeof(T), al) &&
                             (!sigmoid || rows_aligned(x, x_ld, sizeof(T), al)) && rows_aligned(h, h_ld, sizeof(T), al) &&
