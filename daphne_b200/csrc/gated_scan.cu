@@ -24,11 +24,13 @@ namespace db2 {
 namespace {
 
 constexpr int SCAN_WARPS = 4, SCAN_THREADS = SCAN_WARPS * 32;
-// Rows that a warp holds at once.  More rows spread the exchange between the warps over more work; the registers of a
-// thread (gates, inputs and the rows on their way, for VEC columns) set the limit at 128, four CTAs on an SM.
-template <typename T, bool BACK> constexpr int scan_rows() { return (BACK ? 8 : 16) / (sizeof(T) == 8 ? 2 : 1); }
-template <typename T, bool BACK> constexpr int scan_tile() { return SCAN_WARPS * scan_rows<T, BACK>(); }
-constexpr int SCAN_CLUSTER = 8; // most CTAs of a cluster
+// A lane takes 8 bytes of a row, a warp SCAN_R consecutive rows at once.  More rows would spread the exchange between the
+// warps over more work, but the gates and inputs of a thread's rows have to stay in its registers.
+template <typename T> constexpr int widest() { return 8 / sizeof(T); }
+template <bool BACK> constexpr int scan_rows() { return BACK ? 4 : 8; }
+// Rows on their way lie in shared memory, SCAN_STAGES tiles of them, copied asynchronously.
+constexpr int SCAN_STAGES = 3;
+constexpr int SCAN_CLUSTER = 4; // most CTAs of a cluster
 
 template <typename T> struct ScanArgs {
     using W = wide_t<T>;
@@ -58,16 +60,16 @@ __device__ __forceinline__ void sequence(const ScanArgs<T> &a, int64_t s, int64_
     }
 }
 
-// f = sigmoid(g) and 1 - f, each accurate relative to itself: e = exp(-|g|) lies in [0, 1], and the two are 1 / (1 + e) and
-// e / (1 + e).  In float the approximate base-2 exponential and reciprocal cost a few units in the last place of f; a
-// NaN passes through all of it.
+// f = sigmoid(g) = 1 / (1 + e) and o = 1 - f = e / (1 + e) with e = exp(-g), each accurate relative to itself.  In float the
+// approximate base-2 exponential and reciprocal cost a few units in the last place; the exponent is held at 125, so that e
+// * f stays finite: f does not go below 2^-125.  A NaN passes through.
 __device__ __forceinline__ void gate_pair(float g, float *f, float *o) {
-    float e, r;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(fabsf(g) * -1.44269504f));
+    float t = g * -1.44269504f, e, r;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(t) : "f"(t), "f"(125.0f));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t));
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
-    const float q = e * r;
-    *f = g >= 0.0f ? r : q;
-    *o = g >= 0.0f ? q : r;
+    *f = r;
+    *o = e * r;
 }
 __device__ __forceinline__ void gate_pair(double g, double *f, double *o) {
     const double e = exp(-fabs(g)), r = 1.0 / (1.0 + e), q = e * r;
@@ -75,10 +77,19 @@ __device__ __forceinline__ void gate_pair(double g, double *f, double *o) {
     *o = g >= 0.0 ? q : r;
 }
 
-// a * v + b for a state v and a composed step: a state of zero stays out of it, so that a product of large gates that
-// overflowed does not turn it into NaN
-template <typename W> __device__ __forceinline__ W step_state(W a, W v, W b) {
-    return v == W(0) ? b : a * v + b;
+// A product of gates as it is passed on: finite, so that gates above 1 whose product overflows do not turn a state of zero
+// into NaN.  (A NaN among the gates is in the composed step's b as well.)
+__device__ __forceinline__ float finite(float a) { return fminf(fmaxf(a, -3.40282347e38f), 3.40282347e38f); }
+__device__ __forceinline__ double finite(double a) { return fmin(fmax(a, -1.7976931348623157e308), 1.7976931348623157e308); }
+
+// VEC elements from global to shared memory: asynchronously, or at once where they are fewer than four bytes.
+template <typename T, int VEC> __device__ __forceinline__ void fetch(T *to, const T *from) {
+    if constexpr (sizeof(T) * VEC >= 4)
+        asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"((unsigned)__cvta_generic_to_shared(to)), "l"(from),
+                     "n"(sizeof(T) * VEC)
+                     : "memory");
+    else
+        st_vec<T, VEC>(to, ld_vec<T, VEC>(from));
 }
 
 // A composed step per channel of a strip, as it lies in shared memory.
@@ -86,14 +97,11 @@ template <typename W, int VEC> struct Steps {
     W a[32 * VEC], b[32 * VEC];
 };
 template <typename W, int VEC> __device__ __forceinline__ void put(Steps<W, VEC> &s, int lane, const W *A, const W *B) {
-    Vec<W, VEC> x, y;
 #pragma unroll
     for (int k = 0; k < VEC; k++) {
-        x.v[k] = A[k];
-        y.v[k] = B[k];
+        s.a[lane * VEC + k] = finite(A[k]);
+        s.b[lane * VEC + k] = B[k];
     }
-    st_vec<W, VEC>(s.a + lane * VEC, x);
-    st_vec<W, VEC>(s.b + lane * VEC, y);
 }
 
 // CTA (sequence, strip of 32 x VEC columns, block of rows, rank within its cluster).  AGGREGATE: only (A, B) of the
@@ -102,12 +110,15 @@ template <typename W, int VEC> __device__ __forceinline__ void put(Steps<W, VEC>
 // every round each of them sends the composed step of its tile to all of them, so that all know the state that enters
 // each tile, and the data is still read once.
 template <typename T, int VEC, bool BACK, bool SIGMOID, bool AGGREGATE>
-__global__ void __launch_bounds__(SCAN_THREADS, sizeof(T) == 8 ? 3 : 4) gated_scan_kernel(ScanArgs<T> a) {
+__global__ void __launch_bounds__(SCAN_THREADS, 3) gated_scan_kernel(ScanArgs<T> a) {
     using W = wide_t<T>;
     using V = Vec<T, VEC>;
-    constexpr int R = scan_rows<T, BACK>(), TILE = scan_tile<T, BACK>();
-    __shared__ Steps<W, VEC> agg[2][SCAN_WARPS];
-    __shared__ Steps<W, VEC> tiles[2][SCAN_CLUSTER];
+    constexpr int R = scan_rows<BACK>(), TILE = SCAN_WARPS * R;
+    // operands that are read, and where they stand in a stage
+    constexpr bool X = !BACK || (SIGMOID && !AGGREGATE), ABOVE = BACK && !AGGREGATE;
+    constexpr int AT_X = 1, AT_D = X ? 2 : 1, AT_ABOVE = AT_D + 1, OPERANDS = 1 + X + BACK + ABOVE;
+    __shared__ __align__(16) Steps<W, VEC> agg[2][SCAN_WARPS];
+    __shared__ __align__(16) Steps<W, VEC> tiles[2][SCAN_CLUSTER];
     const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
     const int rank = (int)(blockIdx.x % a.cluster);
     const int64_t id = blockIdx.x / a.cluster, strip = id % a.strips, rest = id / a.strips;
@@ -141,8 +152,8 @@ __global__ void __launch_bounds__(SCAN_THREADS, sizeof(T) == 8 ? 3 : 4) gated_sc
             for (int64_t b = b0; b < b1; b++, p += 2 * a.part_ld)
 #pragma unroll
                 for (int k = 0; k < VEC; k++) {
-                    B[k] = step_state(p[k], B[k], p[a.part_ld + k]);
-                    A[k] *= p[k];
+                    B[k] = p[k] * B[k] + p[a.part_ld + k];
+                    A[k] = finite(A[k] * p[k]);
                 }
         }
         put(agg[1][warp], lane, A, B); // the first tile uses the other half
@@ -151,175 +162,224 @@ __global__ void __launch_bounds__(SCAN_THREADS, sizeof(T) == 8 ? 3 : 4) gated_sc
         for (int w = 0; w < SCAN_WARPS; w++)
 #pragma unroll
             for (int k = 0; k < VEC; k++)
-                state[k] = step_state(agg[1][w].a[lane * VEC + k], state[k], agg[1][w].b[lane * VEC + k]);
+                state[k] = agg[1][w].a[lane * VEC + k] * state[k] + agg[1][w].b[lane * VEC + k];
     }
-    // Row q of the block lies q * ld elements behind the first one, or in front of it.
-    const int64_t sg = BACK ? -a.g_ld : a.g_ld, sx = BACK ? -a.x_ld : a.x_ld;
-    const int64_t base = first, q_first = (int64_t)rank * TILE + warp * R;
-    const T *pg = a.g + (base + (BACK ? -q_first : q_first)) * a.g_ld + c;
-    const T *px = a.x + (base + (BACK ? -q_first : q_first)) * a.x_ld + c;
-    const T *pd = BACK ? a.grad + (base - q_first) * a.grad_ld + c : nullptr;
-    const T *pa = BACK ? a.above + (base - q_first - 1) * a.above_ld + c : nullptr;
-    V rg[R], rx[R], rd[R], ra[R];
-    // rows that are there of the R from row q on (for this lane)
+    // Row q of the block lies q leading dimensions behind the first one, or in front of it.
+    const int64_t dir = BACK ? -1 : 1, q_first = (int64_t)rank * TILE + warp * R, stride = (int64_t)TILE * a.cluster;
+    const int64_t r_first = first + dir * q_first;
+    const T *pg = a.g + r_first * a.g_ld + c;
+    const T *px = X ? a.x + r_first * a.x_ld + c : nullptr;
+    const T *pd = BACK ? a.grad + r_first * a.grad_ld + c : nullptr;
+    const T *pa = ABOVE ? a.above + (r_first - 1) * a.above_ld + c : nullptr;
+    // a thread reads nothing from the stages but what it fetched itself: they need no barrier
+    extern __shared__ __align__(16) unsigned char stage_mem[];
+    T *mine_at = reinterpret_cast<T *>(stage_mem) + (int64_t)warp * SCAN_STAGES * OPERANDS * R * 32 * VEC + lane * VEC;
+    auto at = [&](int stage, int operand, int i) { return mine_at + ((stage * OPERANDS + operand) * R + i) * 32 * VEC; };
+    // rows that are there of the R from row q on, for this lane; all: for all lanes, and none is the sequence's first one
     auto rows_from = [&](int64_t q) { return !in || q >= n ? 0 : (n - q < R ? (int)(n - q) : R); };
-    auto load = [&](int64_t q) {
-        const int m = rows_from(q);
-        const int above = BACK && first - q - (m - 1) == begin ? m - 1 : m; // the sequence's first row has none above
-#pragma unroll
-        for (int i = 0; i < R; i++) {
-            if (i < m) {
-                rg[i] = ld_vec<T, VEC>(pg + i * sg);
-                if constexpr (!BACK || (SIGMOID && !AGGREGATE))
-                    rx[i] = ld_vec<T, VEC>(px + i * sx);
-                if constexpr (BACK)
-                    rd[i] = ld_vec<T, VEC>(pd - i * a.grad_ld);
-            }
-            if constexpr (BACK && !AGGREGATE)
-                if (i < above)
-                    ra[i] = ld_vec<T, VEC>(pa - i * a.above_ld);
-        }
-        const int64_t step = (int64_t)TILE * a.cluster;
-        pg += step * sg;
-        if constexpr (!BACK || (SIGMOID && !AGGREGATE))
-            px += step * sx;
-        if constexpr (BACK)
-            pd -= step * a.grad_ld;
-        if constexpr (BACK && !AGGREGATE)
-            pa -= step * a.above_ld;
+    auto all_there = [&](int64_t q, int m) {
+        return (bool)__all_sync(0xffffffffu, m == R && (!ABOVE || first - q - (R - 1) > begin));
     };
-    load(q_first);
+    auto load_row = [&](int stage, int i, bool above) {
+        fetch<T, VEC>(at(stage, 0, i), pg + i * dir * a.g_ld);
+        if constexpr (X)
+            fetch<T, VEC>(at(stage, AT_X, i), px + i * dir * a.x_ld);
+        if constexpr (BACK)
+            fetch<T, VEC>(at(stage, AT_D, i), pd - i * a.grad_ld);
+        if constexpr (ABOVE)
+            if (above)
+                fetch<T, VEC>(at(stage, AT_ABOVE, i), pa - i * a.above_ld);
+    };
+    auto load = [&](int stage, int64_t q) {
+        const int m = rows_from(q);
+        if (all_there(q, m)) {
+#pragma unroll
+            for (int i = 0; i < R; i++)
+                load_row(stage, i, true);
+        } else {
+#pragma unroll
+            for (int i = 0; i < R; i++)
+                if (i < m)
+                    load_row(stage, i, first - q - i > begin);
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        pg += stride * dir * a.g_ld;
+        if constexpr (X)
+            px += stride * dir * a.x_ld;
+        if constexpr (BACK)
+            pd -= stride * a.grad_ld;
+        if constexpr (ABOVE)
+            pa -= stride * a.above_ld;
+    };
+    for (int k = 0; k < SCAN_STAGES - 1; k++)
+        load(k, q_first + k * stride);
+    int stage = 0;
     int turn = 0;
-    for (int64_t round = 0; round < n; round += (int64_t)TILE * a.cluster, turn ^= 1) {
+    for (int64_t round = 0; round < n; round += stride, turn ^= 1) {
         const int64_t q = round + q_first;
         const int m = rows_from(q);
+        const bool all = all_there(q, m);
         W f[R][VEC], o[R][VEC], b[R][VEC]; // gate, 1 - gate, u or dh
+        V kx[R], ka[R];
+        asm volatile("cp.async.wait_group %0;" ::"n"(SCAN_STAGES - 2) : "memory");
+        auto open = [&](int i) {
+            const V rg = ld_vec<T, VEC>(at(stage, 0, i));
+            V rx, rd;
+            if constexpr (X)
+                rx = ld_vec<T, VEC>(at(stage, AT_X, i));
+            if constexpr (BACK)
+                rd = ld_vec<T, VEC>(at(stage, AT_D, i));
+#pragma unroll
+            for (int k = 0; k < VEC; k++) {
+                f[i][k] = widen(rg.v[k]);
+                if constexpr (SIGMOID)
+                    gate_pair(f[i][k], &f[i][k], &o[i][k]);
+                if constexpr (BACK)
+                    b[i][k] = widen(rd.v[k]);
+                else
+                    b[i][k] = SIGMOID ? o[i][k] * widen(rx.v[k]) : W(widen(rx.v[k]));
+            }
+            if constexpr (ABOVE) {
+                if constexpr (X)
+                    kx[i] = rx;
+                ka[i] = ld_vec<T, VEC>(at(stage, AT_ABOVE, i));
+            }
+        };
+        if (all) {
+#pragma unroll
+            for (int i = 0; i < R; i++)
+                open(i);
+        } else { // rows that are not there leave the state as it is
+#pragma unroll
+            for (int i = 0; i < R; i++) {
+                if (i < m)
+                    open(i);
+                else
+#pragma unroll
+                    for (int k = 0; k < VEC; k++) {
+                        f[i][k] = W(1);
+                        b[i][k] = W(0);
+                    }
+            }
+        }
+        // the stage that the round before has emptied
+        load(stage == 0 ? SCAN_STAGES - 1 : stage - 1, q + (SCAN_STAGES - 1) * stride);
+        stage = stage == SCAN_STAGES - 1 ? 0 : stage + 1;
         W A[VEC], B[VEC];
 #pragma unroll
         for (int k = 0; k < VEC; k++) {
-            A[k] = W(1);
-            B[k] = W(0);
+            A[k] = f[0][k];
+            B[k] = BACK ? f[0][k] * b[0][k] : b[0][k];
         }
-        V kx[R], ka[R];
 #pragma unroll
-        for (int i = 0; i < R; i++) {
-#pragma unroll
-            for (int k = 0; k < VEC; k++) {
-                f[i][k] = W(1);
-                o[i][k] = b[i][k] = W(0);
-            }
-            if (i < m) {
-#pragma unroll
-                for (int k = 0; k < VEC; k++) {
-                    f[i][k] = widen(rg[i].v[k]);
-                    if constexpr (SIGMOID)
-                        gate_pair(f[i][k], &f[i][k], &o[i][k]);
-                    if constexpr (BACK)
-                        b[i][k] = widen(rd[i].v[k]);
-                    else
-                        b[i][k] = SIGMOID ? o[i][k] * widen(rx[i].v[k]) : W(widen(rx[i].v[k]));
-                }
-            }
+        for (int i = 1; i < R; i++)
 #pragma unroll
             for (int k = 0; k < VEC; k++) {
                 B[k] = BACK ? f[i][k] * (B[k] + b[i][k]) : f[i][k] * B[k] + b[i][k];
                 A[k] *= f[i][k];
             }
-            if constexpr (BACK && !AGGREGATE) {
-                kx[i] = rx[i];
-                ka[i] = ra[i];
-            }
-        }
-        load(q + (int64_t)TILE * a.cluster); // on its way while the steps are exchanged
         put(agg[turn][warp], lane, A, B);
         __syncthreads(); // the halves of agg alternate: nobody writes this one again before the next barrier
         // the composed step of the warps in front of this one, and of the whole tile
         W fa[VEC], fb[VEC], va[VEC], v[VEC];
 #pragma unroll
         for (int k = 0; k < VEC; k++) {
-            fa[k] = W(1);
-            fb[k] = W(0);
+            fa[k] = va[k] = W(1);
+            fb[k] = v[k] = W(0);
         }
 #pragma unroll
         for (int w = 0; w < SCAN_WARPS; w++) {
-            const Vec<W, VEC> wa = ld_vec<W, VEC>(agg[turn][w].a + lane * VEC), wb = ld_vec<W, VEC>(agg[turn][w].b + lane * VEC);
+            W wa[VEC], wb[VEC];
 #pragma unroll
             for (int k = 0; k < VEC; k++) {
-                if (w == warp) {
-                    va[k] = fa[k];
+                wa[k] = agg[turn][w].a[lane * VEC + k];
+                wb[k] = agg[turn][w].b[lane * VEC + k];
+            }
+            if (w == warp) {
+#pragma unroll
+                for (int k = 0; k < VEC; k++) {
+                    va[k] = finite(fa[k]);
                     v[k] = fb[k];
                 }
-                fb[k] = step_state(wa.v[k], fb[k], wb.v[k]);
-                fa[k] *= wa.v[k];
+            }
+#pragma unroll
+            for (int k = 0; k < VEC; k++) {
+                fb[k] = wa[k] * fb[k] + wb[k];
+                fa[k] *= wa[k];
             }
         }
         if (a.cluster == 1) {
 #pragma unroll
             for (int k = 0; k < VEC; k++) {
-                v[k] = step_state(va[k], state[k], v[k]);
-                state[k] = step_state(fa[k], state[k], fb[k]);
-                prod[k] *= fa[k];
+                v[k] = va[k] * state[k] + v[k];
+                fa[k] = finite(fa[k]);
+                state[k] = fa[k] * state[k] + fb[k];
+                prod[k] = finite(prod[k] * fa[k]);
             }
         } else {
-            for (int t = warp; t < a.cluster; t += SCAN_WARPS) {
-                Steps<W, VEC> *there = cooperative_groups::this_cluster().map_shared_rank(&tiles[turn][rank], t);
-                put(*there, lane, fa, fb);
-            }
+            for (int t = warp; t < a.cluster; t += SCAN_WARPS)
+                put(*cooperative_groups::this_cluster().map_shared_rank(&tiles[turn][rank], t), lane, fa, fb);
             cooperative_groups::this_cluster().sync();
             W mine[VEC];
-            for (int t = 0; t < a.cluster; t++) {
-                const Vec<W, VEC> ta = ld_vec<W, VEC>(tiles[turn][t].a + lane * VEC), tb = ld_vec<W, VEC>(tiles[turn][t].b + lane * VEC);
 #pragma unroll
-                for (int k = 0; k < VEC; k++) {
-                    if (t == rank)
+            for (int k = 0; k < VEC; k++)
+                mine[k] = state[k];
+            for (int t = 0; t < a.cluster; t++) {
+                if (t == rank) {
+#pragma unroll
+                    for (int k = 0; k < VEC; k++)
                         mine[k] = state[k];
-                    state[k] = step_state(ta.v[k], state[k], tb.v[k]);
-                    prod[k] *= ta.v[k];
                 }
+#pragma unroll
+                for (int k = 0; k < VEC; k++)
+                    state[k] = tiles[turn][t].a[lane * VEC + k] * state[k] + tiles[turn][t].b[lane * VEC + k];
             }
 #pragma unroll
             for (int k = 0; k < VEC; k++)
-                v[k] = step_state(va[k], mine[k], v[k]);
+                v[k] = va[k] * mine[k] + v[k];
         }
         if constexpr (!AGGREGATE) {
-            const int64_t r = BACK ? first - q : first + q;
+            const int64_t r = first + dir * q;
+            auto close = [&](int i, bool top) {
+                V y, z;
+                if constexpr (!BACK) {
 #pragma unroll
-            for (int i = 0; i < R; i++)
-                if (i < m) {
-                    V y, z;
-                    if constexpr (!BACK) {
-#pragma unroll
-                        for (int k = 0; k < VEC; k++) {
-                            v[k] = f[i][k] * v[k] + b[i][k];
-                            y.v[k] = narrow<T>(v[k]);
-                        }
-                        st_vec<T, VEC>(a.h + (r + i) * a.h_ld + c, y);
-                    } else {
-                        W above[VEC];
-#pragma unroll
-                        for (int k = 0; k < VEC; k++)
-                            above[k] = widen(ka[i].v[k]);
-                        if (r - i == begin) {
-#pragma unroll
-                            for (int k = 0; k < VEC; k++)
-                                above[k] = a.h0 ? a.h0[seq * a.h0_ld + c + k] : W(0);
-                        }
-#pragma unroll
-                        for (int k = 0; k < VEC; k++) {
-                            const W delta = b[i][k] + v[k];
-                            v[k] = f[i][k] * delta;
-                            if constexpr (SIGMOID) {
-                                y.v[k] = narrow<T>(v[k] * (above[k] - widen(kx[i].v[k])) * o[i][k]);
-                                z.v[k] = narrow<T>(delta * o[i][k]);
-                            } else {
-                                y.v[k] = narrow<T>(delta * above[k]);
-                                z.v[k] = narrow<T>(delta);
-                            }
-                        }
-                        st_vec<T, VEC>(a.dg + (r - i) * a.dg_ld + c, y);
-                        st_vec<T, VEC>(a.dx + (r - i) * a.dx_ld + c, z);
+                    for (int k = 0; k < VEC; k++) {
+                        v[k] = f[i][k] * v[k] + b[i][k];
+                        y.v[k] = narrow<T>(v[k]);
                     }
+                    st_vec<T, VEC>(a.h + (r + i) * a.h_ld + c, y);
+                } else {
+                    W above[VEC];
+#pragma unroll
+                    for (int k = 0; k < VEC; k++)
+                        above[k] = !top ? W(widen(ka[i].v[k])) : (a.h0 ? a.h0[seq * a.h0_ld + c + k] : W(0));
+#pragma unroll
+                    for (int k = 0; k < VEC; k++) {
+                        const W delta = b[i][k] + v[k];
+                        v[k] = f[i][k] * delta;
+                        if constexpr (SIGMOID) {
+                            y.v[k] = narrow<T>(v[k] * ((above[k] - widen(kx[i].v[k])) * o[i][k]));
+                            z.v[k] = narrow<T>(delta * o[i][k]);
+                        } else {
+                            y.v[k] = narrow<T>(delta * above[k]);
+                            z.v[k] = narrow<T>(delta);
+                        }
+                    }
+                    st_vec<T, VEC>(a.dg + (r - i) * a.dg_ld + c, y);
+                    st_vec<T, VEC>(a.dx + (r - i) * a.dx_ld + c, z);
                 }
+            };
+            if (all) {
+#pragma unroll
+                for (int i = 0; i < R; i++)
+                    close(i, false);
+            } else {
+#pragma unroll
+                for (int i = 0; i < R; i++)
+                    if (i < m)
+                        close(i, BACK && r - i == begin);
+            }
         }
     }
     if (warp == 0 && rank == 0 && in) {
@@ -359,7 +419,6 @@ __global__ void __launch_bounds__(256)
 // fewer, the CTAs of a cluster take turns on a sequence's tiles, which reads the data once as before.  Where even
 // clusters leave most SMs without work (few columns, one long sequence), sequences are cut into blocks instead: a first
 // pass composes the blocks' steps, the second one has its inputs from L2 when they fit there.
-template <typename T> constexpr int widest() { return sizeof(T) == 2 ? 2 : 1; }
 struct ScanPlan {
     int blocks, cluster;
 };
@@ -367,10 +426,10 @@ ScanPlan scan_plan(size_t es, int64_t rows, int64_t cols, int64_t seqs) {
     ScanPlan p{1, 1};
     if (rows <= 0 || cols <= 0 || seqs <= 0)
         return p;
-    const int64_t columns = es == 2 ? 64 : 32, strips = (cols + columns - 1) / columns, ctas = strips * seqs;
-    const int64_t tile = 64, tiles = rows / seqs / tile, full = (int64_t)sm_count() * 4;
+    const int64_t columns = 32 * 8 / (int64_t)es, strips = (cols + columns - 1) / columns, ctas = strips * seqs;
+    const int64_t tile = 32, tiles = rows / seqs / tile, full = (int64_t)sm_count() * 4;
     if (ctas * SCAN_CLUSTER >= sm_count() * 2 || tiles < 4 * SCAN_CLUSTER) {
-        while (p.cluster < SCAN_CLUSTER && ctas * p.cluster < full && p.cluster * 2 <= tiles)
+        while (p.cluster < SCAN_CLUSTER && ctas * p.cluster < full && p.cluster * 4 <= tiles)
             p.cluster *= 2;
         return p;
     }
@@ -384,22 +443,26 @@ template <typename T, int VEC, bool BACK, bool SIGMOID> int scan_launch(ScanArgs
     a.strips = (a.cols + 32 * VEC - 1) / (32 * VEC);
     const int64_t ctas = a.strips * a.blocks * a.seqs * a.cluster;
     DB2_CHECK(ctas < ((int64_t)1 << 31), DB2_EUNSUPPORTED, "gatedScan: too many sequences and columns for one launch");
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = (unsigned)a.cluster;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)ctas);
-    cfg.blockDim = dim3(SCAN_THREADS);
-    cfg.stream = st;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    if (a.blocks > 1) {
-        DB2_CUDA(cudaLaunchKernelEx(&cfg, gated_scan_kernel<T, VEC, BACK, SIGMOID, true>, a));
-        DB2_TRY(after_launch("gated_scan_kernel"));
-    }
-    DB2_CUDA(cudaLaunchKernelEx(&cfg, gated_scan_kernel<T, VEC, BACK, SIGMOID, false>, a));
-    return after_launch("gated_scan_kernel");
+    auto launch = [&](auto kernel, int operands) -> int {
+        const size_t smem = (size_t)SCAN_STAGES * operands * SCAN_WARPS * scan_rows<BACK>() * 32 * VEC * sizeof(T);
+        DB2_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = (unsigned)a.cluster;
+        attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+        cudaLaunchConfig_t cfg{};
+        cfg.gridDim = dim3((unsigned)ctas);
+        cfg.blockDim = dim3(SCAN_THREADS);
+        cfg.dynamicSmemBytes = smem;
+        cfg.stream = st;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        DB2_CUDA(cudaLaunchKernelEx(&cfg, kernel, a));
+        return after_launch("gated_scan_kernel");
+    };
+    if (a.blocks > 1)
+        DB2_TRY(launch(gated_scan_kernel<T, VEC, BACK, SIGMOID, true>, 2));
+    return launch(gated_scan_kernel<T, VEC, BACK, SIGMOID, false>, BACK ? (SIGMOID ? 4 : 3) : 2);
 }
 
 template <typename T, bool BACK> int scan_any(const ScanArgs<T> &a, int gate, bool packed, cudaStream_t st) {
