@@ -17,20 +17,16 @@
 #include "runtime.h"
 #include "seq.cuh"
 
-#include <cooperative_groups.h>
-
 namespace db2 {
 
 namespace {
 
-constexpr int SCAN_WARPS = 4, SCAN_THREADS = SCAN_WARPS * 32;
 // A lane takes 8 bytes of a row, a warp SCAN_R consecutive rows at once.  More rows would spread the exchange between the
 // warps over more work, but the gates and inputs of a thread's rows have to stay in its registers.
 template <typename T> constexpr int widest() { return 8 / sizeof(T); }
 template <bool BACK> constexpr int scan_rows() { return BACK ? 4 : 8; }
-// Rows on their way lie in shared memory, SCAN_STAGES tiles of them, copied asynchronously.
+// Rows on their way lie in shared memory, so many tiles (rows of all warps) of them, copied asynchronously.
 constexpr int SCAN_STAGES = 3;
-constexpr int SCAN_CLUSTER = 4; // most CTAs of a cluster
 
 template <typename T> struct ScanArgs {
     using W = wide_t<T>;
@@ -42,8 +38,7 @@ template <typename T> struct ScanArgs {
     const int64_t *off;
     int64_t g_ld, x_ld, grad_ld, above_ld, h_ld, dg_ld, dx_ld, h0_ld, init_ld, last_ld, part_ld;
     int64_t rows, cols, seqs, strips;
-    int blocks;  // blocks that a sequence is cut into, by a pass of its own
-    int cluster; // CTAs that take turns on the tiles of a block
+    int blocks; // blocks that a sequence is cut into, with a pass of its own
 };
 
 // rows of sequence s; offsets outside [0, rows] or that go back give fewer rows, never others' memory
@@ -104,24 +99,22 @@ template <typename W, int VEC> __device__ __forceinline__ void put(Steps<W, VEC>
     }
 }
 
-// CTA (sequence, strip of 32 x VEC columns, block of rows, rank within its cluster).  AGGREGATE: only (A, B) of the
-// block, into part.  Otherwise the results; the state that enters a block is init, advanced by part of the blocks in
-// front of it.  The CTAs of a cluster take the tiles of their block in turns: rank k has tile k, k + cluster, ...; in
-// every round each of them sends the composed step of its tile to all of them, so that all know the state that enters
-// each tile, and the data is still read once.
-template <typename T, int VEC, bool BACK, bool SIGMOID, bool AGGREGATE>
-__global__ void __launch_bounds__(SCAN_THREADS, 3) gated_scan_kernel(ScanArgs<T> a) {
+// CTA (sequence, strip of 32 x VEC columns, block of rows).  AGGREGATE: only (A, B) of the block, into part.  Otherwise the
+// results; the state that enters a block is init, advanced by part of the blocks in front of it.
+// Registers: three CTAs of four warps, or one of eight, on an SM.  With 128 registers a thread, four CTAs fit, but the
+// loads of a tile no longer stand together in front of their uses: 30000 x 2560 f16 in 37 sequences takes 135 us instead
+// of 105, 8 x 4096 x 2048 bf16 (forward and backward, eight warps) 385 instead of 266.
+template <typename T, int VEC, int WARPS, bool BACK, bool SIGMOID, bool AGGREGATE>
+__global__ void __launch_bounds__(WARPS * 32, WARPS == 4 ? 3 : 1) gated_scan_kernel(ScanArgs<T> a) {
     using W = wide_t<T>;
     using V = Vec<T, VEC>;
-    constexpr int R = scan_rows<BACK>(), TILE = SCAN_WARPS * R;
+    constexpr int R = scan_rows<BACK>(), TILE = WARPS * R, STAGES = SCAN_STAGES;
     // operands that are read, and where they stand in a stage
     constexpr bool X = !BACK || (SIGMOID && !AGGREGATE), ABOVE = BACK && !AGGREGATE;
     constexpr int AT_X = 1, AT_D = X ? 2 : 1, AT_ABOVE = AT_D + 1, OPERANDS = 1 + X + BACK + ABOVE;
-    __shared__ __align__(16) Steps<W, VEC> agg[2][SCAN_WARPS];
-    __shared__ __align__(16) Steps<W, VEC> tiles[2][SCAN_CLUSTER];
+    __shared__ __align__(16) Steps<W, VEC> agg[2][WARPS];
     const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-    const int rank = (int)(blockIdx.x % a.cluster);
-    const int64_t id = blockIdx.x / a.cluster, strip = id % a.strips, rest = id / a.strips;
+    const int64_t strip = blockIdx.x % a.strips, rest = blockIdx.x / a.strips;
     const int64_t blk = rest % a.blocks, seq = rest / a.blocks;
     const int64_t c = (strip * 32 + lane) * VEC;
     const bool in = c < a.cols; // cols is a multiple of VEC
@@ -138,8 +131,8 @@ __global__ void __launch_bounds__(SCAN_THREADS, 3) gated_scan_kernel(ScanArgs<T>
         prod[k] = W(1);
         state[k] = !AGGREGATE && in && a.init ? a.init[seq * a.init_ld + c + k] : W(0);
     }
-    if (!AGGREGATE && blk > 0) { // the blocks in front: a quarter for each warp, then the four quarters in order
-        const int64_t share = (blk + SCAN_WARPS - 1) / SCAN_WARPS, b0 = warp * share, b1 = b0 + share < blk ? b0 + share : blk;
+    if (!AGGREGATE && blk > 0) { // the blocks in front: a share for each warp, then the shares in order
+        const int64_t share = (blk + WARPS - 1) / WARPS, b0 = warp * share, b1 = b0 + share < blk ? b0 + share : blk;
         const W *p = a.part + (seq * a.blocks + b0) * 2 * a.part_ld + c;
         W A[VEC], B[VEC];
 #pragma unroll
@@ -148,7 +141,7 @@ __global__ void __launch_bounds__(SCAN_THREADS, 3) gated_scan_kernel(ScanArgs<T>
             B[k] = W(0);
         }
         if (in) {
-#pragma unroll 8
+#pragma unroll 16
             for (int64_t b = b0; b < b1; b++, p += 2 * a.part_ld)
 #pragma unroll
                 for (int k = 0; k < VEC; k++) {
@@ -159,13 +152,13 @@ __global__ void __launch_bounds__(SCAN_THREADS, 3) gated_scan_kernel(ScanArgs<T>
         put(agg[1][warp], lane, A, B); // the first tile uses the other half
         __syncthreads();
 #pragma unroll
-        for (int w = 0; w < SCAN_WARPS; w++)
+        for (int w = 0; w < WARPS; w++)
 #pragma unroll
             for (int k = 0; k < VEC; k++)
                 state[k] = agg[1][w].a[lane * VEC + k] * state[k] + agg[1][w].b[lane * VEC + k];
     }
     // Row q of the block lies q leading dimensions behind the first one, or in front of it.
-    const int64_t dir = BACK ? -1 : 1, q_first = (int64_t)rank * TILE + warp * R, stride = (int64_t)TILE * a.cluster;
+    const int64_t dir = BACK ? -1 : 1, q_first = warp * R;
     const int64_t r_first = first + dir * q_first;
     const T *pg = a.g + r_first * a.g_ld + c;
     const T *px = X ? a.x + r_first * a.x_ld + c : nullptr;
@@ -173,7 +166,7 @@ __global__ void __launch_bounds__(SCAN_THREADS, 3) gated_scan_kernel(ScanArgs<T>
     const T *pa = ABOVE ? a.above + (r_first - 1) * a.above_ld + c : nullptr;
     // a thread reads nothing from the stages but what it fetched itself: they need no barrier
     extern __shared__ __align__(16) unsigned char stage_mem[];
-    T *mine_at = reinterpret_cast<T *>(stage_mem) + (int64_t)warp * SCAN_STAGES * OPERANDS * R * 32 * VEC + lane * VEC;
+    T *mine_at = reinterpret_cast<T *>(stage_mem) + (int64_t)warp * STAGES * OPERANDS * R * 32 * VEC + lane * VEC;
     auto at = [&](int stage, int operand, int i) { return mine_at + ((stage * OPERANDS + operand) * R + i) * 32 * VEC; };
     // rows that are there of the R from row q on, for this lane; all: for all lanes, and none is the sequence's first one
     auto rows_from = [&](int64_t q) { return !in || q >= n ? 0 : (n - q < R ? (int)(n - q) : R); };
@@ -203,25 +196,25 @@ __global__ void __launch_bounds__(SCAN_THREADS, 3) gated_scan_kernel(ScanArgs<T>
                     load_row(stage, i, first - q - i > begin);
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
-        pg += stride * dir * a.g_ld;
+        pg += TILE * dir * a.g_ld;
         if constexpr (X)
-            px += stride * dir * a.x_ld;
+            px += TILE * dir * a.x_ld;
         if constexpr (BACK)
-            pd -= stride * a.grad_ld;
+            pd -= TILE * a.grad_ld;
         if constexpr (ABOVE)
-            pa -= stride * a.above_ld;
+            pa -= TILE * a.above_ld;
     };
-    for (int k = 0; k < SCAN_STAGES - 1; k++)
-        load(k, q_first + k * stride);
+    for (int k = 0; k < STAGES - 1; k++)
+        load(k, q_first + k * TILE);
     int stage = 0;
     int turn = 0;
-    for (int64_t round = 0; round < n; round += stride, turn ^= 1) {
+    for (int64_t round = 0; round < n; round += TILE, turn ^= 1) {
         const int64_t q = round + q_first;
         const int m = rows_from(q);
         const bool all = all_there(q, m);
         W f[R][VEC], o[R][VEC], b[R][VEC]; // gate, 1 - gate, u or dh
         V kx[R], ka[R];
-        asm volatile("cp.async.wait_group %0;" ::"n"(SCAN_STAGES - 2) : "memory");
+        asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
         auto open = [&](int i) {
             const V rg = ld_vec<T, VEC>(at(stage, 0, i));
             V rx, rd;
@@ -263,8 +256,8 @@ __global__ void __launch_bounds__(SCAN_THREADS, 3) gated_scan_kernel(ScanArgs<T>
             }
         }
         // the stage that the round before has emptied
-        load(stage == 0 ? SCAN_STAGES - 1 : stage - 1, q + (SCAN_STAGES - 1) * stride);
-        stage = stage == SCAN_STAGES - 1 ? 0 : stage + 1;
+        load(stage == 0 ? STAGES - 1 : stage - 1, q + (STAGES - 1) * TILE);
+        stage = stage == STAGES - 1 ? 0 : stage + 1;
         W A[VEC], B[VEC];
 #pragma unroll
         for (int k = 0; k < VEC; k++) {
@@ -280,63 +273,20 @@ __global__ void __launch_bounds__(SCAN_THREADS, 3) gated_scan_kernel(ScanArgs<T>
             }
         put(agg[turn][warp], lane, A, B);
         __syncthreads(); // the halves of agg alternate: nobody writes this one again before the next barrier
-        // the composed step of the warps in front of this one, and of the whole tile
-        W fa[VEC], fb[VEC], va[VEC], v[VEC];
+        W v[VEC];
 #pragma unroll
-        for (int k = 0; k < VEC; k++) {
-            fa[k] = va[k] = W(1);
-            fb[k] = v[k] = W(0);
-        }
-#pragma unroll
-        for (int w = 0; w < SCAN_WARPS; w++) {
-            W wa[VEC], wb[VEC];
-#pragma unroll
-            for (int k = 0; k < VEC; k++) {
-                wa[k] = agg[turn][w].a[lane * VEC + k];
-                wb[k] = agg[turn][w].b[lane * VEC + k];
-            }
+        for (int w = 0; w < WARPS; w++) {
             if (w == warp) {
 #pragma unroll
-                for (int k = 0; k < VEC; k++) {
-                    va[k] = finite(fa[k]);
-                    v[k] = fb[k];
-                }
-            }
-#pragma unroll
-            for (int k = 0; k < VEC; k++) {
-                fb[k] = wa[k] * fb[k] + wb[k];
-                fa[k] *= wa[k];
-            }
-        }
-        if (a.cluster == 1) {
-#pragma unroll
-            for (int k = 0; k < VEC; k++) {
-                v[k] = va[k] * state[k] + v[k];
-                fa[k] = finite(fa[k]);
-                state[k] = fa[k] * state[k] + fb[k];
-                prod[k] = finite(prod[k] * fa[k]);
-            }
-        } else {
-            for (int t = warp; t < a.cluster; t += SCAN_WARPS)
-                put(*cooperative_groups::this_cluster().map_shared_rank(&tiles[turn][rank], t), lane, fa, fb);
-            cooperative_groups::this_cluster().sync();
-            W mine[VEC];
-#pragma unroll
-            for (int k = 0; k < VEC; k++)
-                mine[k] = state[k];
-            for (int t = 0; t < a.cluster; t++) {
-                if (t == rank) {
-#pragma unroll
-                    for (int k = 0; k < VEC; k++)
-                        mine[k] = state[k];
-                }
-#pragma unroll
                 for (int k = 0; k < VEC; k++)
-                    state[k] = tiles[turn][t].a[lane * VEC + k] * state[k] + tiles[turn][t].b[lane * VEC + k];
+                    v[k] = state[k];
             }
 #pragma unroll
-            for (int k = 0; k < VEC; k++)
-                v[k] = va[k] * mine[k] + v[k];
+            for (int k = 0; k < VEC; k++) {
+                state[k] = agg[turn][w].a[lane * VEC + k] * state[k] + agg[turn][w].b[lane * VEC + k];
+                if constexpr (AGGREGATE)
+                    prod[k] = finite(prod[k] * agg[turn][w].a[lane * VEC + k]);
+            }
         }
         if constexpr (!AGGREGATE) {
             const int64_t r = first + dir * q;
@@ -382,7 +332,7 @@ __global__ void __launch_bounds__(SCAN_THREADS, 3) gated_scan_kernel(ScanArgs<T>
             }
         }
     }
-    if (warp == 0 && rank == 0 && in) {
+    if (warp == 0 && in) {
         W *p = a.part + (seq * a.blocks + blk) * 2 * a.part_ld + c;
 #pragma unroll
         for (int k = 0; k < VEC; k++) {
@@ -414,62 +364,69 @@ __global__ void __launch_bounds__(256)
         }
 }
 
-// How a sequence is shared out, from the shape and the number of SMs alone (both directions share the scratch).
-// `ctas` = sequences x strips of columns work independently.  Four CTAs on every SM keep enough loads in flight; with
-// fewer, the CTAs of a cluster take turns on a sequence's tiles, which reads the data once as before.  Where even
-// clusters leave most SMs without work (few columns, one long sequence), sequences are cut into blocks instead: a first
-// pass composes the blocks' steps, the second one has its inputs from L2 when they fit there.
+// How sequences are shared out, from the shape and the number of SMs alone (both directions share the scratch).  `ctas` =
+// sequences x strips of columns work independently.  Four warps each when there are more of them than SMs, eight
+// otherwise.  Where they leave more than half of the SMs without work (few columns, few sequences), sequences are cut into
+// blocks: a first pass composes the blocks' steps, and the second one reads the inputs again, from L2 when they fit there.
 struct ScanPlan {
-    int blocks, cluster;
+    int blocks, warps;
+    bool packed; // lanes take 8 bytes
 };
-ScanPlan scan_plan(size_t es, int64_t rows, int64_t cols, int64_t seqs) {
-    ScanPlan p{1, 1};
-    if (rows <= 0 || cols <= 0 || seqs <= 0)
-        return p;
-    const int64_t columns = 32 * 8 / (int64_t)es, strips = (cols + columns - 1) / columns, ctas = strips * seqs;
-    const int64_t tile = 32, tiles = rows / seqs / tile, full = (int64_t)sm_count() * 4;
-    if (ctas * SCAN_CLUSTER >= sm_count() * 2 || tiles < 4 * SCAN_CLUSTER) {
-        while (p.cluster < SCAN_CLUSTER && ctas * p.cluster < full && p.cluster * 4 <= tiles)
-            p.cluster *= 2;
+template <typename T> ScanPlan scan_plan(int64_t rows, int64_t cols, int64_t seqs, bool aligned) {
+    ScanPlan p{1, 4, aligned};
+    const int64_t sms = sm_count();
+    auto strips = [&](int64_t vec) { return (cols + 32 * vec - 1) / (32 * vec); };
+    int64_t ctas = strips(widest<T>()) * seqs; // of whole lanes, aligned or not: the scratch is asked for without pointers
+    if (ctas * 2 >= sms || rows / seqs < 1024) {
+        p.warps = (aligned ? ctas : strips(1) * seqs) <= sms ? 8 : 4;
         return p;
     }
-    const int64_t want = (full + ctas - 1) / ctas, most = tiles / 4;
-    const int64_t b = want < most ? want : most;
-    p.blocks = (int)(b > 1024 ? 1024 : b);
+    // a narrow matrix leaves lanes of its last strip without columns: single elements waste fewer
+    p.packed = aligned && cols % (32 * widest<T>()) == 0;
+    const int64_t want = sms * 3 / ctas, most = rows / seqs / 256;
+    p.blocks = (int)(want < most ? want : most);
     return p;
 }
 
-template <typename T, int VEC, bool BACK, bool SIGMOID> int scan_launch(ScanArgs<T> a, cudaStream_t st) {
+template <typename T, int VEC, int WARPS, bool BACK, bool SIGMOID> int scan_launch(ScanArgs<T> a, cudaStream_t st) {
     a.strips = (a.cols + 32 * VEC - 1) / (32 * VEC);
-    const int64_t ctas = a.strips * a.blocks * a.seqs * a.cluster;
+    const int64_t ctas = a.strips * a.blocks * a.seqs;
     DB2_CHECK(ctas < ((int64_t)1 << 31), DB2_EUNSUPPORTED, "gatedScan: too many sequences and columns for one launch");
-    auto launch = [&](auto kernel, int operands) -> int {
-        const size_t smem = (size_t)SCAN_STAGES * operands * SCAN_WARPS * scan_rows<BACK>() * 32 * VEC * sizeof(T);
-        DB2_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-        cudaLaunchAttribute attr[1];
-        attr[0].id = cudaLaunchAttributeClusterDimension;
-        attr[0].val.clusterDim.x = (unsigned)a.cluster;
-        attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-        cudaLaunchConfig_t cfg{};
-        cfg.gridDim = dim3((unsigned)ctas);
-        cfg.blockDim = dim3(SCAN_THREADS);
-        cfg.dynamicSmemBytes = smem;
-        cfg.stream = st;
-        cfg.attrs = attr;
-        cfg.numAttrs = 1;
-        DB2_CUDA(cudaLaunchKernelEx(&cfg, kernel, a));
-        return after_launch("gated_scan_kernel");
-    };
-    if (a.blocks > 1)
-        DB2_TRY(launch(gated_scan_kernel<T, VEC, BACK, SIGMOID, true>, 2));
-    return launch(gated_scan_kernel<T, VEC, BACK, SIGMOID, false>, BACK ? (SIGMOID ? 4 : 3) : 2);
+    constexpr size_t stage = (size_t)SCAN_STAGES * WARPS * scan_rows<BACK>() * 32 * VEC * sizeof(T);
+    constexpr int operands = BACK ? (SIGMOID ? 4 : 3) : 2;
+    auto whole = gated_scan_kernel<T, VEC, WARPS, BACK, SIGMOID, false>;
+    auto aggregate = gated_scan_kernel<T, VEC, 4, BACK, SIGMOID, true>;
+    static PerDeviceOnce once;
+    if (once.need()) {
+        DB2_CUDA(cudaFuncSetAttribute(whole, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(stage * operands)));
+        DB2_CUDA(cudaFuncSetAttribute(aggregate, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(stage * 2)));
+        once.mark();
+    }
+    if constexpr (WARPS == 4)
+        if (a.blocks > 1) {
+            aggregate<<<(unsigned)ctas, 128, stage * 2, st>>>(a);
+            DB2_TRY(after_launch("gated_scan_kernel"));
+        }
+    whole<<<(unsigned)ctas, WARPS * 32, stage * operands, st>>>(a);
+    return after_launch("gated_scan_kernel");
 }
 
-template <typename T, bool BACK> int scan_any(const ScanArgs<T> &a, int gate, bool packed, cudaStream_t st) {
+template <typename T, bool BACK> int scan_any(ScanArgs<T> &a, int gate, bool aligned, cudaStream_t st) {
     constexpr int N = widest<T>();
-    if (packed)
-        return gate == DB2_GATE_SIGMOID ? scan_launch<T, N, BACK, true>(a, st) : scan_launch<T, N, BACK, false>(a, st);
-    return gate == DB2_GATE_SIGMOID ? scan_launch<T, 1, BACK, true>(a, st) : scan_launch<T, 1, BACK, false>(a, st);
+    const ScanPlan p = scan_plan<T>(a.rows, a.cols, a.seqs, aligned);
+    a.blocks = p.blocks;
+    const bool s = gate == DB2_GATE_SIGMOID;
+#define DB2_SCAN(VEC, WARPS)                                                                                           \
+    return s ? scan_launch<T, VEC, WARPS, BACK, true>(a, st) : scan_launch<T, VEC, WARPS, BACK, false>(a, st)
+    if (p.packed) {
+        if (p.warps == 8)
+            DB2_SCAN(N, 8);
+        DB2_SCAN(N, 4);
+    }
+    if (p.warps == 8)
+        DB2_SCAN(1, 8);
+    DB2_SCAN(1, 4);
+#undef DB2_SCAN
 }
 
 bool seq_type(int dtype) {
@@ -544,7 +501,11 @@ extern "C" {
 size_t db2k_gated_scan_scratch_bytes(int dtype, int64_t rows, int64_t cols, int64_t seqs) {
     if (rows <= 0 || cols <= 0 || seqs <= 0)
         return 0;
-    const int blocks = scan_plan(dtype_size(dtype), rows, cols, seqs).blocks;
+    const int es = (int)dtype_size(dtype);
+    const int blocks = (es == 8   ? scan_plan<double>(rows, cols, seqs, true)
+                        : es == 4 ? scan_plan<float>(rows, cols, seqs, true)
+                                  : scan_plan<__half>(rows, cols, seqs, true))
+                           .blocks;
     return blocks < 2 ? 0 : (size_t)seqs * blocks * 2 * scan_part_ld(cols) * (dtype == DB2_F64 ? 8 : 4);
 }
 
@@ -580,9 +541,6 @@ int db2k_gated_scan(int dtype, int gate, const void *g, int64_t g_ld, const void
         a.rows = rows;
         a.cols = cols;
         a.seqs = seqs;
-        const ScanPlan plan = scan_plan(sizeof(T), rows, cols, seqs);
-        a.blocks = plan.blocks;
-        a.cluster = plan.cluster;
         constexpr size_t al = sizeof(T) * widest<T>();
         const bool packed = cols % widest<T>() == 0 && rows_aligned(g, g_ld, sizeof(T), al) &&
                             rows_aligned(x, x_ld, sizeof(T), al) && rows_aligned(h, h_ld, sizeof(T), al);
@@ -636,9 +594,6 @@ int db2k_gated_scan_grad(int dtype, int gate, const void *g, int64_t g_ld, const
         a.rows = rows;
         a.cols = cols;
         a.seqs = seqs;
-        const ScanPlan plan = scan_plan(sizeof(T), rows, cols, seqs);
-        a.blocks = plan.blocks;
-        a.cluster = plan.cluster;
         constexpr size_t al = sizeof(T) * widest<T>();
         const bool packed = cols % widest<T>() == 0 && rows_aligned(g, g_ld, sizeof(T), al) &&
                             (!sigmoid || rows_aligned(x, x_ld, sizeof(T), al)) && rows_aligned(h, h_ld, sizeof(T), al) &&
