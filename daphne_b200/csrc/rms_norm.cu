@@ -42,33 +42,6 @@ template <typename W, int BLOCK> struct RowSum {
     }
 };
 
-// packet p (N columns) of a row; the last one may be narrower
-template <typename T, int N> __device__ __forceinline__ Vec<T, N> load_packet(const T *row, int64_t p, int64_t cols) {
-    const int64_t c = p * N;
-    if constexpr (N > 1)
-        if (c + N > cols) {
-            Vec<T, N> x;
-#pragma unroll
-            for (int k = 0; k < N; k++)
-                x.v[k] = c + k < cols ? row[c + k] : narrow<T>(0.0f);
-            return x;
-        }
-    return ld_vec<T, N>(row + c);
-}
-template <typename T, int N>
-__device__ __forceinline__ void store_packet(T *row, int64_t p, int64_t cols, const Vec<T, N> &x) {
-    const int64_t c = p * N;
-    if constexpr (N > 1)
-        if (c + N > cols) {
-#pragma unroll
-            for (int k = 0; k < N; k++)
-                if (c + k < cols)
-                    row[c + k] = x.v[k];
-            return;
-        }
-    st_vec<T, N>(row + c, x);
-}
-
 template <typename T> struct NormArgs { // x, residual and sum may be the same matrix, and res one of x and residual
     const T *x, *residual, *weight;
     T *sum;
@@ -96,13 +69,12 @@ template <typename T, int N> __device__ __forceinline__ void squares(const Vec<T
         *ss += v * v;
     }
 }
-// y of a packet; columns behind the end give 0 (their s is 0)
+// y of packet p
 template <typename T, int N>
-__device__ __forceinline__ void normalised(const Vec<T, N> &s, const T *weight, int64_t p, int64_t cols, wide_t<T> rstd,
-                                           wide_t<T> *y) {
+__device__ __forceinline__ void normalised(const Vec<T, N> &s, const T *weight, int64_t p, wide_t<T> rstd, wide_t<T> *y) {
     Vec<T, N> w;
     if (weight)
-        w = load_packet<T, N>(weight, p, cols);
+        w = ld_vec<T, N>(weight + p * N);
 #pragma unroll
     for (int k = 0; k < N; k++)
         y[k] = weight ? widen(s.v[k]) * rstd * widen(w.v[k]) : widen(s.v[k]) * rstd;
@@ -125,13 +97,20 @@ __device__ __forceinline__ float scale_of(unsigned most) {
         return m;
     return fmaxf(m / E4M3_MAX, 1.17549435e-38f);
 }
-template <int N>
-__device__ __forceinline__ void store_q8(void *res, int64_t at, int64_t p, int64_t cols, const float *y, float inv) {
+template <int N> __device__ __forceinline__ void store_q8(void *res, int64_t at, const float *y, float inv) {
     Vec<__nv_fp8_storage_t, N> q;
+    if constexpr (N == 1)
+        q.v[0] = __nv_cvt_float_to_fp8(y[0] * inv, __NV_SATFINITE, __NV_E4M3);
+    else {
 #pragma unroll
-    for (int k = 0; k < N; k++)
-        q.v[k] = __nv_cvt_float_to_fp8(y[k] * inv, __NV_SATFINITE, __NV_E4M3);
-    store_packet<__nv_fp8_storage_t, N>(static_cast<__nv_fp8_storage_t *>(res) + at, p, cols, q);
+        for (int k = 0; k < N; k += 2) {
+            const __nv_fp8x2_storage_t two =
+                __nv_cvt_float2_to_fp8x2(make_float2(y[k] * inv, y[k + 1] * inv), __NV_SATFINITE, __NV_E4M3);
+            q.v[k] = (__nv_fp8_storage_t)(two & 0xff);
+            q.v[k + 1] = (__nv_fp8_storage_t)(two >> 8);
+        }
+    }
+    st_vec<__nv_fp8_storage_t, N>(static_cast<__nv_fp8_storage_t *>(res) + at, q);
 }
 
 // Rows of up to tpr * PPT packets: a thread holds packets tx, tx + tpr, ... of its row.
@@ -141,7 +120,7 @@ __global__ void __launch_bounds__(BLOCK) norm_rows_kernel(NormArgs<T> a, int log
     __shared__ W red[2 * (BLOCK / 32)];
     extern __shared__ unsigned group_max[]; // rows of the CTA x groups (8-bit results whose groups span warps)
     const int tpr = 1 << log_tpr, tx = threadIdx.x & (tpr - 1), ty = threadIdx.x >> log_tpr, at_once = BLOCK >> log_tpr;
-    const int64_t packets = (a.cols + N - 1) / N;
+    const int packets = (int)(a.cols / N); // cols is a multiple of N
     RowSum<W, BLOCK> row_sum{red};
     for (int64_t r0 = (int64_t)blockIdx.x * at_once; r0 < a.rows; r0 += (int64_t)gridDim.x * at_once) {
         const int64_t r = r0 + ty;
@@ -152,14 +131,14 @@ __global__ void __launch_bounds__(BLOCK) norm_rows_kernel(NormArgs<T> a, int log
 #pragma unroll
             for (int k = 0; k < PPT; k++)
                 if (tx + k * tpr < packets)
-                    s[k] = load_packet<T, N>(x, tx + k * tpr, a.cols);
+                    s[k] = ld_vec<T, N>(x + (tx + k * tpr) * N);
             if (a.residual) {
                 const T *res = a.residual + r * a.residual_ld;
                 Vec<T, N> y[PPT];
 #pragma unroll
                 for (int k = 0; k < PPT; k++)
                     if (tx + k * tpr < packets)
-                        y[k] = load_packet<T, N>(res, tx + k * tpr, a.cols);
+                        y[k] = ld_vec<T, N>(res + (tx + k * tpr) * N);
 #pragma unroll
                 for (int k = 0; k < PPT; k++)
                     s[k] = add_residual(s[k], y[k]);
@@ -169,7 +148,7 @@ __global__ void __launch_bounds__(BLOCK) norm_rows_kernel(NormArgs<T> a, int log
 #pragma unroll
                 for (int k = 0; k < PPT; k++)
                     if (tx + k * tpr < packets)
-                        store_packet<T, N>(sum, tx + k * tpr, a.cols, s[k]);
+                        st_vec<T, N>(sum + (tx + k * tpr) * N, s[k]);
             }
         }
         W ss = 0;
@@ -187,12 +166,12 @@ __global__ void __launch_bounds__(BLOCK) norm_rows_kernel(NormArgs<T> a, int log
                 for (int k = 0; k < PPT; k++)
                     if (tx + k * tpr < packets) {
                         W y[N];
-                        normalised<T, N>(s[k], a.weight, tx + k * tpr, a.cols, rstd, y);
+                        normalised<T, N>(s[k], a.weight, tx + k * tpr, rstd, y);
                         Vec<T, N> z;
 #pragma unroll
                         for (int j = 0; j < N; j++)
                             z.v[j] = narrow<T>(y[j]);
-                        store_packet<T, N>(res, tx + k * tpr, a.cols, z);
+                        st_vec<T, N>(res + (tx + k * tpr) * N, z);
                     }
             }
         } else {
@@ -202,7 +181,7 @@ __global__ void __launch_bounds__(BLOCK) norm_rows_kernel(NormArgs<T> a, int log
             for (int k = 0; k < PPT; k++) {
                 most[k] = 0;
                 if (live && tx + k * tpr < packets) {
-                    normalised<T, N>(s[k], a.weight, tx + k * tpr, a.cols, rstd, y[k]);
+                    normalised<T, N>(s[k], a.weight, tx + k * tpr, rstd, y[k]);
                     most[k] = largest<N>(y[k]);
                 }
             }
@@ -230,12 +209,12 @@ __global__ void __launch_bounds__(BLOCK) norm_rows_kernel(NormArgs<T> a, int log
 #pragma unroll
                 for (int k = 0; k < PPT; k++)
                     if (live && tx + k * tpr < packets && (tx & (lanes - 1)) == 0)
-                        atomicMax(&gm[a.group == 0 ? 0 : (int64_t)(tx + k * tpr) * N / a.group], most[k]);
+                        atomicMax(&gm[a.group == 0 ? 0 : (tx + k * tpr) * N / (int)a.group], most[k]);
                 __syncthreads();
 #pragma unroll
                 for (int k = 0; k < PPT; k++)
                     if (tx + k * tpr < packets)
-                        most[k] = gm[a.group == 0 ? 0 : (int64_t)(tx + k * tpr) * N / a.group];
+                        most[k] = gm[a.group == 0 ? 0 : (tx + k * tpr) * N / (int)a.group];
                 __syncthreads();
             }
             if (live) {
@@ -243,10 +222,10 @@ __global__ void __launch_bounds__(BLOCK) norm_rows_kernel(NormArgs<T> a, int log
                 for (int k = 0; k < PPT; k++)
                     if (tx + k * tpr < packets) {
                         const float scale = scale_of(most[k]);
-                        const int64_t c = (int64_t)(tx + k * tpr) * N;
-                        if (a.group == 0 ? c == 0 : c % a.group == 0)
-                            a.scales[r * a.scales_ld + (a.group == 0 ? 0 : c / a.group)] = scale;
-                        store_q8<N>(a.res, r * a.res_ld, tx + k * tpr, a.cols, y[k], 1.0f / scale);
+                        const int c = (tx + k * tpr) * N, group = (int)a.group;
+                        if (group == 0 ? c == 0 : (c & (group - 1)) == 0)
+                            a.scales[r * a.scales_ld + (group == 0 ? 0 : c / group)] = scale;
+                        store_q8<N>(a.res, r * a.res_ld + c, y[k], 1.0f / scale);
                     }
             }
         }
@@ -261,22 +240,22 @@ __global__ void __launch_bounds__(LONG_BLOCK) norm_long_kernel(NormArgs<T> a) {
     using W = wide_t<T>;
     __shared__ W red[2 * (LONG_BLOCK / 32)];
     __shared__ unsigned group_max[LONG_BLOCK * N / 16 + 1];
-    const int64_t packets = (a.cols + N - 1) / N;
+    const int64_t packets = a.cols / N; // cols is a multiple of N
     RowSum<W, LONG_BLOCK> row_sum{red};
     for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
         const T *x = a.x + r * a.x_ld, *residual = a.residual ? a.residual + r * a.residual_ld : nullptr;
         auto stream = [&](int64_t p) {
-            const Vec<T, N> v = load_packet<T, N>(x, p, a.cols);
-            return residual ? add_residual(v, load_packet<T, N>(residual, p, a.cols)) : v;
+            const Vec<T, N> v = ld_vec<T, N>(x + p * N);
+            return residual ? add_residual(v, ld_vec<T, N>(residual + p * N)) : v;
         };
         auto again = [&](int64_t p) {
-            return a.sum ? load_packet<T, N>(a.sum + r * a.sum_ld, p, a.cols) : stream(p);
+            return a.sum ? ld_vec<T, N>(a.sum + r * a.sum_ld + p * N) : stream(p);
         };
         W ss = 0;
         for (int64_t p = threadIdx.x; p < packets; p += LONG_BLOCK) {
             const Vec<T, N> s = stream(p);
             if (a.sum)
-                store_packet<T, N>(a.sum + r * a.sum_ld, p, a.cols, s);
+                st_vec<T, N>(a.sum + r * a.sum_ld + p * N, s);
             squares(s, &ss);
         }
         const W rstd = W(1) / sqrt(row_sum(ss, LONG_BLOCK) / W(a.cols) + a.eps);
@@ -285,12 +264,12 @@ __global__ void __launch_bounds__(LONG_BLOCK) norm_long_kernel(NormArgs<T> a) {
         if constexpr (!Q8) {
             for (int64_t p = threadIdx.x; p < packets; p += LONG_BLOCK) {
                 W y[N];
-                normalised<T, N>(again(p), a.weight, p, a.cols, rstd, y);
+                normalised<T, N>(again(p), a.weight, p, rstd, y);
                 Vec<T, N> z;
 #pragma unroll
                 for (int k = 0; k < N; k++)
                     z.v[k] = narrow<T>(y[k]);
-                store_packet<T, N>(static_cast<T *>(a.res) + r * a.res_ld, p, a.cols, z);
+                st_vec<T, N>(static_cast<T *>(a.res) + r * a.res_ld + p * N, z);
             }
         } else {
             // turns of LONG_BLOCK packets, which hold whole groups (a group has at most 512 columns)
@@ -301,7 +280,7 @@ __global__ void __launch_bounds__(LONG_BLOCK) norm_long_kernel(NormArgs<T> a) {
                 __syncthreads();
                 for (int64_t p = threadIdx.x; p < packets; p += LONG_BLOCK) {
                     float y[N];
-                    normalised<T, N>(again(p), a.weight, p, a.cols, rstd, y);
+                    normalised<T, N>(again(p), a.weight, p, rstd, y);
                     row_most = max(row_most, largest<N>(y));
                 }
                 atomicMax(&group_max[0], row_most);
@@ -314,7 +293,7 @@ __global__ void __launch_bounds__(LONG_BLOCK) norm_long_kernel(NormArgs<T> a) {
                 float y[N];
                 unsigned most = row_most;
                 if (p < packets)
-                    normalised<T, N>(again(p), a.weight, p, a.cols, rstd, y);
+                    normalised<T, N>(again(p), a.weight, p, rstd, y);
                 if (a.group) {
                     const int g = (int)((int64_t)threadIdx.x * N / a.group);
                     for (int i = threadIdx.x; i < (int)(LONG_BLOCK * N / a.group) + 1; i += LONG_BLOCK)
@@ -330,7 +309,7 @@ __global__ void __launch_bounds__(LONG_BLOCK) norm_long_kernel(NormArgs<T> a) {
                     const float scale = scale_of(most);
                     if (a.group == 0 ? p == 0 : p * N % a.group == 0)
                         a.scales[r * a.scales_ld + (a.group == 0 ? 0 : p * N / a.group)] = scale;
-                    store_q8<N>(a.res, r * a.res_ld, p, a.cols, y, 1.0f / scale);
+                    store_q8<N>(a.res, r * a.res_ld + p * N, y, 1.0f / scale);
                 }
             }
         }
@@ -353,7 +332,7 @@ __global__ void __launch_bounds__(BLOCK) norm_grad_rows_kernel(NormGradArgs<T> a
     __shared__ W red[2 * (BLOCK / 32)];
     __shared__ W join[BLOCK * N];
     const int tpr = 1 << log_tpr, tx = threadIdx.x & (tpr - 1), ty = threadIdx.x >> log_tpr, at_once = BLOCK >> log_tpr;
-    const int64_t packets = (a.cols + N - 1) / N;
+    const int packets = (int)(a.cols / N); // cols is a multiple of N
     RowSum<W, BLOCK> row_sum{red};
     W dw[PPT][N];
 #pragma unroll
@@ -370,10 +349,10 @@ __global__ void __launch_bounds__(BLOCK) norm_grad_rows_kernel(NormGradArgs<T> a
 #pragma unroll
             for (int k = 0; k < PPT; k++)
                 if (tx + k * tpr < packets) {
-                    g[k] = load_packet<T, N>(a.grad + r * a.grad_ld, tx + k * tpr, a.cols);
-                    s[k] = load_packet<T, N>(a.sum + r * a.sum_ld, tx + k * tpr, a.cols);
+                    g[k] = ld_vec<T, N>(a.grad + r * a.grad_ld + (tx + k * tpr) * N);
+                    s[k] = ld_vec<T, N>(a.sum + r * a.sum_ld + (tx + k * tpr) * N);
                     if (a.dsum)
-                        d[k] = load_packet<T, N>(a.dsum + r * a.dsum_ld, tx + k * tpr, a.cols);
+                        d[k] = ld_vec<T, N>(a.dsum + r * a.dsum_ld + (tx + k * tpr) * N);
                 }
             rstd = a.rstd[r];
         }
@@ -383,7 +362,7 @@ __global__ void __launch_bounds__(BLOCK) norm_grad_rows_kernel(NormGradArgs<T> a
             if (live && tx + k * tpr < packets) {
                 Vec<T, N> w;
                 if (a.weight)
-                    w = load_packet<T, N>(a.weight, tx + k * tpr, a.cols);
+                    w = ld_vec<T, N>(a.weight + (tx + k * tpr) * N);
 #pragma unroll
                 for (int j = 0; j < N; j++) {
                     const W t = a.weight ? widen(g[k].v[j]) * widen(w.v[j]) : W(widen(g[k].v[j]));
@@ -398,7 +377,7 @@ __global__ void __launch_bounds__(BLOCK) norm_grad_rows_kernel(NormGradArgs<T> a
                 if (tx + k * tpr < packets) {
                     Vec<T, N> w, z;
                     if (a.weight)
-                        w = load_packet<T, N>(a.weight, tx + k * tpr, a.cols);
+                        w = ld_vec<T, N>(a.weight + (tx + k * tpr) * N);
 #pragma unroll
                     for (int j = 0; j < N; j++) {
                         const W t = a.weight ? widen(g[k].v[j]) * widen(w.v[j]) : W(widen(g[k].v[j]));
@@ -407,7 +386,7 @@ __global__ void __launch_bounds__(BLOCK) norm_grad_rows_kernel(NormGradArgs<T> a
                             v += widen(d[k].v[j]);
                         z.v[j] = narrow<T>(v);
                     }
-                    store_packet<T, N>(a.dx + r * a.dx_ld, tx + k * tpr, a.cols, z);
+                    st_vec<T, N>(a.dx + r * a.dx_ld + (tx + k * tpr) * N, z);
                 }
         }
     }
@@ -425,9 +404,7 @@ __global__ void __launch_bounds__(BLOCK) norm_grad_rows_kernel(NormGradArgs<T> a
                 W v = join[tx * N + j];
                 for (int i = 1; i < at_once; i++)
                     v += join[(i * tpr + tx) * N + j];
-                const int64_t c = (int64_t)(tx + k * tpr) * N + j;
-                if (c < a.cols)
-                    a.part[(int64_t)blockIdx.x * a.part_ld + c] = v;
+                a.part[(int64_t)blockIdx.x * a.part_ld + (tx + k * tpr) * N + j] = v;
             }
         }
         __syncthreads();
@@ -438,29 +415,29 @@ template <typename T, int N>
 __global__ void __launch_bounds__(LONG_BLOCK) norm_grad_long_kernel(NormGradArgs<T> a) {
     using W = wide_t<T>;
     __shared__ W red[2 * (LONG_BLOCK / 32)];
-    const int64_t packets = (a.cols + N - 1) / N;
+    const int64_t packets = a.cols / N; // cols is a multiple of N
     RowSum<W, LONG_BLOCK> row_sum{red};
     for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
         const T *g = a.grad + r * a.grad_ld, *s = a.sum + r * a.sum_ld;
         const W rstd = a.rstd[r];
         W dot = 0;
         for (int64_t p = threadIdx.x; p < packets; p += LONG_BLOCK) {
-            const Vec<T, N> gv = load_packet<T, N>(g, p, a.cols), sv = load_packet<T, N>(s, p, a.cols);
+            const Vec<T, N> gv = ld_vec<T, N>(g + p * N), sv = ld_vec<T, N>(s + p * N);
             Vec<T, N> w;
             if (a.weight)
-                w = load_packet<T, N>(a.weight, p, a.cols);
+                w = ld_vec<T, N>(a.weight + p * N);
 #pragma unroll
             for (int j = 0; j < N; j++)
                 dot += (a.weight ? widen(gv.v[j]) * widen(w.v[j]) : W(widen(gv.v[j]))) * widen(sv.v[j]);
         }
         const W factor = row_sum(dot, LONG_BLOCK) / W(a.cols) * rstd * rstd;
         for (int64_t p = threadIdx.x; p < packets; p += LONG_BLOCK) {
-            const Vec<T, N> gv = load_packet<T, N>(g, p, a.cols), sv = load_packet<T, N>(s, p, a.cols);
+            const Vec<T, N> gv = ld_vec<T, N>(g + p * N), sv = ld_vec<T, N>(s + p * N);
             Vec<T, N> w, d, z;
             if (a.weight)
-                w = load_packet<T, N>(a.weight, p, a.cols);
+                w = ld_vec<T, N>(a.weight + p * N);
             if (a.dsum)
-                d = load_packet<T, N>(a.dsum + r * a.dsum_ld, p, a.cols);
+                d = ld_vec<T, N>(a.dsum + r * a.dsum_ld + p * N);
 #pragma unroll
             for (int j = 0; j < N; j++) {
                 W v = rstd * ((a.weight ? widen(gv.v[j]) * widen(w.v[j]) : W(widen(gv.v[j]))) - widen(sv.v[j]) * factor);
@@ -468,7 +445,7 @@ __global__ void __launch_bounds__(LONG_BLOCK) norm_grad_long_kernel(NormGradArgs
                     v += widen(d.v[j]);
                 z.v[j] = narrow<T>(v);
             }
-            store_packet<T, N>(a.dx + r * a.dx_ld, p, a.cols, z);
+            st_vec<T, N>(a.dx + r * a.dx_ld + p * N, z);
         }
     }
 }
@@ -493,87 +470,101 @@ template <typename T> __global__ void __launch_bounds__(256) norm_dweight_kernel
     }
 }
 
-// dweight[c] = sum over the parts, in order within eight shares and over the shares
+// dweight[c] = sum over the parts, in order within JOIN_SHARES shares and over the shares
+constexpr int JOIN_SHARES = 32;
 template <typename W>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(32 * JOIN_SHARES)
     norm_join_kernel(const W *__restrict__ part, int parts, int64_t cols, int64_t part_ld, W *__restrict__ res) {
-    __shared__ W sums[8][33];
+    __shared__ W sums[JOIN_SHARES][33];
     const int tx = threadIdx.x % 32, ty = threadIdx.x / 32;
     const int64_t c = (int64_t)blockIdx.x * 32 + tx;
-    const int share = (parts + 7) / 8, first = ty * share, last = first + share < parts ? first + share : parts;
+    const int share = (parts + JOIN_SHARES - 1) / JOIN_SHARES, first = ty * share;
+    const int last = first + share < parts ? first + share : parts;
     W v = 0;
     if (c < cols) {
-#pragma unroll 8
+#pragma unroll 16
         for (int i = first; i < last; i++)
             v += part[(int64_t)i * part_ld + c];
     }
     sums[ty][tx] = v;
     __syncthreads();
     if (ty == 0 && c < cols) {
-        for (int k = 1; k < 8; k++)
+        for (int k = 1; k < JOIN_SHARES; k++)
             v += sums[k][tx];
         res[c] = v;
     }
 }
 
-// How many threads share a row and how many packets each holds.  Many rows: as few threads as hold the row in `most`
-// packets each, since every thread then has more loads in flight; few rows (fewer than SMs): one packet each, which
-// shortens the way of the single row.
+// How many threads share a row (a power of two) and how many packets each holds: the fewest places without a packet, and
+// among equal ones the most packets a thread, which keep more loads in flight.  Few rows (fewer than SMs): one packet a
+// thread if the block allows it, which shortens the way of the single row.
 struct RowPlan {
     int log_tpr, ppt;
     bool fits;
 };
-RowPlan row_plan(int64_t packets, int64_t rows, int most, int max_log) {
-    const int64_t want = rows < sm_count() ? packets : (packets + most - 1) / most;
-    RowPlan p{3, 1, true};
-    while (p.log_tpr < max_log && ((int64_t)1 << p.log_tpr) < want)
-        p.log_tpr++;
-    while (p.ppt < most && ((int64_t)p.ppt << p.log_tpr) < packets)
-        p.ppt *= 2;
-    p.fits = ((int64_t)p.ppt << p.log_tpr) >= packets;
+RowPlan row_plan(int64_t packets, int64_t rows, int most) {
+    RowPlan p{0, 0, false};
+    for (int log = 3; log <= 9; log++) {
+        const int64_t tpr = (int64_t)1 << log, ppt = (packets + tpr - 1) / tpr;
+        if (ppt > most)
+            continue;
+        const bool fewer = !p.fits || (ppt << log) < ((int64_t)p.ppt << p.log_tpr);
+        if (fewer || rows < sm_count()) {
+            p.log_tpr = log;
+            p.ppt = (int)ppt;
+            p.fits = true;
+        }
+        if (rows < sm_count() && ppt == 1)
+            break;
+    }
     return p;
 }
 
+// PPT of the kernel that is launched for a plan: single elements in eights
+template <int N> constexpr int most_packets(bool back) { return N == 1 ? 8 : (back ? 3 : 5); }
+#define DB2_BY_PACKETS(N, back, ppt, LAUNCH)                                                                           \
+    if constexpr (N == 1) {                                                                                            \
+        LAUNCH(8)                                                                                                      \
+    } else                                                                                                             \
+        switch (ppt) {                                                                                                 \
+        case 1: LAUNCH(1) break;                                                                                       \
+        case 2: LAUNCH(2) break;                                                                                       \
+        case 3: LAUNCH(3) break;                                                                                       \
+        case 4: LAUNCH((back) ? 3 : 4) break;                                                                          \
+        default: LAUNCH((back) ? 3 : 5) break;                                                                         \
+        }
+
 template <typename T, int N, bool Q8> int norm_launch(const NormArgs<T> &a, cudaStream_t st) {
-    constexpr int MOST = N == 1 ? 8 : 4;
-    const RowPlan p = row_plan((a.cols + N - 1) / N, a.rows, MOST, 10);
+    const RowPlan p = row_plan(a.cols / N, a.rows, most_packets<N>(false));
     const int64_t max_grid = (int64_t)1 << 30;
     if (!p.fits) {
         norm_long_kernel<T, N, Q8><<<(unsigned)(a.rows < max_grid ? a.rows : max_grid), LONG_BLOCK, 0, st>>>(a);
         return after_launch("norm_long_kernel");
     }
-    const int block = p.log_tpr > 8 ? 1 << p.log_tpr : 256, at_once = block >> p.log_tpr;
+    const int block = p.log_tpr > 8 ? 512 : 256, at_once = block >> p.log_tpr;
     const int64_t blocks = (a.rows + at_once - 1) / at_once;
     const unsigned grid = (unsigned)(blocks < max_grid ? blocks : max_grid);
     const size_t smem = Q8 ? (size_t)at_once * a.groups * sizeof(unsigned) : 0;
-#define DB2_NORM(PPT, BLOCK) norm_rows_kernel<T, N, PPT, Q8, BLOCK><<<grid, BLOCK, smem, st>>>(a, p.log_tpr)
-#define DB2_NORM_PPT(BLOCK)                                                                                            \
-    switch (p.ppt) {                                                                                                   \
-    case 1: DB2_NORM(1, BLOCK); break;                                                                                 \
-    case 2: DB2_NORM(2, BLOCK); break;                                                                                 \
-    case 4: DB2_NORM(4, BLOCK); break;                                                                                 \
-    default: DB2_NORM(MOST, BLOCK); break;                                                                             \
+#define DB2_NORM(PPT)                                                                                                  \
+    {                                                                                                                  \
+        if (block == 256)                                                                                              \
+            norm_rows_kernel<T, N, PPT, Q8, 256><<<grid, 256, smem, st>>>(a, p.log_tpr);                               \
+        else                                                                                                           \
+            norm_rows_kernel<T, N, PPT, Q8, 512><<<grid, 512, smem, st>>>(a, p.log_tpr);                               \
     }
-    if (block == 256)
-        DB2_NORM_PPT(256)
-    else if (block == 512)
-        DB2_NORM_PPT(512)
-    else
-        DB2_NORM_PPT(1024)
-#undef DB2_NORM_PPT
+    DB2_BY_PACKETS(N, false, p.ppt, DB2_NORM)
 #undef DB2_NORM
     return after_launch("norm_rows_kernel");
 }
 
-// CTAs of the gradient kernel: each keeps its own column sums
+// CTAs of the gradient kernel, which stay for many rows: each keeps its own column sums
 int64_t grad_ctas(int64_t rows) {
-    const int64_t cap = (int64_t)sm_count() * 4;
+    const int64_t cap = (int64_t)sm_count() * 3;
     return rows < 1 ? 1 : (rows < cap ? rows : cap);
 }
 
 template <typename T, int N> int norm_grad_launch(NormGradArgs<T> a, wide_t<T> *dweight, cudaStream_t st) {
-    constexpr int MOST = N == 1 ? 8 : 4;
-    const RowPlan p = row_plan((a.cols + N - 1) / N, a.rows, MOST, 9); // 512 threads: 128 registers each
+    const RowPlan p = row_plan(a.cols / N, a.rows, most_packets<N>(true));
     const int64_t ctas = grad_ctas(a.rows);
     int parts;
     if (!p.fits) {
@@ -588,29 +579,25 @@ template <typename T, int N> int norm_grad_launch(NormGradArgs<T> a, wide_t<T> *
         const int block = p.log_tpr > 8 ? 512 : 256, at_once = block >> p.log_tpr;
         const int64_t blocks = (a.rows + at_once - 1) / at_once;
         parts = (int)(blocks < ctas ? blocks : ctas);
-#define DB2_NORM_GRAD(PPT, BLOCK) norm_grad_rows_kernel<T, N, PPT, BLOCK><<<parts, BLOCK, 0, st>>>(a, p.log_tpr)
-#define DB2_NORM_GRAD_PPT(BLOCK)                                                                                       \
-    switch (p.ppt) {                                                                                                   \
-    case 1: DB2_NORM_GRAD(1, BLOCK); break;                                                                            \
-    case 2: DB2_NORM_GRAD(2, BLOCK); break;                                                                            \
-    case 4: DB2_NORM_GRAD(4, BLOCK); break;                                                                            \
-    default: DB2_NORM_GRAD(MOST, BLOCK); break;                                                                        \
+#define DB2_NORM_GRAD(PPT)                                                                                             \
+    {                                                                                                                  \
+        if (block == 256)                                                                                              \
+            norm_grad_rows_kernel<T, N, PPT, 256><<<parts, 256, 0, st>>>(a, p.log_tpr);                                \
+        else                                                                                                           \
+            norm_grad_rows_kernel<T, N, PPT, 512><<<parts, 512, 0, st>>>(a, p.log_tpr);                                \
     }
-        if (block == 256)
-            DB2_NORM_GRAD_PPT(256)
-        else
-            DB2_NORM_GRAD_PPT(512)
-#undef DB2_NORM_GRAD_PPT
+        DB2_BY_PACKETS(N, true, p.ppt, DB2_NORM_GRAD)
 #undef DB2_NORM_GRAD
         DB2_TRY(after_launch("norm_grad_rows_kernel"));
     }
     if (a.part) {
-        norm_join_kernel<wide_t<T>><<<(unsigned)((a.cols + 31) / 32), 256, 0, st>>>(a.part, parts, a.cols, a.part_ld,
-                                                                                   dweight);
+        norm_join_kernel<wide_t<T>><<<(unsigned)((a.cols + 31) / 32), 32 * JOIN_SHARES, 0, st>>>(a.part, parts, a.cols,
+                                                                                                 a.part_ld, dweight);
         DB2_TRY(after_launch("norm_join_kernel"));
     }
     return DB2_OK;
 }
+#undef DB2_BY_PACKETS
 
 int64_t part_ld_of(int64_t cols) { return (cols + 7) / 8 * 8; }
 
@@ -712,7 +699,7 @@ int db2k_rms_norm(int dtype, const void *x, int64_t rows, int64_t cols, int64_t 
         NormArgs<T> a{static_cast<const T *>(x), static_cast<const T *>(residual), static_cast<const T *>(weight),
                       static_cast<T *>(sum), res, nullptr, static_cast<wide_t<T> *>(rstd), rows, cols, x_ld,
                       residual_ld, sum_ld, res_ld, 0, 0, 0, (wide_t<T>)eps};
-        const bool packed = rows_aligned(x, x_ld, sizeof(T), 16) && rows_aligned(residual, residual_ld, sizeof(T), 16) &&
+        const bool packed = cols % N == 0 && rows_aligned(x, x_ld, sizeof(T), 16) && rows_aligned(residual, residual_ld, sizeof(T), 16) &&
                             rows_aligned(weight, 0, sizeof(T), 16) && rows_aligned(sum, sum_ld, sizeof(T), 16) &&
                             rows_aligned(res, res_ld, sizeof(T), 16);
         return packed ? norm_launch<T, N, false>(a, as_stream(stream)) : norm_launch<T, 1, false>(a, as_stream(stream));
@@ -740,7 +727,7 @@ int db2k_rms_norm_q8(int dtype, const void *x, int64_t rows, int64_t cols, int64
         NormArgs<T> a{static_cast<const T *>(x), static_cast<const T *>(residual), static_cast<const T *>(weight),
                       static_cast<T *>(sum), res, static_cast<float *>(scales), static_cast<float *>(rstd), rows, cols,
                       x_ld, residual_ld, sum_ld, res_ld, scales_ld, group, groups, (float)eps};
-        const bool packed = rows_aligned(x, x_ld, sizeof(T), 16) && rows_aligned(residual, residual_ld, sizeof(T), 16) &&
+        const bool packed = cols % N == 0 && rows_aligned(x, x_ld, sizeof(T), 16) && rows_aligned(residual, residual_ld, sizeof(T), 16) &&
                             rows_aligned(weight, 0, sizeof(T), 16) && rows_aligned(sum, sum_ld, sizeof(T), 16) &&
                             rows_aligned(res, res_ld, 1, N);
         return packed ? norm_launch<T, N, true>(a, as_stream(stream)) : norm_launch<T, 1, true>(a, as_stream(stream));
@@ -779,7 +766,7 @@ int db2k_rms_norm_grad(int dtype, const void *grad, int64_t grad_ld, int64_t row
                           static_cast<const T *>(dsum), static_cast<const wide_t<T> *>(rstd), static_cast<T *>(dx),
                           dweight ? static_cast<wide_t<T> *>(scratch) : nullptr, rows, cols, grad_ld, sum_ld, dsum_ld,
                           dx_ld, part_ld_of(cols)};
-        const bool packed = rows_aligned(grad, grad_ld, sizeof(T), 16) && rows_aligned(sum, sum_ld, sizeof(T), 16) &&
+        const bool packed = cols % N == 0 && rows_aligned(grad, grad_ld, sizeof(T), 16) && rows_aligned(sum, sum_ld, sizeof(T), 16) &&
                             rows_aligned(weight, 0, sizeof(T), 16) && rows_aligned(dsum, dsum_ld, sizeof(T), 16) &&
                             rows_aligned(dx, dx_ld, sizeof(T), 16);
         wide_t<T> *dw = static_cast<wide_t<T> *>(dweight);
