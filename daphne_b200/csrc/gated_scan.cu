@@ -77,16 +77,6 @@ __device__ __forceinline__ void gate_pair(double g, double *f, double *o) {
 __device__ __forceinline__ float finite(float a) { return fminf(fmaxf(a, -3.40282347e38f), 3.40282347e38f); }
 __device__ __forceinline__ double finite(double a) { return fmin(fmax(a, -1.7976931348623157e308), 1.7976931348623157e308); }
 
-// VEC elements from global to shared memory: asynchronously, or at once where they are fewer than four bytes.
-template <typename T, int VEC> __device__ __forceinline__ void fetch(T *to, const T *from) {
-    if constexpr (sizeof(T) * VEC >= 4)
-        asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"((unsigned)__cvta_generic_to_shared(to)), "l"(from),
-                     "n"(sizeof(T) * VEC)
-                     : "memory");
-    else
-        st_vec<T, VEC>(to, ld_vec<T, VEC>(from));
-}
-
 // A composed step per channel of a strip, as it lies in shared memory.
 template <typename W, int VEC> struct Steps {
     W a[32 * VEC], b[32 * VEC];
@@ -195,7 +185,7 @@ __global__ void __launch_bounds__(WARPS * 32, WARPS == 4 ? 3 : 1) gated_scan_ker
                 if (i < m)
                     load_row(stage, i, first - q - i > begin);
         }
-        asm volatile("cp.async.commit_group;" ::: "memory");
+        fetch_commit();
         pg += TILE * dir * a.g_ld;
         if constexpr (X)
             px += TILE * dir * a.x_ld;
@@ -214,7 +204,7 @@ __global__ void __launch_bounds__(WARPS * 32, WARPS == 4 ? 3 : 1) gated_scan_ker
         const bool all = all_there(q, m);
         W f[R][VEC], o[R][VEC], b[R][VEC]; // gate, 1 - gate, u or dh
         V kx[R], ka[R];
-        asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
+        fetch_wait<STAGES - 2>();
         auto open = [&](int i) {
             const V rg = ld_vec<T, VEC>(at(stage, 0, i));
             V rx, rd;

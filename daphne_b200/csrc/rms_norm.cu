@@ -17,10 +17,12 @@ namespace {
 
 constexpr float E4M3_MAX = 448.0f;
 
-// sum over the `tpr` threads of a row (a power of two; rows lie side by side in the CTA), in one fixed order.  Every
-// thread of the CTA calls it the same number of times; `red` alternates between two halves, so one barrier is enough.
-template <typename W, int BLOCK> struct RowSum {
-    W *red; // 2 * BLOCK / 32
+// Sum over the `tpr` threads of a row, in one fixed order; tpr is a power of two below 32 or a multiple of 32, and the rows
+// of a CTA lie side by side.  Every thread of the CTA calls it the same number of times; `red` alternates between two
+// halves, so one barrier is enough.
+constexpr int NORM_MAX_WARPS = 16;
+template <typename W> struct RowSum {
+    W *red; // 2 * NORM_MAX_WARPS
     int turn = 0;
     __device__ W operator()(W v, int tpr) {
         const int in_warp = tpr < 32 ? tpr : 32;
@@ -28,19 +30,35 @@ template <typename W, int BLOCK> struct RowSum {
             v += shfl_xor(v, o);
         if (tpr <= 32)
             return v;
-        W *half = red + turn * (BLOCK / 32);
+        W *half = red + turn * NORM_MAX_WARPS;
         turn ^= 1;
-        const int warp = threadIdx.x / 32;
         if (threadIdx.x % 32 == 0)
-            half[warp] = v;
+            half[threadIdx.x / 32] = v;
         __syncthreads();
-        const int warps = tpr / 32, first = warp / warps * warps;
+        const int warps = tpr / 32, first = threadIdx.x / tpr * warps;
         W s = half[first];
         for (int k = 1; k < warps; k++)
             s += half[first + k];
         return s;
     }
 };
+
+// Rows on their way: a thread's packets of its next NORM_STAGES - 1 rows, in shared memory.  It reads nothing else
+// there, so no barrier is needed.
+constexpr int NORM_STAGES = 3;
+extern __shared__ __align__(16) unsigned char norm_smem[];
+template <typename T, int N, int PPT> struct RowRing {
+    int operands, stage = 0;
+    __device__ T *at(int stage, int operand, int k) const {
+        return reinterpret_cast<T *>(norm_smem) + (((stage * operands + operand) * PPT + k) * (int)blockDim.x + (int)threadIdx.x) * N;
+    }
+    __device__ Vec<T, N> get(int operand, int k) const { return ld_vec<T, N>(at(stage, operand, k)); }
+    __device__ int last() const { return stage == 0 ? NORM_STAGES - 1 : stage - 1; } // the one emptied last
+    __device__ void next() { stage = stage == NORM_STAGES - 1 ? 0 : stage + 1; }
+};
+size_t ring_bytes(size_t packet, int ppt, int operands, int block) {
+    return (size_t)NORM_STAGES * operands * ppt * block * packet;
+}
 
 template <typename T> struct NormArgs { // x, residual and sum may be the same matrix, and res one of x and residual
     const T *x, *residual, *weight;
@@ -113,36 +131,44 @@ template <int N> __device__ __forceinline__ void store_q8(void *res, int64_t at,
     st_vec<__nv_fp8_storage_t, N>(static_cast<__nv_fp8_storage_t *>(res) + at, q);
 }
 
-// Rows of up to tpr * PPT packets: a thread holds packets tx, tx + tpr, ... of its row.
-template <typename T, int N, int PPT, bool Q8, int BLOCK>
-__global__ void __launch_bounds__(BLOCK) norm_rows_kernel(NormArgs<T> a, int log_tpr) {
+// Rows of up to tpr * PPT packets: a thread holds packets tx, tx + tpr, ... of its row.  The CTA stays for many rows.
+template <typename T, int N, int PPT, bool Q8>
+__global__ void __launch_bounds__(NORM_MAX_WARPS * 32) norm_rows_kernel(NormArgs<T> a, int tpr) {
     using W = wide_t<T>;
-    __shared__ W red[2 * (BLOCK / 32)];
-    extern __shared__ unsigned group_max[]; // rows of the CTA x groups (8-bit results whose groups span warps)
-    const int tpr = 1 << log_tpr, tx = threadIdx.x & (tpr - 1), ty = threadIdx.x >> log_tpr, at_once = BLOCK >> log_tpr;
+    __shared__ W red[2 * NORM_MAX_WARPS];
+    const int at_once = blockDim.x / tpr, tx = threadIdx.x % tpr, ty = threadIdx.x / tpr;
     const int packets = (int)(a.cols / N); // cols is a multiple of N
-    RowSum<W, BLOCK> row_sum{red};
-    for (int64_t r0 = (int64_t)blockIdx.x * at_once; r0 < a.rows; r0 += (int64_t)gridDim.x * at_once) {
+    RowSum<W> row_sum{red};
+    RowRing<T, N, PPT> ring{a.residual ? 2 : 1};
+    // rows of the CTA x groups (8-bit results whose groups span warps), behind the ring
+    unsigned *group_max = reinterpret_cast<unsigned *>(ring.at(NORM_STAGES, 0, 0) - (int)threadIdx.x * N);
+    const int64_t step = (int64_t)gridDim.x * at_once;
+    auto load = [&](int stage, int64_t r) {
+        if (r < a.rows)
+#pragma unroll
+            for (int k = 0; k < PPT; k++)
+                if (tx + k * tpr < packets) {
+                    fetch<T, N>(ring.at(stage, 0, k), a.x + r * a.x_ld + (tx + k * tpr) * N);
+                    if (a.residual)
+                        fetch<T, N>(ring.at(stage, 1, k), a.residual + r * a.residual_ld + (tx + k * tpr) * N);
+                }
+        fetch_commit();
+    };
+    for (int i = 0; i < NORM_STAGES - 1; i++)
+        load(i, (int64_t)blockIdx.x * at_once + ty + i * step);
+    for (int64_t r0 = (int64_t)blockIdx.x * at_once; r0 < a.rows; r0 += step) {
         const int64_t r = r0 + ty;
         const bool live = r < a.rows;
         Vec<T, N> s[PPT];
+        fetch_wait<NORM_STAGES - 2>();
         if (live) {
-            const T *x = a.x + r * a.x_ld;
 #pragma unroll
             for (int k = 0; k < PPT; k++)
-                if (tx + k * tpr < packets)
-                    s[k] = ld_vec<T, N>(x + (tx + k * tpr) * N);
-            if (a.residual) {
-                const T *res = a.residual + r * a.residual_ld;
-                Vec<T, N> y[PPT];
-#pragma unroll
-                for (int k = 0; k < PPT; k++)
-                    if (tx + k * tpr < packets)
-                        y[k] = ld_vec<T, N>(res + (tx + k * tpr) * N);
-#pragma unroll
-                for (int k = 0; k < PPT; k++)
-                    s[k] = add_residual(s[k], y[k]);
-            }
+                if (tx + k * tpr < packets) {
+                    s[k] = ring.get(0, k);
+                    if (a.residual)
+                        s[k] = add_residual(s[k], ring.get(1, k));
+                }
             if (a.sum) {
                 T *sum = a.sum + r * a.sum_ld;
 #pragma unroll
@@ -151,6 +177,8 @@ __global__ void __launch_bounds__(BLOCK) norm_rows_kernel(NormArgs<T> a, int log
                         st_vec<T, N>(sum + (tx + k * tpr) * N, s[k]);
             }
         }
+        load(ring.last(), r + (NORM_STAGES - 1) * step);
+        ring.next();
         W ss = 0;
 #pragma unroll
         for (int k = 0; k < PPT; k++)
@@ -238,10 +266,10 @@ constexpr int LONG_BLOCK = 512;
 template <typename T, int N, bool Q8>
 __global__ void __launch_bounds__(LONG_BLOCK) norm_long_kernel(NormArgs<T> a) {
     using W = wide_t<T>;
-    __shared__ W red[2 * (LONG_BLOCK / 32)];
+    __shared__ W red[2 * NORM_MAX_WARPS];
     __shared__ unsigned group_max[LONG_BLOCK * N / 16 + 1];
     const int64_t packets = a.cols / N; // cols is a multiple of N
-    RowSum<W, LONG_BLOCK> row_sum{red};
+    RowSum<W> row_sum{red};
     for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
         const T *x = a.x + r * a.x_ld, *residual = a.residual ? a.residual + r * a.residual_ld : nullptr;
         auto stream = [&](int64_t p) {
@@ -326,36 +354,55 @@ template <typename T> struct NormGradArgs { // dx may be the same matrix as grad
 
 // dx of the rows, and the CTA's column sums of dy * s * rstd: a thread keeps the sums of its columns in registers over
 // all rows that the CTA visits; the rows that a CTA holds at once are joined through shared memory in order.
-template <typename T, int N, int PPT, int BLOCK>
-__global__ void __launch_bounds__(BLOCK) norm_grad_rows_kernel(NormGradArgs<T> a, int log_tpr) {
+template <typename T, int N, int PPT>
+__global__ void __launch_bounds__(NORM_MAX_WARPS * 32) norm_grad_rows_kernel(NormGradArgs<T> a, int tpr) {
     using W = wide_t<T>;
-    __shared__ W red[2 * (BLOCK / 32)];
-    __shared__ W join[BLOCK * N];
-    const int tpr = 1 << log_tpr, tx = threadIdx.x & (tpr - 1), ty = threadIdx.x >> log_tpr, at_once = BLOCK >> log_tpr;
+    __shared__ W red[2 * NORM_MAX_WARPS];
+    const int at_once = blockDim.x / tpr, tx = threadIdx.x % tpr, ty = threadIdx.x / tpr;
     const int packets = (int)(a.cols / N); // cols is a multiple of N
-    RowSum<W, BLOCK> row_sum{red};
+    RowSum<W> row_sum{red};
+    RowRing<T, N, PPT> ring{a.dsum ? 3 : 2};
     W dw[PPT][N];
 #pragma unroll
     for (int k = 0; k < PPT; k++)
 #pragma unroll
         for (int j = 0; j < N; j++)
             dw[k][j] = 0;
-    for (int64_t r0 = (int64_t)blockIdx.x * at_once; r0 < a.rows; r0 += (int64_t)gridDim.x * at_once) {
+    const int64_t step = (int64_t)gridDim.x * at_once;
+    auto load = [&](int stage, int64_t r) {
+        if (r < a.rows)
+#pragma unroll
+            for (int k = 0; k < PPT; k++)
+                if (tx + k * tpr < packets) {
+                    fetch<T, N>(ring.at(stage, 0, k), a.grad + r * a.grad_ld + (tx + k * tpr) * N);
+                    fetch<T, N>(ring.at(stage, 1, k), a.sum + r * a.sum_ld + (tx + k * tpr) * N);
+                    if (a.dsum)
+                        fetch<T, N>(ring.at(stage, 2, k), a.dsum + r * a.dsum_ld + (tx + k * tpr) * N);
+                }
+        fetch_commit();
+    };
+    for (int i = 0; i < NORM_STAGES - 1; i++)
+        load(i, (int64_t)blockIdx.x * at_once + ty + i * step);
+    W next_rstd = (int64_t)blockIdx.x * at_once + ty < a.rows ? a.rstd[(int64_t)blockIdx.x * at_once + ty] : W(0);
+    for (int64_t r0 = (int64_t)blockIdx.x * at_once; r0 < a.rows; r0 += step) {
         const int64_t r = r0 + ty;
         const bool live = r < a.rows;
+        const W rstd = next_rstd;
+        next_rstd = r + step < a.rows ? a.rstd[r + step] : W(0);
         Vec<T, N> g[PPT], s[PPT], d[PPT];
-        W rstd = 0;
+        fetch_wait<NORM_STAGES - 2>();
         if (live) {
 #pragma unroll
             for (int k = 0; k < PPT; k++)
                 if (tx + k * tpr < packets) {
-                    g[k] = ld_vec<T, N>(a.grad + r * a.grad_ld + (tx + k * tpr) * N);
-                    s[k] = ld_vec<T, N>(a.sum + r * a.sum_ld + (tx + k * tpr) * N);
+                    g[k] = ring.get(0, k);
+                    s[k] = ring.get(1, k);
                     if (a.dsum)
-                        d[k] = ld_vec<T, N>(a.dsum + r * a.dsum_ld + (tx + k * tpr) * N);
+                        d[k] = ring.get(2, k);
                 }
-            rstd = a.rstd[r];
         }
+        load(ring.last(), r + (NORM_STAGES - 1) * step);
+        ring.next();
         W dot = 0;
 #pragma unroll
         for (int k = 0; k < PPT; k++)
@@ -392,31 +439,42 @@ __global__ void __launch_bounds__(BLOCK) norm_grad_rows_kernel(NormGradArgs<T> a
     }
     if (!a.part)
         return;
+    W *part = a.part + (int64_t)blockIdx.x * a.part_ld;
+    if (at_once == 1) {
+#pragma unroll
+        for (int k = 0; k < PPT; k++)
+            if (tx + k * tpr < packets)
+#pragma unroll
+                for (int j = 0; j < N; j++)
+                    part[(tx + k * tpr) * N + j] = dw[k][j];
+        return;
+    }
+    fetch_wait<0>();
+    W *join = reinterpret_cast<W *>(norm_smem); // over the ring
 #pragma unroll
     for (int k = 0; k < PPT; k++) {
+        __syncthreads();
 #pragma unroll
         for (int j = 0; j < N; j++)
             join[threadIdx.x * N + j] = dw[k][j];
         __syncthreads();
-        if (ty == 0 && tx + k * tpr < packets) {
+        if (ty == 0 && tx + k * tpr < packets)
 #pragma unroll
             for (int j = 0; j < N; j++) {
                 W v = join[tx * N + j];
                 for (int i = 1; i < at_once; i++)
                     v += join[(i * tpr + tx) * N + j];
-                a.part[(int64_t)blockIdx.x * a.part_ld + (tx + k * tpr) * N + j] = v;
+                part[(tx + k * tpr) * N + j] = v;
             }
-        }
-        __syncthreads();
     }
 }
 
 template <typename T, int N>
 __global__ void __launch_bounds__(LONG_BLOCK) norm_grad_long_kernel(NormGradArgs<T> a) {
     using W = wide_t<T>;
-    __shared__ W red[2 * (LONG_BLOCK / 32)];
+    __shared__ W red[2 * NORM_MAX_WARPS];
     const int64_t packets = a.cols / N; // cols is a multiple of N
-    RowSum<W, LONG_BLOCK> row_sum{red};
+    RowSum<W> row_sum{red};
     for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
         const T *g = a.grad + r * a.grad_ld, *s = a.sum + r * a.sum_ld;
         const W rstd = a.rstd[r];
@@ -495,76 +553,94 @@ __global__ void __launch_bounds__(32 * JOIN_SHARES)
     }
 }
 
-// How many threads share a row (a power of two) and how many packets each holds: the fewest places without a packet, and
-// among equal ones the most packets a thread, which keep more loads in flight.  Few rows (fewer than SMs): one packet a
-// thread if the block allows it, which shortens the way of the single row.
+// How many threads share a row and how many packets each holds: the fewest places without a packet, and among equal ones
+// the most packets a thread.  Few rows (fewer than SMs): as few packets a thread as fit, which shortens the way of the
+// single row.
 struct RowPlan {
-    int log_tpr, ppt;
+    int tpr, ppt, block;
     bool fits;
 };
-RowPlan row_plan(int64_t packets, int64_t rows, int most) {
-    RowPlan p{0, 0, false};
-    for (int log = 3; log <= 9; log++) {
-        const int64_t tpr = (int64_t)1 << log, ppt = (packets + tpr - 1) / tpr;
-        if (ppt > most)
+RowPlan row_plan(int64_t packets, int64_t rows, int first, int most, int step) {
+    RowPlan p{0, 0, 0, false};
+    for (int ppt = first; ppt <= most; ppt += step) {
+        int64_t tpr = (packets + ppt - 1) / ppt;
+        tpr = tpr < 32 ? next_pow2(tpr < 8 ? 8 : tpr) : (tpr + 31) / 32 * 32;
+        if (tpr > NORM_MAX_WARPS * 32)
             continue;
-        const bool fewer = !p.fits || (ppt << log) < ((int64_t)p.ppt << p.log_tpr);
-        if (fewer || rows < sm_count()) {
-            p.log_tpr = log;
-            p.ppt = (int)ppt;
+        if (!p.fits || (rows >= sm_count() && tpr * ppt <= (int64_t)p.tpr * p.ppt)) {
+            p.tpr = (int)tpr;
+            p.ppt = ppt;
             p.fits = true;
         }
-        if (rows < sm_count() && ppt == 1)
-            break;
     }
+    p.block = p.fits ? p.tpr * (p.tpr < 256 ? 256 / p.tpr : 1) : 0;
     return p;
 }
-
-// PPT of the kernel that is launched for a plan: single elements in eights
-template <int N> constexpr int most_packets(bool back) { return N == 1 ? 8 : (back ? 3 : 5); }
-#define DB2_BY_PACKETS(N, back, ppt, LAUNCH)                                                                           \
+// packets a thread that there are kernels for: 1, 2, 3 (forward), or 4 and 8 single elements
+template <int N> RowPlan row_plan(int64_t cols, int64_t rows, bool back) {
+    return N == 1 ? row_plan(cols, rows, 4, 8, 4) : row_plan(cols / N, rows, 1, back ? 2 : 3, 1);
+}
+#define DB2_BY_PACKETS(N, ppt, LAUNCH)                                                                                 \
     if constexpr (N == 1) {                                                                                            \
-        LAUNCH(8)                                                                                                      \
-    } else                                                                                                             \
-        switch (ppt) {                                                                                                 \
-        case 1: LAUNCH(1) break;                                                                                       \
-        case 2: LAUNCH(2) break;                                                                                       \
-        case 3: LAUNCH(3) break;                                                                                       \
-        case 4: LAUNCH((back) ? 3 : 4) break;                                                                          \
-        default: LAUNCH((back) ? 3 : 5) break;                                                                         \
-        }
+        if (ppt == 4) {                                                                                                \
+            LAUNCH(4)                                                                                                  \
+        } else {                                                                                                       \
+            LAUNCH(8)                                                                                                  \
+        }                                                                                                              \
+    } else if (ppt == 1) {                                                                                             \
+        LAUNCH(1)                                                                                                      \
+    } else if (ppt == 2) {                                                                                             \
+        LAUNCH(2)                                                                                                      \
+    } else {                                                                                                           \
+        LAUNCH(3)                                                                                                      \
+    }
+
+// CTAs that stay on the device for all rows: as many as fit at once
+constexpr int NORM_SMEM = 200 << 10; // every launch asks for less
+template <typename K> int resident_ctas(K kernel, PerDeviceOnce &once, int block, size_t smem, int64_t most, unsigned *ctas) {
+    DB2_CHECK(smem <= (size_t)NORM_SMEM, DB2_ECUDA, "rmsNorm: %zu bytes of shared memory", smem);
+    if (once.need()) {
+        DB2_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, NORM_SMEM));
+        once.mark();
+    }
+    *ctas = (unsigned)most;
+    if (most <= sm_count())
+        return DB2_OK;
+    int per_sm = 1;
+    DB2_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, block, smem));
+    DB2_CHECK(per_sm > 0, DB2_ECUDA, "rmsNorm: the kernel does not fit on an SM");
+    const int64_t n = (int64_t)sm_count() * per_sm;
+    *ctas = (unsigned)(most < n ? most : n);
+    return DB2_OK;
+}
 
 template <typename T, int N, bool Q8> int norm_launch(const NormArgs<T> &a, cudaStream_t st) {
-    const RowPlan p = row_plan(a.cols / N, a.rows, most_packets<N>(false));
-    const int64_t max_grid = (int64_t)1 << 30;
+    const RowPlan p = row_plan<N>(a.cols, a.rows, false);
     if (!p.fits) {
+        const int64_t max_grid = (int64_t)1 << 30;
         norm_long_kernel<T, N, Q8><<<(unsigned)(a.rows < max_grid ? a.rows : max_grid), LONG_BLOCK, 0, st>>>(a);
         return after_launch("norm_long_kernel");
     }
-    const int block = p.log_tpr > 8 ? 512 : 256, at_once = block >> p.log_tpr;
-    const int64_t blocks = (a.rows + at_once - 1) / at_once;
-    const unsigned grid = (unsigned)(blocks < max_grid ? blocks : max_grid);
-    const size_t smem = Q8 ? (size_t)at_once * a.groups * sizeof(unsigned) : 0;
+    const int at_once = p.block / p.tpr;
+    unsigned grid = 0;
 #define DB2_NORM(PPT)                                                                                                  \
-    {                                                                                                                  \
-        if (block == 256)                                                                                              \
-            norm_rows_kernel<T, N, PPT, Q8, 256><<<grid, 256, smem, st>>>(a, p.log_tpr);                               \
-        else                                                                                                           \
-            norm_rows_kernel<T, N, PPT, Q8, 512><<<grid, 512, smem, st>>>(a, p.log_tpr);                               \
-    }
-    DB2_BY_PACKETS(N, false, p.ppt, DB2_NORM)
+    const size_t smem = ring_bytes(sizeof(T) * N, PPT, a.residual ? 2 : 1, p.block) + (Q8 ? at_once * a.groups * 4 : 0); \
+    static PerDeviceOnce once;                                                                                         \
+    DB2_TRY(resident_ctas(norm_rows_kernel<T, N, PPT, Q8>, once, p.block, smem, (a.rows + at_once - 1) / at_once, &grid));   \
+    norm_rows_kernel<T, N, PPT, Q8><<<grid, p.block, smem, st>>>(a, p.tpr);
+    DB2_BY_PACKETS(N, p.ppt, DB2_NORM)
 #undef DB2_NORM
     return after_launch("norm_rows_kernel");
 }
 
-// CTAs of the gradient kernel, which stay for many rows: each keeps its own column sums
+// most CTAs of the gradient kernel: each keeps its own column sums
 int64_t grad_ctas(int64_t rows) {
-    const int64_t cap = (int64_t)sm_count() * 3;
+    const int64_t cap = (int64_t)sm_count() * 4;
     return rows < 1 ? 1 : (rows < cap ? rows : cap);
 }
 
 template <typename T, int N> int norm_grad_launch(NormGradArgs<T> a, wide_t<T> *dweight, cudaStream_t st) {
-    const RowPlan p = row_plan(a.cols / N, a.rows, most_packets<N>(true));
+    const RowPlan p = row_plan<N>(a.cols, a.rows, true);
     const int64_t ctas = grad_ctas(a.rows);
     int parts;
     if (!p.fits) {
@@ -576,19 +652,20 @@ template <typename T, int N> int norm_grad_launch(NormGradArgs<T> a, wide_t<T> *
         norm_grad_long_kernel<T, N><<<(unsigned)ctas, LONG_BLOCK, 0, st>>>(a);
         DB2_TRY(after_launch("norm_grad_long_kernel"));
     } else {
-        const int block = p.log_tpr > 8 ? 512 : 256, at_once = block >> p.log_tpr;
+        const int at_once = p.block / p.tpr;
         const int64_t blocks = (a.rows + at_once - 1) / at_once;
-        parts = (int)(blocks < ctas ? blocks : ctas);
+        unsigned grid = 0;
 #define DB2_NORM_GRAD(PPT)                                                                                             \
-    {                                                                                                                  \
-        if (block == 256)                                                                                              \
-            norm_grad_rows_kernel<T, N, PPT, 256><<<parts, 256, 0, st>>>(a, p.log_tpr);                                \
-        else                                                                                                           \
-            norm_grad_rows_kernel<T, N, PPT, 512><<<parts, 512, 0, st>>>(a, p.log_tpr);                                \
-    }
-        DB2_BY_PACKETS(N, true, p.ppt, DB2_NORM_GRAD)
+    size_t smem = ring_bytes(sizeof(T) * N, PPT, a.dsum ? 3 : 2, p.block);                                             \
+    if (smem < p.block * N * sizeof(wide_t<T>)) /* where the rows of a CTA are joined */                               \
+        smem = p.block * N * sizeof(wide_t<T>);                                                                        \
+    static PerDeviceOnce once;                                                                                         \
+    DB2_TRY(resident_ctas(norm_grad_rows_kernel<T, N, PPT>, once, p.block, smem, blocks < ctas ? blocks : ctas, &grid));     \
+    norm_grad_rows_kernel<T, N, PPT><<<grid, p.block, smem, st>>>(a, p.tpr);
+        DB2_BY_PACKETS(N, p.ppt, DB2_NORM_GRAD)
 #undef DB2_NORM_GRAD
         DB2_TRY(after_launch("norm_grad_rows_kernel"));
+        parts = (int)grid;
     }
     if (a.part) {
         norm_join_kernel<wide_t<T>><<<(unsigned)((a.cols + 31) / 32), 32 * JOIN_SHARES, 0, st>>>(a.part, parts, a.cols,

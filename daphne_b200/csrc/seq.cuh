@@ -51,6 +51,21 @@ template <typename T, int N> __device__ __forceinline__ void st_vec(T *p, const 
     *reinterpret_cast<Vec<T, N> *>(p) = x;
 }
 
+// N elements from global to shared memory, asynchronously (at once where they are fewer than four bytes).  fetch_commit
+// closes a group of them, fetch_wait<K> waits until all but the last K groups have arrived, for the calling thread.
+template <typename T, int N> __device__ __forceinline__ void fetch(T *to, const T *from) {
+    constexpr int bytes = sizeof(T) * N;
+    const unsigned at = (unsigned)__cvta_generic_to_shared(to);
+    if constexpr (bytes == 16)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(at), "l"(from) : "memory");
+    else if constexpr (bytes >= 4)
+        asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(at), "l"(from), "n"(bytes) : "memory");
+    else
+        st_vec<T, N>(to, ld_vec<T, N>(from));
+}
+__device__ __forceinline__ void fetch_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int K> __device__ __forceinline__ void fetch_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(K) : "memory"); }
+
 // whether rows of ld elements of es bytes starting at p all lie on multiples of `bytes` (absent operands do)
 inline bool rows_aligned(const void *p, int64_t ld, size_t es, size_t bytes) {
     return !p || (reinterpret_cast<uintptr_t>(p) % bytes == 0 && (size_t)ld * es % bytes == 0);
