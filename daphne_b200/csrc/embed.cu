@@ -95,10 +95,9 @@ int embed_launch(const void *table, int64_t vocab, int64_t cols, int64_t table_l
 // Every sort delivers key[] (ascending) and pos[] (ascending among equal keys).  A token that names no row gets the key
 // `vocab`, behind all others.
 
-constexpr int RANK_MAX = 16384; // tokens that are sorted by counting (their keys fill 64 KB of shared memory)
-constexpr int RANK_THREADS = 512;
-constexpr int RANK_SHARE = 8;                            // threads that count for one token
-constexpr int RANK_TILE = RANK_THREADS / RANK_SHARE * 2; // tokens of a CTA: two per thread, which share the loads
+constexpr int SORT_CHUNK = 1024;          // tokens that a CTA sorts by itself
+constexpr int MERGE_MAX = 40 * SORT_CHUNK; // tokens that are merged in one go: their sorted chunks lie in shared memory
+constexpr int MERGE_THREADS = 512, MERGE_TOKENS = 128; // of a CTA
 
 template <typename I>
 __device__ __forceinline__ uint32_t token_key(const void *tokens, int64_t ld, int64_t i, int64_t vocab,
@@ -111,55 +110,81 @@ __device__ __forceinline__ uint32_t token_key(const void *tokens, int64_t ld, in
     return (uint32_t)vocab;
 }
 
-// Place of token i in sorted order = how many tokens have a smaller key, or the same key and a smaller position.  All
-// keys lie in shared memory; RANK_SHARE threads count for a token, each over every RANK_SHARE-th packet of four keys.
-// n^2 comparisons in one launch without any exchange between CTAs: fewer microseconds than the launches of a radix sort
-// as long as the keys of all tokens fit (measured in the comment at embed_sort).
+// Chunks of SORT_CHUNK tokens, each sorted by (key, position): a bitonic network over 64-bit numbers, whose short strides
+// stay within a warp.  The last chunk is filled up with numbers behind all others, which are not written.
 template <typename I>
-__global__ void __launch_bounds__(RANK_THREADS)
-    token_rank_kernel(const void *tokens, int64_t tokens_ld, int n, int64_t vocab, uint32_t *__restrict__ key,
-                      uint32_t *__restrict__ pos, int32_t *status) {
-    extern __shared__ uint4 rank_smem[];
-    uint32_t *k = reinterpret_cast<uint32_t *>(rank_smem);
-    const int padded = (n + 3) / 4 * 4;
-    for (int i = threadIdx.x; i < padded; i += RANK_THREADS)
-        k[i] = i < n ? token_key<I>(tokens, tokens_ld, i, vocab, blockIdx.x == 0 ? status : nullptr) : 0xffffffffu;
+__global__ void __launch_bounds__(SORT_CHUNK / 2)
+    token_chunk_kernel(const void *tokens, int64_t tokens_ld, int n, int64_t vocab, uint32_t *__restrict__ key,
+                       uint32_t *__restrict__ pos, int32_t *status) {
+    __shared__ uint64_t v[SORT_CHUNK];
+    const int base = blockIdx.x * SORT_CHUNK, t = threadIdx.x;
+    for (int i = t; i < SORT_CHUNK; i += SORT_CHUNK / 2)
+        v[i] = base + i < n ? (uint64_t)token_key<I>(tokens, tokens_ld, base + i, vocab, status) << 32 | (uint32_t)(base + i)
+                            : ~(uint64_t)0;
     __syncthreads();
-    const int part = threadIdx.x % RANK_SHARE, i0 = blockIdx.x * RANK_TILE + threadIdx.x / RANK_SHARE * 2;
-    const unsigned stay = __ballot_sync(0xffffffffu, i0 < n); // the threads of a token stay or leave together
-    if (i0 >= n)
-        return;
-    const uint32_t ka = k[i0], kb = i0 + 1 < n ? k[i0 + 1] : 0xffffffffu;
-    int ca = 0, cb = 0;
-    // tokens in packets before the own one also count when their key is the same, those behind only when it is smaller
-    // (the largest key is below 2^32 - 1, so key + 1 does not wrap)
-    const int own = i0 / 4;
-    for (int q = part; q < own; q += RANK_SHARE) {
-        const uint4 x = rank_smem[q];
-        ca += (x.x <= ka) + (x.y <= ka) + (x.z <= ka) + (x.w <= ka);
-        cb += (x.x <= kb) + (x.y <= kb) + (x.z <= kb) + (x.w <= kb);
-    }
-    for (int q = own + 1 + part; q < padded / 4; q += RANK_SHARE) {
-        const uint4 x = rank_smem[q];
-        ca += (x.x < ka) + (x.y < ka) + (x.z < ka) + (x.w < ka);
-        cb += (x.x < kb) + (x.y < kb) + (x.z < kb) + (x.w < kb);
-    }
-    if (part == 0)
-        for (int j = own * 4; j < own * 4 + 4; j++) {
-            ca += k[j] < ka || (k[j] == ka && j < i0);
-            cb += k[j] < kb || (k[j] == kb && j < i0 + 1);
+    for (int size = 2; size <= SORT_CHUNK; size *= 2)
+        for (int stride = size / 2; stride >= 1; stride /= 2) {
+            const int i = 2 * t - (t & (stride - 1)), j = i + stride;
+            const uint64_t a = v[i], b = v[j];
+            if ((a > b) == ((i & size) == 0)) {
+                v[i] = b;
+                v[j] = a;
+            }
+            // up to a stride of 32 a warp's 32 pairs are the same 64 numbers in the next step
+            if (stride > 32 || (stride == 1 && size >= 64))
+                __syncthreads();
+            else
+                __syncwarp();
         }
+    for (int i = t; i < SORT_CHUNK; i += SORT_CHUNK / 2)
+        if (base + i < n) {
+            key[base + i] = (uint32_t)(v[i] >> 32);
+            pos[base + i] = (uint32_t)v[i];
+        }
+}
+
+// Sorted chunks -> sorted tokens: the place of a token is its place within its chunk plus, for every other chunk, how many of
+// its keys are smaller (or the same, in chunks in front).  A warp takes a token, a lane every 32nd chunk; the keys of all
+// chunks lie in shared memory, ten steps of a binary search each.
+__global__ void __launch_bounds__(MERGE_THREADS)
+    token_merge_kernel(const uint32_t *__restrict__ key, const uint32_t *__restrict__ pos, int n,
+                       uint32_t *__restrict__ key_out, uint32_t *__restrict__ pos_out) {
+    extern __shared__ uint4 merge_smem[];
+    uint32_t *k = reinterpret_cast<uint32_t *>(merge_smem);
+    const int quads = n / 4; // the buffers are 16-byte aligned
+#pragma unroll 8
+    for (int i = threadIdx.x; i < quads; i += MERGE_THREADS)
+        merge_smem[i] = reinterpret_cast<const uint4 *>(key)[i];
+    for (int i = quads * 4 + threadIdx.x; i < n; i += MERGE_THREADS)
+        k[i] = key[i];
+    __syncthreads();
+    const int lane = threadIdx.x % 32, chunks = (n + SORT_CHUNK - 1) / SORT_CHUNK;
+    const int group = chunks <= 8 ? 8 : (chunks <= 16 ? 16 : 32); // lanes that share a token
+    const int first = blockIdx.x * MERGE_TOKENS, part = lane % group;
+    for (int i = first + threadIdx.x / group; i < first + MERGE_TOKENS; i += MERGE_THREADS / group) {
+        const int at = i < n ? i : n - 1, own = at / SORT_CHUNK; // all lanes stay for the sum
+        const uint32_t mine = k[at];
+        int place = 0;
+        for (int c = part; c < chunks; c += group) {
+            if (c == own) {
+                place += at - own * SORT_CHUNK;
+                continue;
+            }
+            const uint32_t *chunk = k + c * SORT_CHUNK;
+            const int len = n - c * SORT_CHUNK < SORT_CHUNK ? n - c * SORT_CHUNK : SORT_CHUNK;
+            const uint32_t below = mine + (c < own); // keys are smaller than 2^32 - 1
+            int lo = 0;
 #pragma unroll
-    for (int o = RANK_SHARE / 2; o >= 1; o >>= 1) {
-        ca += __shfl_xor_sync(stay, ca, o);
-        cb += __shfl_xor_sync(stay, cb, o);
-    }
-    if (part == 0) {
-        key[ca] = ka;
-        pos[ca] = (uint32_t)i0;
-        if (i0 + 1 < n) {
-            key[cb] = kb;
-            pos[cb] = (uint32_t)(i0 + 1);
+            for (int step = SORT_CHUNK / 2; step >= 1; step /= 2)
+                if (lo + step <= len && chunk[lo + step - 1] < below)
+                    lo += step;
+            place += lo + (lo < len && chunk[lo] < below); // the steps add up to SORT_CHUNK - 1
+        }
+        for (int o = group / 2; o >= 1; o >>= 1)
+            place += __shfl_xor_sync(0xffffffffu, place, o);
+        if (part == 0 && i < n) {
+            key_out[place] = mine;
+            pos_out[place] = pos[at];
         }
     }
 }
@@ -301,13 +326,13 @@ __global__ void __launch_bounds__(RADIX_THREADS)
 constexpr int SUM_THREADS = 128;
 constexpr int SUM_RUN = 32;   // sorted tokens that one group of threads adds up
 constexpr int SUM_AHEAD = 4;  // gradient rows in flight per thread
-constexpr int FILL_ROWS = 32; // table rows per CTA that are looked at for being untouched
+constexpr int FILL_ROWS = 128; // table rows per CTA that are looked at for being untouched
 
 struct SumArgs {
     const uint32_t *key, *pos;
     int64_t n, cols, vocab, grad_ld, res_ld, part_ld;
     int64_t runs;     // ceil(n / SUM_RUN)
-    unsigned fill_x;  // CTAs (in x) that write zeros
+    unsigned sum_x;   // CTAs (in x) that add; those behind them write zeros
     int log_tpr;
 };
 
@@ -315,18 +340,18 @@ struct SumArgs {
 // where the token changes, the sum is finished -- written to the table when all its rows lie in the run, to `part`
 // otherwise: part[run][0] holds the sum of a token that came over from the run before, part[run][1] that of a token that
 // starts in the run and goes on behind it.  Equal amounts of work whatever the tokens' frequencies.
-// The CTAs in front write zeros to the table's untouched rows (not when adding to the table).
+// The CTAs behind write zeros to the table's untouched rows (not when adding to the table).
 // Bound by memory: every gradient row is read once, every table row written once.
 template <typename T, typename R, int N, bool ADD>
 __global__ void __launch_bounds__(SUM_THREADS)
     embed_sum_kernel(SumArgs a, const T *__restrict__ grad, wide_t<T> scale, R *__restrict__ res,
                      wide_t<T> *__restrict__ part) {
     using W = wide_t<T>;
-    if (blockIdx.x < a.fill_x) {
-        __shared__ uint32_t hit;
-        const int64_t v0 = (int64_t)blockIdx.x * FILL_ROWS;
-        if (threadIdx.x == 0)
-            hit = 0;
+    if (blockIdx.x >= a.sum_x) {
+        __shared__ uint32_t hit[FILL_ROWS / 32];
+        const int64_t v0 = (int64_t)(blockIdx.x - a.sum_x) * FILL_ROWS;
+        if (threadIdx.x < FILL_ROWS / 32)
+            hit[threadIdx.x] = 0;
         __syncthreads();
         // first sorted token >= v0
         int64_t lo = 0, hi = a.n;
@@ -343,13 +368,12 @@ __global__ void __launch_bounds__(SUM_THREADS)
             if (v >= FILL_ROWS)
                 break;
             if (i == lo || a.key[i] != a.key[i - 1])
-                atomicOr(&hit, 1u << v);
+                atomicOr(&hit[v / 32], 1u << (v % 32));
         }
         __syncthreads();
-        const uint32_t mask = hit;
         const int64_t packets = a.cols / N;
         for (int j = 0; j < FILL_ROWS && v0 + j < a.vocab; j++) {
-            if (mask >> j & 1u)
+            if (hit[j / 32] >> (j % 32) & 1u)
                 continue;
             R *dst = res + (v0 + j) * a.res_ld;
             Vec<R, N> z;
@@ -366,7 +390,7 @@ __global__ void __launch_bounds__(SUM_THREADS)
         return;
     }
     const int tpr = 1 << a.log_tpr, tx = threadIdx.x & (tpr - 1), ty = threadIdx.x >> a.log_tpr;
-    const int64_t run = (int64_t)(blockIdx.x - a.fill_x) * (SUM_THREADS >> a.log_tpr) + ty;
+    const int64_t run = (int64_t)blockIdx.x * (SUM_THREADS >> a.log_tpr) + ty;
     if (run >= a.runs)
         return;
     const int64_t b = run * SUM_RUN, e = b + SUM_RUN < a.n ? b + SUM_RUN : a.n;
@@ -450,18 +474,19 @@ __global__ void __launch_bounds__(SUM_THREADS)
 }
 
 // Tokens whose rows span several runs: the run in which such a token starts adds the partial sums behind it, in order.
-// JOIN_Y groups of threads take equal shares of the runs, their sums are added in the order of the shares.
-constexpr int JOIN_X = 32, JOIN_Y = 8;
+// A CTA looks at one run and 32 x JOIN_N columns; its warps take equal shares of the runs, whose sums are added in the
+// order of the shares.  Most CTAs find nothing to do.
+constexpr int JOIN_Y = 8, JOIN_N = 4;
 template <typename T, typename R, bool ADD>
-__global__ void __launch_bounds__(JOIN_X *JOIN_Y)
+__global__ void __launch_bounds__(32 * JOIN_Y)
     embed_join_kernel(SumArgs a, wide_t<T> scale, R *__restrict__ res, const wide_t<T> *__restrict__ part) {
     using W = wide_t<T>;
-    __shared__ W sums[JOIN_Y][JOIN_X];
-    const int tx = threadIdx.x % JOIN_X, ty = threadIdx.x / JOIN_X;
+    __shared__ W sums[JOIN_Y][32 * JOIN_N];
+    const int tx = threadIdx.x % 32, ty = threadIdx.x / 32;
     for (int64_t run = blockIdx.x; run + 1 < a.runs; run += gridDim.x) {
         const int64_t b = run * SUM_RUN, e = b + SUM_RUN; // e < n: the run is not the last
-        const uint32_t v = a.key[e - 1];
-        if (v >= (uint32_t)a.vocab || a.key[e] != v || (b > 0 && a.key[b] == v && a.key[b - 1] == v))
+        const uint32_t v = a.key[e - 1], next = a.key[e], start = a.key[b], before = b > 0 ? a.key[b - 1] : 0xffffffffu;
+        if (v >= (uint32_t)a.vocab || next != v || (start == v && before == v))
             continue; // uniform over the CTA: the last token ends here, or started in an earlier run
         // one past the last row with this token
         int64_t lo = e + 1, hi = a.n;
@@ -475,22 +500,34 @@ __global__ void __launch_bounds__(JOIN_X *JOIN_Y)
         const int64_t more = (lo - 1) / SUM_RUN - run; // runs behind this one that hold a part
         const int64_t share = (more + JOIN_Y) / JOIN_Y;
         const int64_t first = ty * share, last = first + share < more + 1 ? first + share : more + 1;
-        for (int64_t c0 = (int64_t)blockIdx.y * JOIN_X; c0 < a.cols; c0 += (int64_t)gridDim.y * JOIN_X) {
-            const int64_t c = c0 + tx;
-            W acc = W(0);
-            if (c < a.cols) {
+        for (int64_t c0 = (int64_t)blockIdx.y * 32 * JOIN_N; c0 < a.cols; c0 += (int64_t)gridDim.y * 32 * JOIN_N) {
+            W acc[JOIN_N];
+#pragma unroll
+            for (int k = 0; k < JOIN_N; k++)
+                acc[k] = W(0);
+            if (c0 + tx * JOIN_N < a.cols) { // part_ld is a multiple of JOIN_N
 #pragma unroll 8
-                for (int64_t j = first; j < last; j++)
-                    acc += part[((run + j) * 2 + (j == 0 ? 1 : 0)) * a.part_ld + c];
+                for (int64_t j = first; j < last; j++) {
+                    const W *p = part + ((run + j) * 2 + (j == 0 ? 1 : 0)) * a.part_ld + c0 + tx * JOIN_N;
+#pragma unroll
+                    for (int k = 0; k < JOIN_N; k += 16 / sizeof(W)) {
+                        const Vec<W, 16 / sizeof(W)> x = ld_vec<W, 16 / sizeof(W)>(p + k);
+#pragma unroll
+                        for (int i = 0; i < (int)(16 / sizeof(W)); i++)
+                            acc[k + i] += x.v[i];
+                    }
+                }
             }
             __syncthreads();
-            sums[ty][tx] = acc;
+#pragma unroll
+            for (int k = 0; k < JOIN_N; k++)
+                sums[ty][tx * JOIN_N + k] = acc[k];
             __syncthreads();
-            if (ty == 0 && c < a.cols) {
-                W s = sums[0][tx];
+            for (int i = threadIdx.x; i < 32 * JOIN_N && c0 + i < a.cols; i += 32 * JOIN_Y) {
+                W s = sums[0][i];
                 for (int k = 1; k < JOIN_Y; k++)
-                    s += sums[k][tx];
-                R *dst = res + (int64_t)v * a.res_ld + c;
+                    s += sums[k][i];
+                R *dst = res + (int64_t)v * a.res_ld + c0 + i;
                 *dst = narrow<R>(ADD ? W(widen(*dst)) + s * scale : s * scale);
             }
         }
@@ -512,10 +549,10 @@ GradPlan grad_plan(size_t wide_size, int64_t vocab, int64_t cols, int64_t n) {
     p.runs = (n + SUM_RUN - 1) / SUM_RUN;
     p.part_ld = (cols + 7) / 8 * 8;
     p.bits = log2_ceil(vocab + 1);
-    p.passes = n <= RANK_MAX ? 0 : (p.bits + RADIX_BITS - 1) / RADIX_BITS;
+    p.passes = n <= MERGE_MAX ? 0 : (p.bits + RADIX_BITS - 1) / RADIX_BITS;
     p.tiles = (n + RADIX_TILE - 1) / RADIX_TILE;
     size_t at = 0;
-    for (int i = 0; i < (p.passes > 1 ? 2 : 1); i++) {
+    for (int i = 0; i < (p.passes == 1 || n <= SORT_CHUNK ? 1 : 2); i++) {
         p.key_off[i] = take(&at, (size_t)n * 4);
         p.pos_off[i] = take(&at, (size_t)n * 4);
     }
@@ -535,18 +572,24 @@ int embed_sort(const GradPlan &p, const void *tokens, int64_t tokens_ld, int64_t
         q[i] = reinterpret_cast<uint32_t *>(scratch + p.pos_off[i]);
     }
     if (p.passes == 0) {
-        static PerDeviceOnce once;
-        if (once.need()) {
-            DB2_CUDA(cudaFuncSetAttribute(token_rank_kernel<I>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                          RANK_MAX * 4));
-            once.mark();
-        }
-        const int grid = (int)((n + RANK_TILE - 1) / RANK_TILE);
-        token_rank_kernel<I><<<grid, RANK_THREADS, (size_t)(n + 3) / 4 * 16, st>>>(tokens, tokens_ld, (int)n, vocab,
-                                                                                  k[0], q[0], status);
-        DB2_TRY(after_launch("token_rank_kernel"));
+        // two launches, or one: 16384 tokens in 13 us, where counting with 9-bit digits takes six launches
+        const int chunks = (int)((n + SORT_CHUNK - 1) / SORT_CHUNK);
+        token_chunk_kernel<I><<<chunks, SORT_CHUNK / 2, 0, st>>>(tokens, tokens_ld, (int)n, vocab, k[0], q[0], status);
+        DB2_TRY(after_launch("token_chunk_kernel"));
         *key = k[0];
         *pos = q[0];
+        if (chunks == 1)
+            return DB2_OK;
+        static PerDeviceOnce once;
+        if (once.need()) {
+            DB2_CUDA(cudaFuncSetAttribute(token_merge_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, MERGE_MAX * 4));
+            once.mark();
+        }
+        token_merge_kernel<<<(unsigned)((n + MERGE_TOKENS - 1) / MERGE_TOKENS), MERGE_THREADS, (size_t)(n + 3) / 4 * 16,
+                             st>>>(k[0], q[0], (int)n, k[1], q[1]);
+        DB2_TRY(after_launch("token_merge_kernel"));
+        *key = k[1];
+        *pos = q[1];
         return DB2_OK;
     }
     uint32_t *counts = reinterpret_cast<uint32_t *>(scratch + p.counts_off);
@@ -580,16 +623,17 @@ int embed_sum(SumArgs a, const void *grad, double scale, void *res, void *part, 
     const int64_t gx = (a.runs + groups - 1) / groups;
     int64_t gy = (packets + (1 << a.log_tpr) - 1) >> a.log_tpr;
     gy = gy > 1024 ? 1024 : gy;
-    a.fill_x = ADD ? 0u : (unsigned)((a.vocab + FILL_ROWS - 1) / FILL_ROWS);
-    embed_sum_kernel<T, R, N, ADD><<<dim3((unsigned)(gx + a.fill_x), (unsigned)gy), SUM_THREADS, 0, st>>>(
+    a.sum_x = (unsigned)gx;
+    const int64_t fill = ADD ? 0 : (a.vocab + FILL_ROWS - 1) / FILL_ROWS;
+    embed_sum_kernel<T, R, N, ADD><<<dim3((unsigned)(gx + fill), (unsigned)gy), SUM_THREADS, 0, st>>>(
         a, static_cast<const T *>(grad), (wide_t<T>)scale, static_cast<R *>(res), static_cast<wide_t<T> *>(part));
     DB2_TRY(after_launch("embed_sum_kernel"));
     if (a.runs > 1) {
-        int64_t jy = (a.cols + JOIN_X - 1) / JOIN_X;
-        jy = jy > 128 ? 128 : jy;
+        int64_t jy = (a.cols + 32 * JOIN_N - 1) / (32 * JOIN_N);
+        jy = jy > 64 ? 64 : jy;
         int64_t jx = a.runs - 1;
-        jx = jx > 4096 ? 4096 : jx;
-        embed_join_kernel<T, R, ADD><<<dim3((unsigned)jx, (unsigned)jy), JOIN_X * JOIN_Y, 0, st>>>(
+        jx = jx > 65536 / jy ? 65536 / jy : jx;
+        embed_join_kernel<T, R, ADD><<<dim3((unsigned)jx, (unsigned)jy), 32 * JOIN_Y, 0, st>>>(
             a, (wide_t<T>)scale, static_cast<R *>(res), static_cast<const wide_t<T> *>(part));
         DB2_TRY(after_launch("embed_join_kernel"));
     }

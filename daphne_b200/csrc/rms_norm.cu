@@ -45,7 +45,7 @@ template <typename W> struct RowSum {
 
 // Rows on their way: a thread's packets of its next NORM_STAGES - 1 rows, in shared memory.  It reads nothing else
 // there, so no barrier is needed.
-constexpr int NORM_STAGES = 3;
+constexpr int NORM_STAGES = 2;
 extern __shared__ __align__(16) unsigned char norm_smem[];
 template <typename T, int N, int PPT> struct RowRing {
     int operands, stage = 0;
@@ -74,11 +74,11 @@ template <typename T> struct NormArgs { // x, residual and sum may be the same m
 
 template <typename T, int N>
 __device__ __forceinline__ Vec<T, N> add_residual(const Vec<T, N> &x, const Vec<T, N> &r) {
-    Vec<T, N> s;
+    wide_t<T> s[N];
 #pragma unroll
     for (int k = 0; k < N; k++)
-        s.v[k] = narrow<T>(widen(x.v[k]) + widen(r.v[k]));
-    return s;
+        s[k] = widen(x.v[k]) + widen(r.v[k]);
+    return narrow_all<T, N>(s);
 }
 template <typename T, int N> __device__ __forceinline__ void squares(const Vec<T, N> &s, wide_t<T> *ss) {
 #pragma unroll
@@ -97,14 +97,14 @@ __device__ __forceinline__ void normalised(const Vec<T, N> &s, const T *weight, 
     for (int k = 0; k < N; k++)
         y[k] = weight ? widen(s.v[k]) * rstd * widen(w.v[k]) : widen(s.v[k]) * rstd;
 }
-// |y| as an integer: the order of non-negative floats is that of their bits, and a NaN is above infinity, so a maximum
-// over the bits does not depend on the order and keeps a NaN
+// max |y|, NaN if there is one, as an integer: the order of non-negative floats is that of their bits, and a NaN is above
+// infinity, so that maxima over the bits do not depend on the order and keep a NaN
 template <int N> __device__ __forceinline__ unsigned largest(const float *y) {
-    unsigned m = 0;
+    float m = 0.0f;
 #pragma unroll
     for (int k = 0; k < N; k++)
-        m = max(m, __float_as_uint(y[k]) & 0x7fffffffu);
-    return m;
+        asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(m), "f"(fabsf(y[k])));
+    return __float_as_uint(m);
 }
 // 1 for a group of zeros; never below the smallest normal number, whose reciprocal is finite
 __device__ __forceinline__ float scale_of(unsigned most) {
@@ -195,11 +195,7 @@ __global__ void __launch_bounds__(NORM_MAX_WARPS * 32) norm_rows_kernel(NormArgs
                     if (tx + k * tpr < packets) {
                         W y[N];
                         normalised<T, N>(s[k], a.weight, tx + k * tpr, rstd, y);
-                        Vec<T, N> z;
-#pragma unroll
-                        for (int j = 0; j < N; j++)
-                            z.v[j] = narrow<T>(y[j]);
-                        st_vec<T, N>(res + (tx + k * tpr) * N, z);
+                        st_vec<T, N>(res + (tx + k * tpr) * N, narrow_all<T, N>(y));
                     }
             }
         } else {
@@ -389,53 +385,48 @@ __global__ void __launch_bounds__(NORM_MAX_WARPS * 32) norm_grad_rows_kernel(Nor
         const bool live = r < a.rows;
         const W rstd = next_rstd;
         next_rstd = r + step < a.rows ? a.rstd[r + step] : W(0);
-        Vec<T, N> g[PPT], s[PPT], d[PPT];
-        fetch_wait<NORM_STAGES - 2>();
+        load(ring.last(), r + (NORM_STAGES - 1) * step);
+        fetch_wait<NORM_STAGES - 1>();
+        W dot = 0;
         if (live) {
 #pragma unroll
             for (int k = 0; k < PPT; k++)
                 if (tx + k * tpr < packets) {
-                    g[k] = ring.get(0, k);
-                    s[k] = ring.get(1, k);
-                    if (a.dsum)
-                        d[k] = ring.get(2, k);
+                    const Vec<T, N> g = ring.get(0, k), s = ring.get(1, k);
+                    Vec<T, N> w;
+                    if (a.weight)
+                        w = ld_vec<T, N>(a.weight + (tx + k * tpr) * N);
+#pragma unroll
+                    for (int j = 0; j < N; j++) {
+                        const W gs = widen(g.v[j]) * widen(s.v[j]);
+                        dot = a.weight ? dot + gs * widen(w.v[j]) : dot + gs;
+                        dw[k][j] += gs * rstd;
+                    }
                 }
         }
-        load(ring.last(), r + (NORM_STAGES - 1) * step);
-        ring.next();
-        W dot = 0;
-#pragma unroll
-        for (int k = 0; k < PPT; k++)
-            if (live && tx + k * tpr < packets) {
-                Vec<T, N> w;
-                if (a.weight)
-                    w = ld_vec<T, N>(a.weight + (tx + k * tpr) * N);
-#pragma unroll
-                for (int j = 0; j < N; j++) {
-                    const W t = a.weight ? widen(g[k].v[j]) * widen(w.v[j]) : W(widen(g[k].v[j]));
-                    dot += t * widen(s[k].v[j]);
-                    dw[k][j] += widen(g[k].v[j]) * (widen(s[k].v[j]) * rstd);
-                }
-            }
         const W factor = row_sum(dot, tpr) / W(a.cols) * rstd * rstd;
         if (live) {
 #pragma unroll
             for (int k = 0; k < PPT; k++)
                 if (tx + k * tpr < packets) {
-                    Vec<T, N> w, z;
+                    const Vec<T, N> g = ring.get(0, k), s = ring.get(1, k);
+                    Vec<T, N> w, d;
                     if (a.weight)
                         w = ld_vec<T, N>(a.weight + (tx + k * tpr) * N);
+                    if (a.dsum)
+                        d = ring.get(2, k);
+                    W v[N];
 #pragma unroll
                     for (int j = 0; j < N; j++) {
-                        const W t = a.weight ? widen(g[k].v[j]) * widen(w.v[j]) : W(widen(g[k].v[j]));
-                        W v = rstd * (t - widen(s[k].v[j]) * factor);
+                        const W t = a.weight ? widen(g.v[j]) * widen(w.v[j]) : W(widen(g.v[j]));
+                        v[j] = rstd * (t - widen(s.v[j]) * factor);
                         if (a.dsum)
-                            v += widen(d[k].v[j]);
-                        z.v[j] = narrow<T>(v);
+                            v[j] += widen(d.v[j]);
                     }
-                    st_vec<T, N>(a.dx + r * a.dx_ld + (tx + k * tpr) * N, z);
+                    st_vec<T, N>(a.dx + r * a.dx_ld + (tx + k * tpr) * N, narrow_all<T, N>(v));
                 }
         }
+        ring.next();
     }
     if (!a.part)
         return;
@@ -560,12 +551,13 @@ struct RowPlan {
     int tpr, ppt, block;
     bool fits;
 };
-RowPlan row_plan(int64_t packets, int64_t rows, int first, int most, int step) {
+constexpr int NORM_SMEM = 210 << 10, NORM_RING = 192 << 10; // of a CTA: all, and the ring
+RowPlan row_plan(int64_t packets, int64_t rows, int first, int most, int step, int place_bytes) {
     RowPlan p{0, 0, 0, false};
     for (int ppt = first; ppt <= most; ppt += step) {
         int64_t tpr = (packets + ppt - 1) / ppt;
         tpr = tpr < 32 ? next_pow2(tpr < 8 ? 8 : tpr) : (tpr + 31) / 32 * 32;
-        if (tpr > NORM_MAX_WARPS * 32)
+        if (tpr > NORM_MAX_WARPS * 32 || tpr * ppt * place_bytes > NORM_RING)
             continue;
         if (!p.fits || (rows >= sm_count() && tpr * ppt <= (int64_t)p.tpr * p.ppt)) {
             p.tpr = (int)tpr;
@@ -576,11 +568,12 @@ RowPlan row_plan(int64_t packets, int64_t rows, int first, int most, int step) {
     p.block = p.fits ? p.tpr * (p.tpr < 256 ? 256 / p.tpr : 1) : 0;
     return p;
 }
-// packets a thread that there are kernels for: 1, 2, 3 (forward), or 4 and 8 single elements
-template <int N> RowPlan row_plan(int64_t cols, int64_t rows, bool back) {
-    return N == 1 ? row_plan(cols, rows, 4, 8, 4) : row_plan(cols / N, rows, 1, back ? 2 : 3, 1);
+// packets a thread that there are kernels for: 1 to 3 (gradient: 4), or 4 and 8 single elements
+template <typename T, int N> RowPlan row_plan(int64_t cols, int64_t rows, bool back) {
+    const int place = NORM_STAGES * (back ? 3 : 2) * N * (int)sizeof(T);
+    return N == 1 ? row_plan(cols, rows, 4, 8, 4, place) : row_plan(cols / N, rows, 1, back ? 4 : 3, 1, place);
 }
-#define DB2_BY_PACKETS(N, ppt, LAUNCH)                                                                                 \
+#define DB2_BY_PACKETS(N, BACK, ppt, LAUNCH)                                                                                 \
     if constexpr (N == 1) {                                                                                            \
         if (ppt == 4) {                                                                                                \
             LAUNCH(4)                                                                                                  \
@@ -591,12 +584,15 @@ template <int N> RowPlan row_plan(int64_t cols, int64_t rows, bool back) {
         LAUNCH(1)                                                                                                      \
     } else if (ppt == 2) {                                                                                             \
         LAUNCH(2)                                                                                                      \
-    } else {                                                                                                           \
+    } else if (ppt == 3) {                                                                                             \
         LAUNCH(3)                                                                                                      \
+    } else {                                                                                                           \
+        if constexpr (BACK) {                                                                                          \
+            LAUNCH(4)                                                                                                  \
+        }                                                                                                              \
     }
 
 // CTAs that stay on the device for all rows: as many as fit at once
-constexpr int NORM_SMEM = 200 << 10; // every launch asks for less
 template <typename K> int resident_ctas(K kernel, PerDeviceOnce &once, int block, size_t smem, int64_t most, unsigned *ctas) {
     DB2_CHECK(smem <= (size_t)NORM_SMEM, DB2_ECUDA, "rmsNorm: %zu bytes of shared memory", smem);
     if (once.need()) {
@@ -615,7 +611,7 @@ template <typename K> int resident_ctas(K kernel, PerDeviceOnce &once, int block
 }
 
 template <typename T, int N, bool Q8> int norm_launch(const NormArgs<T> &a, cudaStream_t st) {
-    const RowPlan p = row_plan<N>(a.cols, a.rows, false);
+    const RowPlan p = row_plan<T, N>(a.cols, a.rows, false);
     if (!p.fits) {
         const int64_t max_grid = (int64_t)1 << 30;
         norm_long_kernel<T, N, Q8><<<(unsigned)(a.rows < max_grid ? a.rows : max_grid), LONG_BLOCK, 0, st>>>(a);
@@ -628,19 +624,19 @@ template <typename T, int N, bool Q8> int norm_launch(const NormArgs<T> &a, cuda
     static PerDeviceOnce once;                                                                                         \
     DB2_TRY(resident_ctas(norm_rows_kernel<T, N, PPT, Q8>, once, p.block, smem, (a.rows + at_once - 1) / at_once, &grid));   \
     norm_rows_kernel<T, N, PPT, Q8><<<grid, p.block, smem, st>>>(a, p.tpr);
-    DB2_BY_PACKETS(N, p.ppt, DB2_NORM)
+    DB2_BY_PACKETS(N, false, p.ppt, DB2_NORM)
 #undef DB2_NORM
     return after_launch("norm_rows_kernel");
 }
 
 // most CTAs of the gradient kernel: each keeps its own column sums
 int64_t grad_ctas(int64_t rows) {
-    const int64_t cap = (int64_t)sm_count() * 4;
+    const int64_t cap = (int64_t)sm_count() * 8;
     return rows < 1 ? 1 : (rows < cap ? rows : cap);
 }
 
 template <typename T, int N> int norm_grad_launch(NormGradArgs<T> a, wide_t<T> *dweight, cudaStream_t st) {
-    const RowPlan p = row_plan<N>(a.cols, a.rows, true);
+    const RowPlan p = row_plan<T, N>(a.cols, a.rows, true);
     const int64_t ctas = grad_ctas(a.rows);
     int parts;
     if (!p.fits) {
@@ -662,7 +658,7 @@ template <typename T, int N> int norm_grad_launch(NormGradArgs<T> a, wide_t<T> *
     static PerDeviceOnce once;                                                                                         \
     DB2_TRY(resident_ctas(norm_grad_rows_kernel<T, N, PPT>, once, p.block, smem, blocks < ctas ? blocks : ctas, &grid));     \
     norm_grad_rows_kernel<T, N, PPT><<<grid, p.block, smem, st>>>(a, p.tpr);
-        DB2_BY_PACKETS(N, p.ppt, DB2_NORM_GRAD)
+        DB2_BY_PACKETS(N, true, p.ppt, DB2_NORM_GRAD)
 #undef DB2_NORM_GRAD
         DB2_TRY(after_launch("norm_grad_rows_kernel"));
         parts = (int)grid;

@@ -51,6 +51,25 @@ template <typename T, int N> __device__ __forceinline__ void st_vec(T *p, const 
     *reinterpret_cast<Vec<T, N> *>(p) = x;
 }
 
+// the same for N values, pairs of 16-bit ones in one instruction
+template <typename T, int N, typename W> __device__ __forceinline__ Vec<T, N> narrow_all(const W *x) {
+    Vec<T, N> z;
+    if constexpr (sizeof(T) == 2 && N % 2 == 0) {
+#pragma unroll
+        for (int k = 0; k < N; k += 2) {
+            if constexpr (std::is_same_v<T, __half>)
+                *reinterpret_cast<__half2 *>(&z.v[k]) = __floats2half2_rn(x[k], x[k + 1]);
+            else
+                *reinterpret_cast<__nv_bfloat162 *>(&z.v[k]) = __floats2bfloat162_rn(x[k], x[k + 1]);
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < N; k++)
+            z.v[k] = narrow<T>(x[k]);
+    }
+    return z;
+}
+
 // N elements from global to shared memory, asynchronously (at once where they are fewer than four bytes).  fetch_commit
 // closes a group of them, fetch_wait<K> waits until all but the last K groups have arrived, for the calling thread.
 template <typename T, int N> __device__ __forceinline__ void fetch(T *to, const T *from) {

@@ -113,10 +113,16 @@ def _expect(G, tok, vocab, scale):
     (33, 64, 3000, 8, 8, "i64", "outside"),
     (500, 130, 4097, 3, 1, "i64", "skewed"),
     (5, 2000, 1000, 0, 0, "i32", "one"),             # one token: every run holds a part of one sum
-    (70000, 16, 16384, 0, 0, "i64", "skewed"),       # the most tokens that are sorted by counting
-    (70000, 24, 16385, 0, 0, "i64", "outside"),      # the fewest that go through the radix passes
-    (300000, 8, 20001, 0, 0, "i64", "skewed"),       # three passes
+    (90, 16, 1024, 0, 0, "i64", "skewed"),           # one chunk of the sort, and one token more
+    (90, 16, 1025, 0, 0, "i32", "outside"),
+    (3000, 12, 9001, 0, 0, "i64", "skewed"),         # nine chunks
+    (70000, 16, 16384, 0, 0, "i64", "skewed"),       # sixteen chunks, no remainder
+    (70000, 24, 16385, 0, 0, "i64", "outside"),
+    (70000, 8, 40960, 0, 0, "i64", "skewed"),        # the most tokens that are merged, and one more for the radix passes
+    (70000, 8, 40961, 0, 0, "i64", "outside"),
+    (300000, 8, 45001, 0, 0, "i64", "skewed"),       # three passes
     (400, 9, 50000, 1, 0, "i32", "skewed"),          # one pass
+    (3, 4, 40000, 0, 0, "i64", "one"),
     (3, 4, 30000, 0, 0, "i64", "one"),
 ])
 def test_gradient(tname, res_t, vocab, cols, n, pad, shift, index, kind):

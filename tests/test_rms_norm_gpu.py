@@ -21,6 +21,7 @@ SHAPES = [  # rows, cols, pad, shift
     (1, 1, 0, 0), (3, 7, 0, 0), (5, 64, 0, 0), (300, 33, 0, 0), (200, 129, 7, 0), (170, 333, 0, 1), (64, 1000, 24, 16),
     (1000, 512, 0, 0), (9, 4096, 0, 0), (300, 4100, 4, 8), (4, 9001, 0, 0), (160, 8200, 0, 8), (2, 16500, 12, 0),
     (3, 40000, 0, 0), (150, 33000, 0, 8), (40003, 8, 0, 0),
+    (150, 12288, 0, 0), (4, 20480, 0, 0), (151, 640, 0, 0), (7000, 320, 0, 8), (6001, 24, 0, 0),
 ]
 
 
