@@ -95,9 +95,40 @@ int embed_launch(const void *table, int64_t vocab, int64_t cols, int64_t table_l
 // Every sort delivers key[] (ascending) and pos[] (ascending among equal keys).  A token that names no row gets the key
 // `vocab`, behind all others.
 
-constexpr int SORT_CHUNK = 1024;          // tokens that a CTA sorts by itself
-constexpr int MERGE_MAX = 40 * SORT_CHUNK; // tokens that are merged in one go: their sorted chunks lie in shared memory
+constexpr int SORT_CHUNK = 512;            // tokens that a CTA sorts by itself
+constexpr int MERGE_MAX = 80 * SORT_CHUNK; // tokens that are merged in one go: their sorted chunks lie in shared memory
 constexpr int MERGE_THREADS = 512, MERGE_TOKENS = 128; // of a CTA
+
+// The table's rows [first, first + rows), which become zero before the sums are written: the sorting kernels, which keep
+// few SMs busy, do it with further CTAs.  A CTA writes 128 packets of a row at a time.
+struct Zeros {
+    char *at;
+    int64_t first, rows, row_bytes, ld_bytes;
+    int packet; // 16, or the size of an element
+};
+template <int BYTES> struct alignas(BYTES) Blank {
+    unsigned char b[BYTES];
+};
+template <int BYTES> __device__ __forceinline__ void write_zeros(const Zeros &z, int cta, int ctas) {
+    const int groups = blockDim.x / 128, tx = threadIdx.x % 128;
+    const int64_t packets = z.row_bytes / BYTES;
+    const Blank<BYTES> zero{};
+    for (int64_t r = (int64_t)cta * groups + threadIdx.x / 128; r < z.rows; r += (int64_t)ctas * groups) {
+        char *row = z.at + (z.first + r) * z.ld_bytes;
+#pragma unroll 4
+        for (int64_t p = tx; p < packets; p += 128)
+            *reinterpret_cast<Blank<BYTES> *>(row + p * BYTES) = zero;
+    }
+}
+__device__ __forceinline__ void write_zeros_any(const Zeros &z, int cta, int ctas) {
+    switch (z.packet) {
+    case 16: write_zeros<16>(z, cta, ctas); break;
+    case 8: write_zeros<8>(z, cta, ctas); break;
+    case 4: write_zeros<4>(z, cta, ctas); break;
+    default: write_zeros<2>(z, cta, ctas); break;
+    }
+}
+__global__ void __launch_bounds__(512) table_zero_kernel(Zeros z) { write_zeros_any(z, blockIdx.x, gridDim.x); }
 
 template <typename I>
 __device__ __forceinline__ uint32_t token_key(const void *tokens, int64_t ld, int64_t i, int64_t vocab,
@@ -110,37 +141,45 @@ __device__ __forceinline__ uint32_t token_key(const void *tokens, int64_t ld, in
     return (uint32_t)vocab;
 }
 
-// Chunks of SORT_CHUNK tokens, each sorted by (key, position): a bitonic network over 64-bit numbers, whose short strides
-// stay within a warp.  The last chunk is filled up with numbers behind all others, which are not written.
+// Chunks of SORT_CHUNK tokens, each sorted by (key, position): a token's place is how many keys of its chunk are smaller, or
+// the same and in front of it.  A thread per token compares it with all of them, four at a time; what comes before and
+// behind the warp's own 32 tokens needs one comparison each.  (A bitonic network over chunks of 1024 takes 9 us.)
 template <typename I>
-__global__ void __launch_bounds__(SORT_CHUNK / 2)
+__global__ void __launch_bounds__(SORT_CHUNK)
     token_chunk_kernel(const void *tokens, int64_t tokens_ld, int n, int64_t vocab, uint32_t *__restrict__ key,
-                       uint32_t *__restrict__ pos, int32_t *status) {
-    __shared__ uint64_t v[SORT_CHUNK];
+                       uint32_t *__restrict__ pos, int32_t *status, int chunks, Zeros z) {
+    if ((int)blockIdx.x >= chunks) {
+        write_zeros_any(z, blockIdx.x - chunks, gridDim.x - chunks);
+        return;
+    }
+    __shared__ uint4 quads[SORT_CHUNK / 4];
     const int base = blockIdx.x * SORT_CHUNK, t = threadIdx.x;
-    for (int i = t; i < SORT_CHUNK; i += SORT_CHUNK / 2)
-        v[i] = base + i < n ? (uint64_t)token_key<I>(tokens, tokens_ld, base + i, vocab, status) << 32 | (uint32_t)(base + i)
-                            : ~(uint64_t)0;
+    // places behind the last token hold a key behind all others
+    const uint32_t k = base + t < n ? token_key<I>(tokens, tokens_ld, base + t, vocab, status) : 0xffffffffu;
+    reinterpret_cast<uint32_t *>(quads)[t] = k;
     __syncthreads();
-    for (int size = 2; size <= SORT_CHUNK; size *= 2)
-        for (int stride = size / 2; stride >= 1; stride /= 2) {
-            const int i = 2 * t - (t & (stride - 1)), j = i + stride;
-            const uint64_t a = v[i], b = v[j];
-            if ((a > b) == ((i & size) == 0)) {
-                v[i] = b;
-                v[j] = a;
-            }
-            // up to a stride of 32 a warp's 32 pairs are the same 64 numbers in the next step
-            if (stride > 32 || (stride == 1 && size >= 64))
-                __syncthreads();
-            else
-                __syncwarp();
-        }
-    for (int i = t; i < SORT_CHUNK; i += SORT_CHUNK / 2)
-        if (base + i < n) {
-            key[base + i] = (uint32_t)(v[i] >> 32);
-            pos[base + i] = (uint32_t)v[i];
-        }
+    const int own = t / 32 * 8;
+    int place = 0;
+#pragma unroll 4
+    for (int q = 0; q < own; q++) {
+        const uint4 x = quads[q];
+        place += (x.x <= k) + (x.y <= k) + (x.z <= k) + (x.w <= k);
+    }
+#pragma unroll
+    for (int q = own; q < own + 8; q++) {
+        const uint4 x = quads[q];
+        place += (x.x < k || (x.x == k && q * 4 < t)) + (x.y < k || (x.y == k && q * 4 + 1 < t)) +
+                 (x.z < k || (x.z == k && q * 4 + 2 < t)) + (x.w < k || (x.w == k && q * 4 + 3 < t));
+    }
+#pragma unroll 4
+    for (int q = own + 8; q < SORT_CHUNK / 4; q++) {
+        const uint4 x = quads[q];
+        place += (x.x < k) + (x.y < k) + (x.z < k) + (x.w < k);
+    }
+    if (base + t < n) {
+        key[base + place] = k;
+        pos[base + place] = (uint32_t)(base + t);
+    }
 }
 
 // Sorted chunks -> sorted tokens: the place of a token is its place within its chunk plus, for every other chunk, how many of
@@ -148,7 +187,11 @@ __global__ void __launch_bounds__(SORT_CHUNK / 2)
 // chunks lie in shared memory, ten steps of a binary search each.
 __global__ void __launch_bounds__(MERGE_THREADS)
     token_merge_kernel(const uint32_t *__restrict__ key, const uint32_t *__restrict__ pos, int n,
-                       uint32_t *__restrict__ key_out, uint32_t *__restrict__ pos_out) {
+                       uint32_t *__restrict__ key_out, uint32_t *__restrict__ pos_out, int ctas, Zeros z) {
+    if ((int)blockIdx.x >= ctas) {
+        write_zeros_any(z, blockIdx.x - ctas, gridDim.x - ctas);
+        return;
+    }
     extern __shared__ uint4 merge_smem[];
     uint32_t *k = reinterpret_cast<uint32_t *>(merge_smem);
     const int quads = n / 4; // the buffers are 16-byte aligned
@@ -325,14 +368,14 @@ __global__ void __launch_bounds__(RADIX_THREADS)
 
 constexpr int SUM_THREADS = 128;
 constexpr int SUM_RUN = 32;   // sorted tokens that one group of threads adds up
-constexpr int SUM_AHEAD = 4;  // gradient rows in flight per thread
-constexpr int FILL_ROWS = 128; // table rows per CTA that are looked at for being untouched
+constexpr int SUM_AHEAD = 8;  // gradient rows in flight per thread
+
+constexpr int SUM_MIN_LOG = 2; // at least four threads share a run
 
 struct SumArgs {
     const uint32_t *key, *pos;
     int64_t n, cols, vocab, grad_ld, res_ld, part_ld;
     int64_t runs;     // ceil(n / SUM_RUN)
-    unsigned sum_x;   // CTAs (in x) that add; those behind them write zeros
     int log_tpr;
 };
 
@@ -340,62 +383,31 @@ struct SumArgs {
 // where the token changes, the sum is finished -- written to the table when all its rows lie in the run, to `part`
 // otherwise: part[run][0] holds the sum of a token that came over from the run before, part[run][1] that of a token that
 // starts in the run and goes on behind it.  Equal amounts of work whatever the tokens' frequencies.
-// The CTAs behind write zeros to the table's untouched rows (not when adding to the table).
 // Bound by memory: every gradient row is read once, every table row written once.
 template <typename T, typename R, int N, bool ADD>
 __global__ void __launch_bounds__(SUM_THREADS)
     embed_sum_kernel(SumArgs a, const T *__restrict__ grad, wide_t<T> scale, R *__restrict__ res,
                      wide_t<T> *__restrict__ part) {
     using W = wide_t<T>;
-    if (blockIdx.x >= a.sum_x) {
-        __shared__ uint32_t hit[FILL_ROWS / 32];
-        const int64_t v0 = (int64_t)(blockIdx.x - a.sum_x) * FILL_ROWS;
-        if (threadIdx.x < FILL_ROWS / 32)
-            hit[threadIdx.x] = 0;
-        __syncthreads();
-        // first sorted token >= v0
-        int64_t lo = 0, hi = a.n;
-        while (lo < hi) {
-            const int64_t mid = (lo + hi) / 2;
-            if ((int64_t)a.key[mid] < v0)
-                lo = mid + 1;
-            else
-                hi = mid;
-        }
-        // the tokens of the block: mark them
-        for (int64_t i = lo + threadIdx.x; i < a.n; i += SUM_THREADS) {
-            const int64_t v = (int64_t)a.key[i] - v0;
-            if (v >= FILL_ROWS)
-                break;
-            if (i == lo || a.key[i] != a.key[i - 1])
-                atomicOr(&hit[v / 32], 1u << (v % 32));
-        }
-        __syncthreads();
-        const int64_t packets = a.cols / N;
-        for (int j = 0; j < FILL_ROWS && v0 + j < a.vocab; j++) {
-            if (hit[j / 32] >> (j % 32) & 1u)
-                continue;
-            R *dst = res + (v0 + j) * a.res_ld;
-            Vec<R, N> z;
-#pragma unroll
-            for (int k = 0; k < N; k++)
-                z.v[k] = narrow<R>(W(0));
-            for (int64_t p = (int64_t)blockIdx.y * SUM_THREADS + threadIdx.x; p < packets;
-                 p += (int64_t)gridDim.y * SUM_THREADS)
-                st_vec<R, N>(dst + p * N, z);
-            if (N > 1 && blockIdx.y == 0)
-                for (int64_t c = packets * N + threadIdx.x; c < a.cols; c += SUM_THREADS)
-                    dst[c] = narrow<R>(W(0));
-        }
-        return;
-    }
+    // the tokens of the CTA's runs, and the one in front and behind: key k of a run stands at keys[1 + k]
+    __shared__ uint32_t keys[(SUM_THREADS >> SUM_MIN_LOG) * SUM_RUN + 2], rows[(SUM_THREADS >> SUM_MIN_LOG) * SUM_RUN];
     const int tpr = 1 << a.log_tpr, tx = threadIdx.x & (tpr - 1), ty = threadIdx.x >> a.log_tpr;
+    const int here = (SUM_THREADS >> a.log_tpr) * SUM_RUN;
+    const int64_t cta_first = (int64_t)blockIdx.x * here;
+    for (int i = threadIdx.x; i < here + 2; i += SUM_THREADS) {
+        const int64_t at = cta_first + i - 1;
+        keys[i] = at >= 0 && at < a.n ? a.key[at] : 0xffffffffu;
+        if (i < here && at + 1 < a.n)
+            rows[i] = a.pos[at + 1];
+    }
+    __syncthreads();
     const int64_t run = (int64_t)blockIdx.x * (SUM_THREADS >> a.log_tpr) + ty;
     if (run >= a.runs)
         return;
-    const int64_t b = run * SUM_RUN, e = b + SUM_RUN < a.n ? b + SUM_RUN : a.n;
-    const uint32_t vocab = (uint32_t)a.vocab;
-    const uint32_t before = b > 0 ? a.key[b - 1] : 0xffffffffu, behind = e < a.n ? a.key[e] : 0xffffffffu;
+    const int64_t b = run * SUM_RUN;
+    const int len = a.n - b < SUM_RUN ? (int)(a.n - b) : SUM_RUN;
+    const uint32_t *key = keys + 1 + ty * SUM_RUN, *row = rows + ty * SUM_RUN;
+    const uint32_t vocab = (uint32_t)a.vocab, before = key[-1], behind = key[len];
     // packets of N columns; the columns behind the last whole packet are a packet of their own with single accesses
     const int64_t packets = (a.cols + N - 1) / N;
     for (int64_t p = (int64_t)blockIdx.y * tpr + tx; p < packets; p += (int64_t)gridDim.y * tpr) {
@@ -405,7 +417,7 @@ __global__ void __launch_bounds__(SUM_THREADS)
 #pragma unroll
         for (int k = 0; k < N; k++)
             acc[k] = W(0);
-        uint32_t cur = a.key[b];
+        uint32_t cur = key[0];
         int slot = cur == before ? 0 : -1; // -1: the sum starts in this run
         auto finish = [&](uint32_t next) {
             if (cur >= vocab)
@@ -433,14 +445,12 @@ __global__ void __launch_bounds__(SUM_THREADS)
                         dst[k] = acc[k];
             }
         };
-        for (int64_t i = b; i < e; i += SUM_AHEAD) {
+        for (int i = 0; i < len; i += SUM_AHEAD) {
             Vec<T, N> x[SUM_AHEAD];
-            uint32_t kk[SUM_AHEAD];
 #pragma unroll
-            for (int u = 0; u < SUM_AHEAD; u++) {
-                kk[u] = i + u < e ? a.key[i + u] : 0xffffffffu;
-                if (kk[u] < vocab) {
-                    const T *src = grad + (int64_t)a.pos[i + u] * a.grad_ld + c;
+            for (int u = 0; u < SUM_AHEAD; u++)
+                if (i + u < len && key[i + u] < vocab) {
+                    const T *src = grad + (int64_t)row[i + u] * a.grad_ld + c;
                     if (width == N)
                         x[u] = ld_vec<T, N>(src);
                     else
@@ -448,14 +458,13 @@ __global__ void __launch_bounds__(SUM_THREADS)
                             if (k < width)
                                 x[u].v[k] = src[k];
                 }
-            }
 #pragma unroll
             for (int u = 0; u < SUM_AHEAD; u++) {
-                if (i + u >= e)
+                if (i + u >= len)
                     break;
-                if (kk[u] != cur) {
-                    finish(kk[u]);
-                    cur = kk[u];
+                if (key[i + u] != cur) {
+                    finish(key[i + u]);
+                    cur = key[i + u];
                     slot = -1;
 #pragma unroll
                     for (int k = 0; k < N; k++)
@@ -488,16 +497,15 @@ __global__ void __launch_bounds__(32 * JOIN_Y)
         const uint32_t v = a.key[e - 1], next = a.key[e], start = a.key[b], before = b > 0 ? a.key[b - 1] : 0xffffffffu;
         if (v >= (uint32_t)a.vocab || next != v || (start == v && before == v))
             continue; // uniform over the CTA: the last token ends here, or started in an earlier run
-        // one past the last row with this token
-        int64_t lo = e + 1, hi = a.n;
-        while (lo < hi) {
-            const int64_t mid = (lo + hi) / 2;
-            if (a.key[mid] == v)
-                lo = mid + 1;
-            else
-                hi = mid;
+        // runs behind this one that hold a part: those that begin with this token
+        int64_t more = 0;
+        for (;;) {
+            const int64_t j = run + 1 + more + tx;
+            const unsigned part_of = __ballot_sync(0xffffffffu, j < a.runs && a.key[j * SUM_RUN] == v);
+            more += part_of == 0xffffffffu ? 32 : __ffs(~part_of) - 1;
+            if (part_of != 0xffffffffu)
+                break;
         }
-        const int64_t more = (lo - 1) / SUM_RUN - run; // runs behind this one that hold a part
         const int64_t share = (more + JOIN_Y) / JOIN_Y;
         const int64_t first = ty * share, last = first + share < more + 1 ? first + share : more + 1;
         for (int64_t c0 = (int64_t)blockIdx.y * 32 * JOIN_N; c0 < a.cols; c0 += (int64_t)gridDim.y * 32 * JOIN_N) {
@@ -565,16 +573,29 @@ GradPlan grad_plan(size_t wide_size, int64_t vocab, int64_t cols, int64_t n) {
 
 template <typename I>
 int embed_sort(const GradPlan &p, const void *tokens, int64_t tokens_ld, int64_t n, int64_t vocab, char *scratch,
-               const uint32_t **key, const uint32_t **pos, int32_t *status, cudaStream_t st) {
+               const uint32_t **key, const uint32_t **pos, int32_t *status, Zeros z, cudaStream_t st) {
     uint32_t *k[2], *q[2];
     for (int i = 0; i < 2; i++) {
         k[i] = reinterpret_cast<uint32_t *>(scratch + p.key_off[i]);
         q[i] = reinterpret_cast<uint32_t *>(scratch + p.pos_off[i]);
     }
+    // CTAs that write zeros: as many as the rows need, at most what fits beside the sorting ones
+    auto zero_ctas = [&](int64_t rows, int per_sm) {
+        const int64_t want = (rows + 3) / 4, cap = (int64_t)sm_count() * per_sm;
+        return (unsigned)(want < cap ? want : cap);
+    };
     if (p.passes == 0) {
-        // two launches, or one: 16384 tokens in 13 us, where counting with 9-bit digits takes six launches
+        // Two launches, or one: 16384 tokens in 11 us, where counting with 9-bit digits takes six launches.  The second
+        // one takes a third of the zeros: its CTAs are fewer on an SM, by their shared memory.
         const int chunks = (int)((n + SORT_CHUNK - 1) / SORT_CHUNK);
-        token_chunk_kernel<I><<<chunks, SORT_CHUNK / 2, 0, st>>>(tokens, tokens_ld, (int)n, vocab, k[0], q[0], status);
+        Zeros z0 = z, z1 = z;
+        if (chunks > 1) {
+            z0.rows = z.rows - z.rows / 3;
+            z1.first = z0.rows;
+            z1.rows = z.rows - z0.rows;
+        }
+        token_chunk_kernel<I><<<chunks + zero_ctas(z0.rows, 3), SORT_CHUNK, 0, st>>>(tokens, tokens_ld, (int)n, vocab, k[0],
+                                                                                  q[0], status, chunks, z0);
         DB2_TRY(after_launch("token_chunk_kernel"));
         *key = k[0];
         *pos = q[0];
@@ -585,12 +606,17 @@ int embed_sort(const GradPlan &p, const void *tokens, int64_t tokens_ld, int64_t
             DB2_CUDA(cudaFuncSetAttribute(token_merge_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, MERGE_MAX * 4));
             once.mark();
         }
-        token_merge_kernel<<<(unsigned)((n + MERGE_TOKENS - 1) / MERGE_TOKENS), MERGE_THREADS, (size_t)(n + 3) / 4 * 16,
-                             st>>>(k[0], q[0], (int)n, k[1], q[1]);
+        const int ctas = (int)((n + MERGE_TOKENS - 1) / MERGE_TOKENS);
+        token_merge_kernel<<<ctas + zero_ctas(z1.rows, 2), MERGE_THREADS, (size_t)(n + 3) / 4 * 16, st>>>(
+            k[0], q[0], (int)n, k[1], q[1], ctas, z1);
         DB2_TRY(after_launch("token_merge_kernel"));
         *key = k[1];
         *pos = q[1];
         return DB2_OK;
+    }
+    if (z.rows > 0) {
+        table_zero_kernel<<<zero_ctas(z.rows, 4), 512, 0, st>>>(z);
+        DB2_TRY(after_launch("table_zero_kernel"));
     }
     uint32_t *counts = reinterpret_cast<uint32_t *>(scratch + p.counts_off);
     RadixIn in{tokens, tokens_ld, vocab, nullptr, nullptr};
@@ -617,15 +643,12 @@ template <typename T, typename R, int N, bool ADD>
 int embed_sum(SumArgs a, const void *grad, double scale, void *res, void *part, cudaStream_t st) {
     const int64_t packets = (a.cols + N - 1) / N;
     a.log_tpr = log2_ceil(packets);
-    if (a.log_tpr > 7)
-        a.log_tpr = 7;
+    a.log_tpr = a.log_tpr > 7 ? 7 : (a.log_tpr < SUM_MIN_LOG ? SUM_MIN_LOG : a.log_tpr);
     const int64_t groups = SUM_THREADS >> a.log_tpr;
     const int64_t gx = (a.runs + groups - 1) / groups;
     int64_t gy = (packets + (1 << a.log_tpr) - 1) >> a.log_tpr;
     gy = gy > 1024 ? 1024 : gy;
-    a.sum_x = (unsigned)gx;
-    const int64_t fill = ADD ? 0 : (a.vocab + FILL_ROWS - 1) / FILL_ROWS;
-    embed_sum_kernel<T, R, N, ADD><<<dim3((unsigned)(gx + fill), (unsigned)gy), SUM_THREADS, 0, st>>>(
+    embed_sum_kernel<T, R, N, ADD><<<dim3((unsigned)gx, (unsigned)gy), SUM_THREADS, 0, st>>>(
         a, static_cast<const T *>(grad), (wide_t<T>)scale, static_cast<R *>(res), static_cast<wide_t<T> *>(part));
     DB2_TRY(after_launch("embed_sum_kernel"));
     if (a.runs > 1) {
@@ -781,10 +804,13 @@ int db2k_embed_grad(int dtype, const void *grad, int64_t grad_ld, int64_t n, int
               "embedGrad: scratch smaller than db2k_embed_grad_scratch_bytes, or not 16-byte aligned");
     SumArgs a{};
     char *s = static_cast<char *>(scratch);
+    const size_t es = dtype_size(res_dtype);
+    Zeros z{static_cast<char *>(res), 0, accumulate ? 0 : vocab, (int64_t)((size_t)cols * es), (int64_t)((size_t)res_ld * es), 0};
+    z.packet = rows_aligned(res, vocab > 1 ? res_ld : 0, es, 16) && z.row_bytes % 16 == 0 ? 16 : (int)es;
     if (index_dtype == DB2_I64)
-        DB2_TRY(embed_sort<int64_t>(p, tokens, tokens_ld, n, vocab, s, &a.key, &a.pos, dev_status, st));
+        DB2_TRY(embed_sort<int64_t>(p, tokens, tokens_ld, n, vocab, s, &a.key, &a.pos, dev_status, z, st));
     else
-        DB2_TRY(embed_sort<int32_t>(p, tokens, tokens_ld, n, vocab, s, &a.key, &a.pos, dev_status, st));
+        DB2_TRY(embed_sort<int32_t>(p, tokens, tokens_ld, n, vocab, s, &a.key, &a.pos, dev_status, z, st));
     a.n = n;
     a.cols = cols;
     a.vocab = vocab;
