@@ -97,7 +97,9 @@ int embed_launch(const void *table, int64_t vocab, int64_t cols, int64_t table_l
 
 constexpr int SORT_CHUNK = 512;            // tokens that a CTA sorts by itself
 constexpr int MERGE_MAX = 80 * SORT_CHUNK; // tokens that are merged in one go: their sorted chunks lie in shared memory
-constexpr int MERGE_THREADS = 512, MERGE_TOKENS = 128; // of a CTA
+constexpr int MERGE_THREADS = 512, MERGE_ROUND = MERGE_THREADS / 8; // of a CTA; tokens that eight lanes each share
+// chunks lie one word apart from multiples of the 32 banks: lanes at the same step of their searches do not collide
+constexpr int MERGE_PITCH = SORT_CHUNK + 1;
 
 // The table's rows [first, first + rows), which become zero before the sums are written: the sorting kernels, which keep
 // few SMs busy, do it with further CTAs.  A CTA writes 128 packets of a row at a time.
@@ -128,7 +130,7 @@ __device__ __forceinline__ void write_zeros_any(const Zeros &z, int cta, int cta
     default: write_zeros<2>(z, cta, ctas); break;
     }
 }
-__global__ void __launch_bounds__(512) table_zero_kernel(Zeros z) { write_zeros_any(z, blockIdx.x, gridDim.x); }
+__global__ void __launch_bounds__(SORT_CHUNK) table_zero_kernel(Zeros z) { write_zeros_any(z, blockIdx.x, gridDim.x); }
 
 template <typename I>
 __device__ __forceinline__ uint32_t token_key(const void *tokens, int64_t ld, int64_t i, int64_t vocab,
@@ -183,37 +185,29 @@ __global__ void __launch_bounds__(SORT_CHUNK)
 }
 
 // Sorted chunks -> sorted tokens: the place of a token is its place within its chunk plus, for every other chunk, how many of
-// its keys are smaller (or the same, in chunks in front).  A warp takes a token, a lane every 32nd chunk; the keys of all
-// chunks lie in shared memory, ten steps of a binary search each.
+// its keys are smaller (or the same, in chunks in front).  8 to 32 lanes share a token, each takes every so many chunks; the
+// keys of all chunks lie in shared memory, ten steps of a binary search each.
 __global__ void __launch_bounds__(MERGE_THREADS)
     token_merge_kernel(const uint32_t *__restrict__ key, const uint32_t *__restrict__ pos, int n,
-                       uint32_t *__restrict__ key_out, uint32_t *__restrict__ pos_out, int ctas, Zeros z) {
-    if ((int)blockIdx.x >= ctas) {
-        write_zeros_any(z, blockIdx.x - ctas, gridDim.x - ctas);
-        return;
-    }
-    extern __shared__ uint4 merge_smem[];
-    uint32_t *k = reinterpret_cast<uint32_t *>(merge_smem);
-    const int quads = n / 4; // the buffers are 16-byte aligned
+                       uint32_t *__restrict__ key_out, uint32_t *__restrict__ pos_out, int per_cta) {
+    extern __shared__ uint32_t k[];
 #pragma unroll 8
-    for (int i = threadIdx.x; i < quads; i += MERGE_THREADS)
-        merge_smem[i] = reinterpret_cast<const uint4 *>(key)[i];
-    for (int i = quads * 4 + threadIdx.x; i < n; i += MERGE_THREADS)
-        k[i] = key[i];
+    for (int i = threadIdx.x; i < n; i += MERGE_THREADS)
+        k[i / SORT_CHUNK * MERGE_PITCH + i % SORT_CHUNK] = key[i];
     __syncthreads();
     const int lane = threadIdx.x % 32, chunks = (n + SORT_CHUNK - 1) / SORT_CHUNK;
     const int group = chunks <= 8 ? 8 : (chunks <= 16 ? 16 : 32); // lanes that share a token
-    const int first = blockIdx.x * MERGE_TOKENS, part = lane % group;
-    for (int i = first + threadIdx.x / group; i < first + MERGE_TOKENS; i += MERGE_THREADS / group) {
+    const int first = blockIdx.x * per_cta, part = lane % group;
+    for (int i = first + threadIdx.x / group; i < first + per_cta; i += MERGE_THREADS / group) {
         const int at = i < n ? i : n - 1, own = at / SORT_CHUNK; // all lanes stay for the sum
-        const uint32_t mine = k[at];
+        const uint32_t mine = k[own * MERGE_PITCH + at % SORT_CHUNK], its_pos = pos[at];
         int place = 0;
         for (int c = part; c < chunks; c += group) {
             if (c == own) {
                 place += at - own * SORT_CHUNK;
                 continue;
             }
-            const uint32_t *chunk = k + c * SORT_CHUNK;
+            const uint32_t *chunk = k + c * MERGE_PITCH;
             const int len = n - c * SORT_CHUNK < SORT_CHUNK ? n - c * SORT_CHUNK : SORT_CHUNK;
             const uint32_t below = mine + (c < own); // keys are smaller than 2^32 - 1
             int lo = 0;
@@ -227,7 +221,7 @@ __global__ void __launch_bounds__(MERGE_THREADS)
             place += __shfl_xor_sync(0xffffffffu, place, o);
         if (part == 0 && i < n) {
             key_out[place] = mine;
-            pos_out[place] = pos[at];
+            pos_out[place] = its_pos;
         }
     }
 }
@@ -408,11 +402,9 @@ __global__ void __launch_bounds__(SUM_THREADS)
     const int len = a.n - b < SUM_RUN ? (int)(a.n - b) : SUM_RUN;
     const uint32_t *key = keys + 1 + ty * SUM_RUN, *row = rows + ty * SUM_RUN;
     const uint32_t vocab = (uint32_t)a.vocab, before = key[-1], behind = key[len];
-    // packets of N columns; the columns behind the last whole packet are a packet of their own with single accesses
-    const int64_t packets = (a.cols + N - 1) / N;
+    const int64_t packets = a.cols / N; // cols is a multiple of N
     for (int64_t p = (int64_t)blockIdx.y * tpr + tx; p < packets; p += (int64_t)gridDim.y * tpr) {
         const int64_t c = p * N;
-        const int width = a.cols - c < N ? (int)(a.cols - c) : N;
         W acc[N];
 #pragma unroll
         for (int k = 0; k < N; k++)
@@ -424,40 +416,31 @@ __global__ void __launch_bounds__(SUM_THREADS)
                 return;
             if (slot < 0 && next != cur) {
                 R *dst = res + (int64_t)cur * a.res_ld + c;
-                if (width == N) {
-                    Vec<R, N> y;
-                    if constexpr (ADD)
-                        y = ld_vec<R, N>(dst);
+                W y[N];
+#pragma unroll
+                for (int k = 0; k < N; k++)
+                    y[k] = acc[k] * scale;
+                if constexpr (ADD) {
+                    const Vec<R, N> old = ld_vec<R, N>(dst);
 #pragma unroll
                     for (int k = 0; k < N; k++)
-                        y.v[k] = narrow<R>(ADD ? W(widen(y.v[k])) + acc[k] * scale : acc[k] * scale);
-                    st_vec<R, N>(dst, y);
-                } else {
-                    for (int k = 0; k < N; k++)
-                        if (k < width)
-                            dst[k] = narrow<R>(ADD ? W(widen(dst[k])) + acc[k] * scale : acc[k] * scale);
+                        y[k] += W(widen(old.v[k]));
                 }
+                st_vec<R, N>(dst, narrow_all<R, N>(y));
             } else {
                 W *dst = part + (run * 2 + (slot < 0 ? 1 : 0)) * a.part_ld + c;
 #pragma unroll
                 for (int k = 0; k < N; k++)
-                    if (k < width)
-                        dst[k] = acc[k];
+                    dst[k] = acc[k];
             }
         };
         for (int i = 0; i < len; i += SUM_AHEAD) {
             Vec<T, N> x[SUM_AHEAD];
 #pragma unroll
-            for (int u = 0; u < SUM_AHEAD; u++)
-                if (i + u < len && key[i + u] < vocab) {
-                    const T *src = grad + (int64_t)row[i + u] * a.grad_ld + c;
-                    if (width == N)
-                        x[u] = ld_vec<T, N>(src);
-                    else
-                        for (int k = 0; k < N; k++)
-                            if (k < width)
-                                x[u].v[k] = src[k];
-                }
+            for (int u = 0; u < SUM_AHEAD; u++) { // places without a row load row 0: loads under conditions go one by one
+                const int64_t r = i + u < len && key[i + u] < vocab ? row[i + u] : 0;
+                x[u] = ld_vec<T, N>(grad + r * a.grad_ld + c);
+            }
 #pragma unroll
             for (int u = 0; u < SUM_AHEAD; u++) {
                 if (i + u >= len)
@@ -473,8 +456,7 @@ __global__ void __launch_bounds__(SUM_THREADS)
                 if (cur < vocab) {
 #pragma unroll
                     for (int k = 0; k < N; k++)
-                        if (k < width)
-                            acc[k] += widen(x[u].v[k]);
+                        acc[k] += widen(x[u].v[k]);
                 }
             }
         }
@@ -579,23 +561,14 @@ int embed_sort(const GradPlan &p, const void *tokens, int64_t tokens_ld, int64_t
         k[i] = reinterpret_cast<uint32_t *>(scratch + p.key_off[i]);
         q[i] = reinterpret_cast<uint32_t *>(scratch + p.pos_off[i]);
     }
-    // CTAs that write zeros: as many as the rows need, at most what fits beside the sorting ones
-    auto zero_ctas = [&](int64_t rows, int per_sm) {
-        const int64_t want = (rows + 3) / 4, cap = (int64_t)sm_count() * per_sm;
-        return (unsigned)(want < cap ? want : cap);
-    };
+    // CTAs that write zeros: as many as the rows need, at most what fits on the device
+    const int64_t want = (z.rows + 3) / 4, cap = (int64_t)sm_count() * 4;
+    const unsigned zero_ctas = (unsigned)(want < cap ? want : cap);
     if (p.passes == 0) {
-        // Two launches, or one: 16384 tokens in 11 us, where counting with 9-bit digits takes six launches.  The second
-        // one takes a third of the zeros: its CTAs are fewer on an SM, by their shared memory.
+        // two launches, or one, where counting with 9-bit digits takes six
         const int chunks = (int)((n + SORT_CHUNK - 1) / SORT_CHUNK);
-        Zeros z0 = z, z1 = z;
-        if (chunks > 1) {
-            z0.rows = z.rows - z.rows / 3;
-            z1.first = z0.rows;
-            z1.rows = z.rows - z0.rows;
-        }
-        token_chunk_kernel<I><<<chunks + zero_ctas(z0.rows, 3), SORT_CHUNK, 0, st>>>(tokens, tokens_ld, (int)n, vocab, k[0],
-                                                                                  q[0], status, chunks, z0);
+        token_chunk_kernel<I><<<chunks + zero_ctas, SORT_CHUNK, 0, st>>>(tokens, tokens_ld, (int)n, vocab, k[0], q[0],
+                                                                         status, chunks, z);
         DB2_TRY(after_launch("token_chunk_kernel"));
         *key = k[0];
         *pos = q[0];
@@ -603,19 +576,21 @@ int embed_sort(const GradPlan &p, const void *tokens, int64_t tokens_ld, int64_t
             return DB2_OK;
         static PerDeviceOnce once;
         if (once.need()) {
-            DB2_CUDA(cudaFuncSetAttribute(token_merge_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, MERGE_MAX * 4));
+            DB2_CUDA(cudaFuncSetAttribute(token_merge_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                          MERGE_MAX / SORT_CHUNK * MERGE_PITCH * 4));
             once.mark();
         }
-        const int ctas = (int)((n + MERGE_TOKENS - 1) / MERGE_TOKENS);
-        token_merge_kernel<<<ctas + zero_ctas(z1.rows, 2), MERGE_THREADS, (size_t)(n + 3) / 4 * 16, st>>>(
-            k[0], q[0], (int)n, k[1], q[1], ctas, z1);
+        // every CTA reads all keys: no more CTAs than SMs, of whole rounds of MERGE_ROUND tokens
+        const int per_cta = (int)((n + sm_count() * MERGE_ROUND - 1) / (sm_count() * MERGE_ROUND)) * MERGE_ROUND;
+        token_merge_kernel<<<(unsigned)((n + per_cta - 1) / per_cta), MERGE_THREADS, (size_t)chunks * MERGE_PITCH * 4, st>>>(
+            k[0], q[0], (int)n, k[1], q[1], per_cta);
         DB2_TRY(after_launch("token_merge_kernel"));
         *key = k[1];
         *pos = q[1];
         return DB2_OK;
     }
     if (z.rows > 0) {
-        table_zero_kernel<<<zero_ctas(z.rows, 4), 512, 0, st>>>(z);
+        table_zero_kernel<<<zero_ctas, SORT_CHUNK, 0, st>>>(z);
         DB2_TRY(after_launch("table_zero_kernel"));
     }
     uint32_t *counts = reinterpret_cast<uint32_t *>(scratch + p.counts_off);
@@ -641,7 +616,7 @@ int embed_sort(const GradPlan &p, const void *tokens, int64_t tokens_ld, int64_t
 
 template <typename T, typename R, int N, bool ADD>
 int embed_sum(SumArgs a, const void *grad, double scale, void *res, void *part, cudaStream_t st) {
-    const int64_t packets = (a.cols + N - 1) / N;
+    const int64_t packets = a.cols / N;
     a.log_tpr = log2_ceil(packets);
     a.log_tpr = a.log_tpr > 7 ? 7 : (a.log_tpr < SUM_MIN_LOG ? SUM_MIN_LOG : a.log_tpr);
     const int64_t groups = SUM_THREADS >> a.log_tpr;
@@ -667,7 +642,7 @@ template <typename T, typename R>
 int embed_sum_any(const SumArgs &a, const void *grad, double scale, void *res, void *part, int accumulate,
                   cudaStream_t st) {
     constexpr int N = 16 / (sizeof(T) > sizeof(R) ? sizeof(T) : sizeof(R)); // both sides' packets are at most 16 bytes
-    const bool wide = rows_aligned(grad, a.grad_ld, sizeof(T), N * sizeof(T)) &&
+    const bool wide = a.cols % N == 0 && rows_aligned(grad, a.grad_ld, sizeof(T), N * sizeof(T)) &&
                       rows_aligned(res, a.res_ld, sizeof(R), N * sizeof(R));
     if (wide)
         return accumulate ? embed_sum<T, R, N, true>(a, grad, scale, res, part, st)
