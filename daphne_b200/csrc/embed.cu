@@ -101,12 +101,14 @@ constexpr int MERGE_THREADS = 512, MERGE_ROUND = MERGE_THREADS / 8; // of a CTA;
 // chunks lie one word apart from multiples of the 32 banks: lanes at the same step of their searches do not collide
 constexpr int MERGE_PITCH = SORT_CHUNK + 1;
 
-// The table's rows [first, first + rows), which become zero before the sums are written: the sorting kernels, which keep
+// The table's rows, which become zero before the sums are written: the sorting kernels, which keep
 // few SMs busy, do it with further CTAs.  A CTA writes 128 packets of a row at a time.
 struct Zeros {
     char *at;
-    int64_t first, rows, row_bytes, ld_bytes;
-    int packet; // 16, or the size of an element
+    int64_t rows, row_bytes, ld_bytes;
+    int packet;     // 16, or the size of an element
+    int64_t tail;   // bytes behind the last row, a multiple of the element's size
+    int element;
 };
 template <int BYTES> struct alignas(BYTES) Blank {
     unsigned char b[BYTES];
@@ -116,13 +118,23 @@ template <int BYTES> __device__ __forceinline__ void write_zeros(const Zeros &z,
     const int64_t packets = z.row_bytes / BYTES;
     const Blank<BYTES> zero{};
     for (int64_t r = (int64_t)cta * groups + threadIdx.x / 128; r < z.rows; r += (int64_t)ctas * groups) {
-        char *row = z.at + (z.first + r) * z.ld_bytes;
+        char *row = z.at + r * z.ld_bytes;
 #pragma unroll 4
         for (int64_t p = tx; p < packets; p += 128)
             *reinterpret_cast<Blank<BYTES> *>(row + p * BYTES) = zero;
     }
 }
 __device__ __forceinline__ void write_zeros_any(const Zeros &z, int cta, int ctas) {
+    if (cta == 0 && z.tail > 0) {
+        char *p = z.at + z.rows * z.ld_bytes;
+        for (int64_t i = (int64_t)threadIdx.x * z.element; i < z.tail; i += (int64_t)blockDim.x * z.element)
+            if (z.element == 2)
+                *reinterpret_cast<uint16_t *>(p + i) = 0;
+            else if (z.element == 4)
+                *reinterpret_cast<uint32_t *>(p + i) = 0;
+            else
+                *reinterpret_cast<uint64_t *>(p + i) = 0;
+    }
     switch (z.packet) {
     case 16: write_zeros<16>(z, cta, ctas); break;
     case 8: write_zeros<8>(z, cta, ctas); break;
@@ -562,7 +574,7 @@ int embed_sort(const GradPlan &p, const void *tokens, int64_t tokens_ld, int64_t
         q[i] = reinterpret_cast<uint32_t *>(scratch + p.pos_off[i]);
     }
     // CTAs that write zeros: as many as the rows need, at most what fits on the device
-    const int64_t want = (z.rows + 3) / 4, cap = (int64_t)sm_count() * 4;
+    const int64_t want = (z.rows + (z.tail > 0) + 3) / 4, cap = (int64_t)sm_count() * 4;
     const unsigned zero_ctas = (unsigned)(want < cap ? want : cap);
     if (p.passes == 0) {
         // two launches, or one, where counting with 9-bit digits takes six
@@ -589,7 +601,7 @@ int embed_sort(const GradPlan &p, const void *tokens, int64_t tokens_ld, int64_t
         *pos = q[1];
         return DB2_OK;
     }
-    if (z.rows > 0) {
+    if (zero_ctas > 0) {
         table_zero_kernel<<<zero_ctas, SORT_CHUNK, 0, st>>>(z);
         DB2_TRY(after_launch("table_zero_kernel"));
     }
@@ -780,8 +792,15 @@ int db2k_embed_grad(int dtype, const void *grad, int64_t grad_ld, int64_t n, int
     SumArgs a{};
     char *s = static_cast<char *>(scratch);
     const size_t es = dtype_size(res_dtype);
-    Zeros z{static_cast<char *>(res), 0, accumulate ? 0 : vocab, (int64_t)((size_t)cols * es), (int64_t)((size_t)res_ld * es), 0};
-    z.packet = rows_aligned(res, vocab > 1 ? res_ld : 0, es, 16) && z.row_bytes % 16 == 0 ? 16 : (int)es;
+    Zeros z{static_cast<char *>(res), accumulate ? 0 : vocab, (int64_t)((size_t)cols * es), (int64_t)((size_t)res_ld * es), 0,
+            0, (int)es};
+    if (!accumulate && (res_ld == cols || vocab == 1) && aligned16(res)) { // one run of bytes: rows of 8 KB, and the rest
+        const int64_t all = vocab * z.row_bytes;
+        z.row_bytes = z.ld_bytes = 8192;
+        z.rows = all / 8192;
+        z.tail = all % 8192;
+    }
+    z.packet = rows_aligned(res, z.rows > 1 ? z.ld_bytes : 0, 1, 16) && z.row_bytes % 16 == 0 ? 16 : (int)es;
     if (index_dtype == DB2_I64)
         DB2_TRY(embed_sort<int64_t>(p, tokens, tokens_ld, n, vocab, s, &a.key, &a.pos, dev_status, z, st));
     else
