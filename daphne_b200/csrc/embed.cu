@@ -654,11 +654,17 @@ template <typename T, typename R>
 int embed_sum_any(const SumArgs &a, const void *grad, double scale, void *res, void *part, int accumulate,
                   cudaStream_t st) {
     constexpr int N = 16 / (sizeof(T) > sizeof(R) ? sizeof(T) : sizeof(R)); // both sides' packets are at most 16 bytes
-    const bool wide = a.cols % N == 0 && rows_aligned(grad, a.grad_ld, sizeof(T), N * sizeof(T)) &&
-                      rows_aligned(res, a.res_ld, sizeof(R), N * sizeof(R));
-    if (wide)
+    auto packed = [&](int n) {
+        return a.cols % n == 0 && rows_aligned(grad, a.grad_ld, sizeof(T), n * sizeof(T)) &&
+               rows_aligned(res, a.res_ld, sizeof(R), n * sizeof(R));
+    };
+    if (packed(N))
         return accumulate ? embed_sum<T, R, N, true>(a, grad, scale, res, part, st)
                           : embed_sum<T, R, N, false>(a, grad, scale, res, part, st);
+    if constexpr (N > 2)
+        if (packed(2)) // pairs
+            return accumulate ? embed_sum<T, R, 2, true>(a, grad, scale, res, part, st)
+                              : embed_sum<T, R, 2, false>(a, grad, scale, res, part, st);
     return accumulate ? embed_sum<T, R, 1, true>(a, grad, scale, res, part, st)
                       : embed_sum<T, R, 1, false>(a, grad, scale, res, part, st);
 }
@@ -747,6 +753,12 @@ int db2k_embed(int dtype, const void *table, int64_t vocab, int64_t cols, int64_
             if (index_dtype == DB2_I64)
                 DB2_EMBED(N, int64_t);
             DB2_EMBED(N, int32_t);
+        }
+        if (N > 2 && rows_aligned(table, table_ld, sizeof(T), 2 * sizeof(T)) && // pairs
+            rows_aligned(res, res_ld, sizeof(T), 2 * sizeof(T))) {
+            if (index_dtype == DB2_I64)
+                DB2_EMBED(2, int64_t);
+            DB2_EMBED(2, int32_t);
         }
         if (index_dtype == DB2_I64)
             DB2_EMBED(1, int64_t);

@@ -361,20 +361,23 @@ __global__ void __launch_bounds__(256)
 // there.  (128 CTAs of eight warps reach 70 % of the memory's rate, the two passes 53 %.)
 struct ScanPlan {
     int blocks, warps;
-    bool packed; // lanes take 8 bytes
+    int vec; // columns that a lane takes
 };
-template <typename T> ScanPlan scan_plan(int64_t rows, int64_t cols, int64_t seqs, bool aligned) {
-    ScanPlan p{1, 4, aligned};
+// `vec`: the most that shapes and addresses allow.  The number of blocks does not depend on it: the scratch is asked for
+// without pointers.
+template <typename T> ScanPlan scan_plan(int64_t rows, int64_t cols, int64_t seqs, int vec) {
+    ScanPlan p{1, 4, vec};
     const int64_t sms = sm_count();
-    auto strips = [&](int64_t vec) { return (cols + 32 * vec - 1) / (32 * vec); };
-    int64_t ctas = strips(widest<T>()) * seqs; // of whole lanes, aligned or not: the scratch is asked for without pointers
-    if (ctas * 3 >= sms * 2 || rows / seqs < 1024) {
-        p.warps = (aligned ? ctas : strips(1) * seqs) <= sms ? 8 : 4;
+    auto ctas = [&](int64_t v) { return (cols + 32 * v - 1) / (32 * v) * seqs; };
+    const int64_t fewest = ctas(widest<T>());
+    if (fewest * 3 >= sms * 2 || rows / seqs < 1024) {
+        p.warps = ctas(vec) <= sms ? 8 : 4;
         return p;
     }
     // a narrow matrix leaves lanes of its last strip without columns: single elements waste fewer
-    p.packed = aligned && cols % (32 * widest<T>()) == 0;
-    const int64_t want = sms * 3 / ctas, most = rows / seqs / 256;
+    if (cols % (32 * vec) != 0)
+        p.vec = 1;
+    const int64_t want = sms * 3 / fewest, most = rows / seqs / 256;
     p.blocks = (int)(want < most ? want : most);
     return p;
 }
@@ -402,17 +405,22 @@ template <typename T, int VEC, int WARPS, bool BACK, bool SIGMOID> int scan_laun
     return after_launch("gated_scan_kernel");
 }
 
-template <typename T, bool BACK> int scan_any(ScanArgs<T> &a, int gate, bool aligned, cudaStream_t st) {
+template <typename T, bool BACK> int scan_any(ScanArgs<T> &a, int gate, int vec, cudaStream_t st) {
     constexpr int N = widest<T>();
-    const ScanPlan p = scan_plan<T>(a.rows, a.cols, a.seqs, aligned);
+    const ScanPlan p = scan_plan<T>(a.rows, a.cols, a.seqs, vec);
     a.blocks = p.blocks;
     const bool s = gate == DB2_GATE_SIGMOID;
 #define DB2_SCAN(VEC, WARPS)                                                                                           \
     return s ? scan_launch<T, VEC, WARPS, BACK, true>(a, st) : scan_launch<T, VEC, WARPS, BACK, false>(a, st)
-    if (p.packed) {
+    if (p.vec == N) {
         if (p.warps == 8)
             DB2_SCAN(N, 8);
         DB2_SCAN(N, 4);
+    }
+    if (N > 2 && p.vec == 2) {
+        if (p.warps == 8)
+            DB2_SCAN(2, 8);
+        DB2_SCAN(2, 4);
     }
     if (p.warps == 8)
         DB2_SCAN(1, 8);
@@ -493,9 +501,9 @@ size_t db2k_gated_scan_scratch_bytes(int dtype, int64_t rows, int64_t cols, int6
     if (rows <= 0 || cols <= 0 || seqs <= 0)
         return 0;
     const int es = (int)dtype_size(dtype);
-    const int blocks = (es == 8   ? scan_plan<double>(rows, cols, seqs, true)
-                        : es == 4 ? scan_plan<float>(rows, cols, seqs, true)
-                                  : scan_plan<__half>(rows, cols, seqs, true))
+    const int blocks = (es == 8   ? scan_plan<double>(rows, cols, seqs, 1)
+                        : es == 4 ? scan_plan<float>(rows, cols, seqs, 1)
+                                  : scan_plan<__half>(rows, cols, seqs, 1))
                            .blocks;
     return blocks < 2 ? 0 : (size_t)seqs * blocks * 2 * scan_part_ld(cols) * (dtype == DB2_F64 ? 8 : 4);
 }
@@ -532,10 +540,13 @@ int db2k_gated_scan(int dtype, int gate, const void *g, int64_t g_ld, const void
         a.rows = rows;
         a.cols = cols;
         a.seqs = seqs;
-        constexpr size_t al = sizeof(T) * widest<T>();
-        const bool packed = cols % widest<T>() == 0 && rows_aligned(g, g_ld, sizeof(T), al) &&
-                            rows_aligned(x, x_ld, sizeof(T), al) && rows_aligned(h, h_ld, sizeof(T), al);
-        return scan_any<T, false>(a, gate, packed, as_stream(stream));
+        auto packed = [&](int n) {
+            const size_t b = n * sizeof(T);
+            return cols % n == 0 && rows_aligned(g, g_ld, sizeof(T), b) && rows_aligned(x, x_ld, sizeof(T), b) &&
+                   rows_aligned(h, h_ld, sizeof(T), b);
+        };
+        const int vec = packed(widest<T>()) ? widest<T>() : (widest<T>() > 2 && packed(2) ? 2 : 1);
+        return scan_any<T, false>(a, gate, vec, as_stream(stream));
     });
     return DB2_OK;
 }
@@ -585,12 +596,14 @@ int db2k_gated_scan_grad(int dtype, int gate, const void *g, int64_t g_ld, const
         a.rows = rows;
         a.cols = cols;
         a.seqs = seqs;
-        constexpr size_t al = sizeof(T) * widest<T>();
-        const bool packed = cols % widest<T>() == 0 && rows_aligned(g, g_ld, sizeof(T), al) &&
-                            (!sigmoid || rows_aligned(x, x_ld, sizeof(T), al)) && rows_aligned(h, h_ld, sizeof(T), al) &&
-                            rows_aligned(grad, grad_ld, sizeof(T), al) && rows_aligned(dg, dg_ld, sizeof(T), al) &&
-                            rows_aligned(dx, dx_ld, sizeof(T), al);
-        return scan_any<T, true>(a, gate, packed, as_stream(stream));
+        auto packed = [&](int n) {
+            const size_t b = n * sizeof(T);
+            return cols % n == 0 && rows_aligned(g, g_ld, sizeof(T), b) && (!sigmoid || rows_aligned(x, x_ld, sizeof(T), b)) &&
+                   rows_aligned(h, h_ld, sizeof(T), b) && rows_aligned(grad, grad_ld, sizeof(T), b) &&
+                   rows_aligned(dg, dg_ld, sizeof(T), b) && rows_aligned(dx, dx_ld, sizeof(T), b);
+        };
+        const int vec = packed(widest<T>()) ? widest<T>() : (widest<T>() > 2 && packed(2) ? 2 : 1);
+        return scan_any<T, true>(a, gate, vec, as_stream(stream));
     });
     return DB2_OK;
 }

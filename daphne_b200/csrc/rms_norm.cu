@@ -568,13 +568,13 @@ RowPlan row_plan(int64_t packets, int64_t rows, int first, int most, int step, i
     p.block = p.fits ? p.tpr * (p.tpr < 256 ? 256 / p.tpr : 1) : 0;
     return p;
 }
-// packets a thread that there are kernels for: 1 to 3 (gradient: 4), or 4 and 8 single elements
+// packets a thread that there are kernels for: 1 to 3 (gradient: 4), or 4 and 8 smaller ones
 template <typename T, int N> RowPlan row_plan(int64_t cols, int64_t rows, bool back) {
     const int place = NORM_STAGES * (back ? 3 : 2) * N * (int)sizeof(T);
-    return N == 1 ? row_plan(cols, rows, 4, 8, 4, place) : row_plan(cols / N, rows, 1, back ? 4 : 3, 1, place);
+    return N <= 2 && sizeof(T) * N < 16 ? row_plan(cols / N, rows, 4, 8, 4, place) : row_plan(cols / N, rows, 1, back ? 4 : 3, 1, place);
 }
 #define DB2_BY_PACKETS(N, BACK, ppt, LAUNCH)                                                                                 \
-    if constexpr (N == 1) {                                                                                            \
+    if constexpr (N * sizeof(T) < 16) {                                                                                \
         if (ppt == 4) {                                                                                                \
             LAUNCH(4)                                                                                                  \
         } else {                                                                                                       \
@@ -772,10 +772,16 @@ int db2k_rms_norm(int dtype, const void *x, int64_t rows, int64_t cols, int64_t 
         NormArgs<T> a{static_cast<const T *>(x), static_cast<const T *>(residual), static_cast<const T *>(weight),
                       static_cast<T *>(sum), res, nullptr, static_cast<wide_t<T> *>(rstd), rows, cols, x_ld,
                       residual_ld, sum_ld, res_ld, 0, 0, 0, (wide_t<T>)eps};
-        const bool packed = cols % N == 0 && rows_aligned(x, x_ld, sizeof(T), 16) && rows_aligned(residual, residual_ld, sizeof(T), 16) &&
-                            rows_aligned(weight, 0, sizeof(T), 16) && rows_aligned(sum, sum_ld, sizeof(T), 16) &&
-                            rows_aligned(res, res_ld, sizeof(T), 16);
-        return packed ? norm_launch<T, N, false>(a, as_stream(stream)) : norm_launch<T, 1, false>(a, as_stream(stream));
+        auto packed = [&](int n) {
+            const size_t b = n * sizeof(T);
+            return cols % n == 0 && rows_aligned(x, x_ld, sizeof(T), b) && rows_aligned(residual, residual_ld, sizeof(T), b) &&
+                   rows_aligned(weight, 0, sizeof(T), b) && rows_aligned(sum, sum_ld, sizeof(T), b) &&
+                   rows_aligned(res, res_ld, sizeof(T), b);
+        };
+        if (packed(N))
+            return norm_launch<T, N, false>(a, as_stream(stream));
+        return N > 2 && packed(2) ? norm_launch<T, 2, false>(a, as_stream(stream))
+                                  : norm_launch<T, 1, false>(a, as_stream(stream));
     });
     return DB2_OK;
 }
@@ -800,10 +806,15 @@ int db2k_rms_norm_q8(int dtype, const void *x, int64_t rows, int64_t cols, int64
         NormArgs<T> a{static_cast<const T *>(x), static_cast<const T *>(residual), static_cast<const T *>(weight),
                       static_cast<T *>(sum), res, static_cast<float *>(scales), static_cast<float *>(rstd), rows, cols,
                       x_ld, residual_ld, sum_ld, res_ld, scales_ld, group, groups, (float)eps};
-        const bool packed = cols % N == 0 && rows_aligned(x, x_ld, sizeof(T), 16) && rows_aligned(residual, residual_ld, sizeof(T), 16) &&
-                            rows_aligned(weight, 0, sizeof(T), 16) && rows_aligned(sum, sum_ld, sizeof(T), 16) &&
-                            rows_aligned(res, res_ld, 1, N);
-        return packed ? norm_launch<T, N, true>(a, as_stream(stream)) : norm_launch<T, 1, true>(a, as_stream(stream));
+        auto packed = [&](int n) {
+            const size_t b = n * sizeof(T);
+            return cols % n == 0 && rows_aligned(x, x_ld, sizeof(T), b) && rows_aligned(residual, residual_ld, sizeof(T), b) &&
+                   rows_aligned(weight, 0, sizeof(T), b) && rows_aligned(sum, sum_ld, sizeof(T), b) &&
+                   rows_aligned(res, res_ld, 1, n);
+        };
+        if (packed(N))
+            return norm_launch<T, N, true>(a, as_stream(stream));
+        return packed(2) ? norm_launch<T, 2, true>(a, as_stream(stream)) : norm_launch<T, 1, true>(a, as_stream(stream));
     };
     return dtype == DB2_F32 ? go(float()) : dtype == DB2_F16 ? go(__half()) : go(__nv_bfloat16());
 }
@@ -839,11 +850,17 @@ int db2k_rms_norm_grad(int dtype, const void *grad, int64_t grad_ld, int64_t row
                           static_cast<const T *>(dsum), static_cast<const wide_t<T> *>(rstd), static_cast<T *>(dx),
                           dweight ? static_cast<wide_t<T> *>(scratch) : nullptr, rows, cols, grad_ld, sum_ld, dsum_ld,
                           dx_ld, part_ld_of(cols)};
-        const bool packed = cols % N == 0 && rows_aligned(grad, grad_ld, sizeof(T), 16) && rows_aligned(sum, sum_ld, sizeof(T), 16) &&
-                            rows_aligned(weight, 0, sizeof(T), 16) && rows_aligned(dsum, dsum_ld, sizeof(T), 16) &&
-                            rows_aligned(dx, dx_ld, sizeof(T), 16);
+        auto packed = [&](int n) {
+            const size_t b = n * sizeof(T);
+            return cols % n == 0 && rows_aligned(grad, grad_ld, sizeof(T), b) && rows_aligned(sum, sum_ld, sizeof(T), b) &&
+                   rows_aligned(weight, 0, sizeof(T), b) && rows_aligned(dsum, dsum_ld, sizeof(T), b) &&
+                   rows_aligned(dx, dx_ld, sizeof(T), b);
+        };
         wide_t<T> *dw = static_cast<wide_t<T> *>(dweight);
-        return packed ? norm_grad_launch<T, N>(a, dw, as_stream(stream)) : norm_grad_launch<T, 1>(a, dw, as_stream(stream));
+        if (packed(N))
+            return norm_grad_launch<T, N>(a, dw, as_stream(stream));
+        return N > 2 && packed(2) ? norm_grad_launch<T, 2>(a, dw, as_stream(stream))
+                                  : norm_grad_launch<T, 1>(a, dw, as_stream(stream));
     });
     return DB2_OK;
 }

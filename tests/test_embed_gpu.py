@@ -52,6 +52,8 @@ def _lookup(tname, table, tok, scale, index="i64", tok_ld=1, pad=0, shift=0, sta
     (64, 4100, 9, 4, 8, "i64", 1, "uniform"),        # few rows, cut along the columns
     (9, 20000, 2, 0, 0, "i64", 1, "uniform"),
     (17, 24, 40001, 8, 16, "i32", 1, "skewed"),
+    (77, 130, 300, 0, 0, "i64", 1, "outside"),       # pairs
+    (20, 1030, 40, 2, 2, "i64", 1, "uniform"),
 ])
 def test_lookup(tname, vocab, cols, n, pad, shift, index, tok_ld, kind):
     rng = np.random.default_rng(vocab + cols + n)
@@ -123,6 +125,10 @@ def _expect(G, tok, vocab, scale):
     (300000, 8, 45001, 0, 0, "i64", "skewed"),       # three passes
     (400, 9, 50000, 1, 0, "i32", "skewed"),          # one pass
     (3, 4, 40000, 0, 0, "i64", "one"),
+    (50, 130, 2000, 0, 0, "i64", "skewed"),          # pairs
+    (50, 258, 900, 2, 2, "i64", "outside"),
+    (1000, 33, 700, 0, 1, "i64", "skewed"),          # a contiguous table off 16-byte boundaries
+    (1000, 33, 700, 0, 0, "i64", "skewed"),          # and on one, with bytes behind the last whole packet
     (3, 4, 30000, 0, 0, "i64", "one"),
 ])
 def test_gradient(tname, res_t, vocab, cols, n, pad, shift, index, kind):

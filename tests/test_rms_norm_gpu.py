@@ -22,6 +22,7 @@ SHAPES = [  # rows, cols, pad, shift
     (1000, 512, 0, 0), (9, 4096, 0, 0), (300, 4100, 4, 8), (4, 9001, 0, 0), (160, 8200, 0, 8), (2, 16500, 12, 0),
     (3, 40000, 0, 0), (150, 33000, 0, 8), (40003, 8, 0, 0),
     (150, 12288, 0, 0), (4, 20480, 0, 0), (151, 640, 0, 0), (7000, 320, 0, 8), (6001, 24, 0, 0),
+    (300, 130, 0, 0), (160, 2050, 2, 2), (3, 9002, 0, 0), (151, 5002, 0, 6),  # pairs
 ]
 
 
