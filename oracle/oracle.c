@@ -424,16 +424,34 @@ int orc_matmul_i32(const int32_t *a, int64_t ar, int64_t ac, int64_t lda, const 
 /* Syrk<Dense,Dense> (Syrk.h:51-71): cblas_dsyrk on the upper triangle, then the mirror loop (:65-69) */
 int orc_syrk_f64(const double *arg, int64_t rows, int64_t cols, int64_t ld, int trans_left, double *res) {
     const int64_t n = trans_left ? cols : rows, k = trans_left ? rows : cols;
-    for (int64_t i = 0; i < n; i++)
-        for (int64_t j = i; j < n; j++) {
-            double s = 0.0;
+    if (trans_left) {
+        /* every entry is the sum over the rows in their order, starting from zero; row by row, so that a tall argument is
+         * read along its rows, 16 result rows per turn */
+#pragma omp parallel for schedule(dynamic)
+        for (int64_t i0 = 0; i0 < n; i0 += 16) {
+            const int64_t i1 = i0 + 16 < n ? i0 + 16 : n;
+            for (int64_t i = i0; i < i1; i++)
+                for (int64_t j = i; j < n; j++)
+                    res[i * n + j] = 0.0;
             for (int64_t l = 0; l < k; l++) {
-                const double x = trans_left ? arg[l * ld + i] : arg[i * ld + l];
-                const double y = trans_left ? arg[l * ld + j] : arg[j * ld + l];
-                s = s + x * y;
+                const double *row = arg + l * ld;
+                for (int64_t i = i0; i < i1; i++) {
+                    const double x = row[i];
+                    double *out = res + i * n;
+#pragma omp simd
+                    for (int64_t j = i; j < n; j++)
+                        out[j] = out[j] + x * row[j];
+                }
             }
-            res[i * n + j] = s;
         }
+    } else
+        for (int64_t i = 0; i < n; i++)
+            for (int64_t j = i; j < n; j++) {
+                double s = 0.0;
+                for (int64_t l = 0; l < k; l++)
+                    s = s + arg[i * ld + l] * arg[j * ld + l];
+                res[i * n + j] = s;
+            }
     for (int64_t r = 0; r < n; r++)
         for (int64_t c = r + 1; c < n; c++)
             res[c * n + r] = res[r * n + c];
