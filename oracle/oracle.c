@@ -371,6 +371,26 @@ int orc_matmul_f64(const double *a, int64_t ar, int64_t ac, int64_t lda, const d
     const int64_t m = transa ? ac : ar, k = transa ? ar : ac, k2 = transb ? bc : br, n = transb ? br : bc;
     if (k != k2)
         return 1;
+    if (transa && !transb) { /* the same sums in the same order, along the rows of both arguments */
+#pragma omp parallel for schedule(dynamic) if (m * n * k > 1 << 20)
+        for (int64_t i0 = 0; i0 < m; i0 += 8) {
+            const int64_t i1 = i0 + 8 < m ? i0 + 8 : m;
+            for (int64_t i = i0; i < i1; i++)
+                for (int64_t j = 0; j < n; j++)
+                    res[i * ldc + j] = 0.0;
+            for (int64_t l = 0; l < k; l++)
+                for (int64_t i = i0; i < i1; i++) {
+                    const double x = a[l * lda + i];
+                    double *out = res + i * ldc;
+                    const double *row = b + l * ldb;
+#pragma omp simd
+                    for (int64_t j = 0; j < n; j++)
+                        out[j] = out[j] + x * row[j];
+                }
+        }
+        return 0;
+    }
+#pragma omp parallel for schedule(static) if (m * n * k > 1 << 20)
     for (int64_t i = 0; i < m; i++)
         for (int64_t j = 0; j < n; j++) {
             double s = 0.0;
