@@ -70,6 +70,92 @@ template <typename T, int N, typename W> __device__ __forceinline__ Vec<T, N> na
     return z;
 }
 
+// ---- arithmetic on N wide values at once; floats go in pairs, two to an instruction ----
+template <typename T, int N> __device__ __forceinline__ void widen_all(const Vec<T, N> &x, wide_t<T> *y) {
+    if constexpr (std::is_same_v<T, __nv_bfloat16> && N % 2 == 0) {
+#pragma unroll
+        for (int k = 0; k < N; k += 2) { // a bfloat16 is the upper half of a float
+            const uint32_t two = *reinterpret_cast<const uint32_t *>(&x.v[k]);
+            y[k] = __uint_as_float(two << 16);
+            y[k + 1] = __uint_as_float(two & 0xffff0000u);
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < N; k++)
+            y[k] = widen(x.v[k]);
+    }
+}
+__device__ __forceinline__ uint64_t pair_of(float a, float b) {
+    uint64_t p;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(p) : "f"(a), "f"(b));
+    return p;
+}
+__device__ __forceinline__ void pair_to(uint64_t p, float *a) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a[0]), "=f"(a[1]) : "l"(p)); }
+// o = a * b + c
+template <int N, typename W> __device__ __forceinline__ void fma_all(const W *a, const W *b, const W *c, W *o) {
+    if constexpr (std::is_same_v<W, float> && N % 2 == 0) {
+#pragma unroll
+        for (int k = 0; k < N; k += 2) {
+            uint64_t r;
+            asm("fma.rn.f32x2 %0, %1, %2, %3;"
+                : "=l"(r)
+                : "l"(pair_of(a[k], a[k + 1])), "l"(pair_of(b[k], b[k + 1])), "l"(pair_of(c[k], c[k + 1])));
+            pair_to(r, o + k);
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < N; k++)
+            o[k] = a[k] * b[k] + c[k];
+    }
+}
+// o = a * b
+template <int N, typename W> __device__ __forceinline__ void mul_all(const W *a, const W *b, W *o) {
+    if constexpr (std::is_same_v<W, float> && N % 2 == 0) {
+#pragma unroll
+        for (int k = 0; k < N; k += 2) {
+            uint64_t r;
+            asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(pair_of(a[k], a[k + 1])), "l"(pair_of(b[k], b[k + 1])));
+            pair_to(r, o + k);
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < N; k++)
+            o[k] = a[k] * b[k];
+    }
+}
+// o = a + b
+template <int N, typename W> __device__ __forceinline__ void add_all(const W *a, const W *b, W *o) {
+    if constexpr (std::is_same_v<W, float> && N % 2 == 0) {
+#pragma unroll
+        for (int k = 0; k < N; k += 2) {
+            uint64_t r;
+            asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(pair_of(a[k], a[k + 1])), "l"(pair_of(b[k], b[k + 1])));
+            pair_to(r, o + k);
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < N; k++)
+            o[k] = a[k] + b[k];
+    }
+}
+template <int N, typename W> __device__ __forceinline__ void set_all(W *o, W x) {
+#pragma unroll
+    for (int k = 0; k < N; k++)
+        o[k] = x;
+}
+// sum over k of a[k] * b[k], added to two partial sums (pairs), or to the first of them
+template <int N, typename W> __device__ __forceinline__ void dot_all(const W *a, const W *b, W *sums) {
+    if constexpr (N % 2 == 0) {
+#pragma unroll
+        for (int k = 0; k < N; k += 2)
+            fma_all<2>(a + k, b + k, sums, sums);
+    } else {
+#pragma unroll
+        for (int k = 0; k < N; k++)
+            sums[0] = a[k] * b[k] + sums[0];
+    }
+}
+
 // N elements from global to shared memory, asynchronously (at once where they are fewer than four bytes).  fetch_commit
 // closes a group of them, fetch_wait<K> waits until all but the last K groups have arrived, for the calling thread.
 template <typename T, int N> __device__ __forceinline__ void fetch(T *to, const T *from) {
