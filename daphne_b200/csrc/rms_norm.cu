@@ -56,6 +56,20 @@ template <typename T, int N, int PPT> struct RowRing {
     __device__ int last() const { return stage == 0 ? NORM_STAGES - 1 : stage - 1; } // the one emptied last
     __device__ void next() { stage = stage == NORM_STAGES - 1 ? 0 : stage + 1; }
 };
+// A thread's two-byte elements of one row into the ring, which cannot be copied asynchronously: they are loaded all at once,
+// without conditions (places without an element repeat the last one), since a load whose store to shared memory follows
+// at once holds up the next one.
+template <typename T, int N, int PPT>
+__device__ __forceinline__ void fetch_row(const RowRing<T, N, PPT> &ring, int stage, int operand, const T *row, int tx, int tpr,
+                                          int packets) {
+    Vec<T, N> x[PPT];
+#pragma unroll
+    for (int k = 0; k < PPT; k++)
+        x[k] = ld_vec<T, N>(row + (tx + k * tpr < packets ? tx + k * tpr : packets - 1) * N);
+#pragma unroll
+    for (int k = 0; k < PPT; k++)
+        st_vec<T, N>(ring.at(stage, operand, k), x[k]);
+}
 size_t ring_bytes(size_t packet, int ppt, int operands, int block) {
     return (size_t)NORM_STAGES * operands * ppt * block * packet;
 }
@@ -69,7 +83,7 @@ template <typename T> struct NormArgs { // x, residual and sum may be the same m
     int64_t rows, cols, x_ld, residual_ld, sum_ld, res_ld, scales_ld;
     int64_t group;  // columns per scale; 0: one scale a row
     int64_t groups; // scales per row
-    wide_t<T> eps;
+    wide_t<T> eps, share; // share: 1 / cols
 };
 
 template <typename T, int N>
@@ -145,14 +159,21 @@ __global__ void __launch_bounds__(NORM_MAX_WARPS * 32) norm_rows_kernel(NormArgs
     unsigned *group_max = reinterpret_cast<unsigned *>(ring.at(NORM_STAGES, 0, 0) - (int)threadIdx.x * N);
     const int64_t step = (int64_t)gridDim.x * at_once;
     auto load = [&](int stage, int64_t r) {
-        if (r < a.rows)
+        if (r < a.rows) {
+            if constexpr (sizeof(T) * N >= 4) {
 #pragma unroll
-            for (int k = 0; k < PPT; k++)
-                if (tx + k * tpr < packets) {
-                    fetch<T, N>(ring.at(stage, 0, k), a.x + r * a.x_ld + (tx + k * tpr) * N);
-                    if (a.residual)
-                        fetch<T, N>(ring.at(stage, 1, k), a.residual + r * a.residual_ld + (tx + k * tpr) * N);
-                }
+                for (int k = 0; k < PPT; k++)
+                    if (tx + k * tpr < packets) {
+                        fetch<T, N>(ring.at(stage, 0, k), a.x + r * a.x_ld + (tx + k * tpr) * N);
+                        if (a.residual)
+                            fetch<T, N>(ring.at(stage, 1, k), a.residual + r * a.residual_ld + (tx + k * tpr) * N);
+                    }
+            } else {
+                fetch_row(ring, stage, 0, a.x + r * a.x_ld, tx, tpr, packets);
+                if (a.residual)
+                    fetch_row(ring, stage, 1, a.residual + r * a.residual_ld, tx, tpr, packets);
+            }
+        }
         fetch_commit();
     };
     for (int i = 0; i < NORM_STAGES - 1; i++)
@@ -185,7 +206,7 @@ __global__ void __launch_bounds__(NORM_MAX_WARPS * 32) norm_rows_kernel(NormArgs
         for (int k = 0; k < PPT; k++)
             if (live && tx + k * tpr < packets)
                 squares(s[k], ss);
-        const W rstd = W(1) / sqrt(row_sum(ss[0] + ss[1], tpr) / W(a.cols) + a.eps);
+        const W rstd = rsqrt(row_sum(ss[0] + ss[1], tpr) * a.share + a.eps); // every thread of a row: no divisions
         if (live && tx == 0 && a.rstd)
             a.rstd[r] = rstd;
         if constexpr (!Q8) {
@@ -283,7 +304,7 @@ __global__ void __launch_bounds__(LONG_BLOCK) norm_long_kernel(NormArgs<T> a) {
                 st_vec<T, N>(a.sum + r * a.sum_ld + p * N, s);
             squares(s, ss);
         }
-        const W rstd = W(1) / sqrt(row_sum(ss[0] + ss[1], LONG_BLOCK) / W(a.cols) + a.eps);
+        const W rstd = rsqrt(row_sum(ss[0] + ss[1], LONG_BLOCK) * a.share + a.eps);
         if (threadIdx.x == 0 && a.rstd)
             a.rstd[r] = rstd;
         if constexpr (!Q8) {
@@ -347,6 +368,7 @@ template <typename T> struct NormGradArgs { // dx may be the same matrix as grad
     T *dx;
     wide_t<T> *part; // CTAs x part_ld column sums, or null
     int64_t rows, cols, grad_ld, sum_ld, dsum_ld, dx_ld, part_ld;
+    wide_t<T> share; // 1 / cols
 };
 
 // dx of the rows, and the CTA's column sums of dy * s * rstd: a thread keeps the sums of its columns in registers over
@@ -367,15 +389,23 @@ __global__ void __launch_bounds__(NORM_MAX_WARPS * 32) norm_grad_rows_kernel(Nor
             dw[k][j] = 0;
     const int64_t step = (int64_t)gridDim.x * at_once;
     auto load = [&](int stage, int64_t r) {
-        if (r < a.rows)
+        if (r < a.rows) {
+            if constexpr (sizeof(T) * N >= 4) {
 #pragma unroll
-            for (int k = 0; k < PPT; k++)
-                if (tx + k * tpr < packets) {
-                    fetch<T, N>(ring.at(stage, 0, k), a.grad + r * a.grad_ld + (tx + k * tpr) * N);
-                    fetch<T, N>(ring.at(stage, 1, k), a.sum + r * a.sum_ld + (tx + k * tpr) * N);
-                    if (a.dsum)
-                        fetch<T, N>(ring.at(stage, 2, k), a.dsum + r * a.dsum_ld + (tx + k * tpr) * N);
-                }
+                for (int k = 0; k < PPT; k++)
+                    if (tx + k * tpr < packets) {
+                        fetch<T, N>(ring.at(stage, 0, k), a.grad + r * a.grad_ld + (tx + k * tpr) * N);
+                        fetch<T, N>(ring.at(stage, 1, k), a.sum + r * a.sum_ld + (tx + k * tpr) * N);
+                        if (a.dsum)
+                            fetch<T, N>(ring.at(stage, 2, k), a.dsum + r * a.dsum_ld + (tx + k * tpr) * N);
+                    }
+            } else {
+                fetch_row(ring, stage, 0, a.grad + r * a.grad_ld, tx, tpr, packets);
+                fetch_row(ring, stage, 1, a.sum + r * a.sum_ld, tx, tpr, packets);
+                if (a.dsum)
+                    fetch_row(ring, stage, 2, a.dsum + r * a.dsum_ld, tx, tpr, packets);
+            }
+        }
         fetch_commit();
     };
     for (int i = 0; i < NORM_STAGES - 1; i++)
@@ -407,7 +437,7 @@ __global__ void __launch_bounds__(NORM_MAX_WARPS * 32) norm_grad_rows_kernel(Nor
                     dot_all<N>(t[k], v[k], dots);
                 }
         }
-        const W factor = row_sum(dots[0] + dots[1], tpr) / W(a.cols) * rstd * rstd;
+        const W factor = row_sum(dots[0] + dots[1], tpr) * a.share * rstd * rstd;
         if (live) {
             W f[N], r[N];
             set_all<N>(f, -factor);
@@ -478,7 +508,7 @@ __global__ void __launch_bounds__(LONG_BLOCK) norm_grad_long_kernel(NormGradArgs
             for (int j = 0; j < N; j++)
                 dot += (a.weight ? widen(gv.v[j]) * widen(w.v[j]) : W(widen(gv.v[j]))) * widen(sv.v[j]);
         }
-        const W factor = row_sum(dot, LONG_BLOCK) / W(a.cols) * rstd * rstd;
+        const W factor = row_sum(dot, LONG_BLOCK) * a.share * rstd * rstd;
         for (int64_t p = threadIdx.x; p < packets; p += LONG_BLOCK) {
             const Vec<T, N> gv = ld_vec<T, N>(g + p * N), sv = ld_vec<T, N>(s + p * N);
             Vec<T, N> w, d, z;
@@ -567,18 +597,14 @@ RowPlan row_plan(int64_t packets, int64_t rows, int first, int most, int step, i
     p.block = p.fits ? p.tpr * (p.tpr < 256 ? 256 / p.tpr : 1) : 0;
     return p;
 }
-// packets a thread that there are kernels for: 1 to 3 (gradient: 4), or 4 and 8 smaller ones
+// packets a thread that there are kernels for: 1 to 3 (gradient: 4), or 4 smaller ones
 template <typename T, int N> RowPlan row_plan(int64_t cols, int64_t rows, bool back) {
     const int place = NORM_STAGES * (back ? 3 : 2) * N * (int)sizeof(T);
-    return N <= 2 && sizeof(T) * N < 16 ? row_plan(cols / N, rows, 4, 8, 4, place) : row_plan(cols / N, rows, 1, back ? 4 : 3, 1, place);
+    return N <= 2 && sizeof(T) * N < 16 ? row_plan(cols / N, rows, 4, 4, 1, place) : row_plan(cols / N, rows, 1, back ? 4 : 3, 1, place);
 }
 #define DB2_BY_PACKETS(N, BACK, ppt, LAUNCH)                                                                                 \
     if constexpr (N * sizeof(T) < 16) {                                                                                \
-        if (ppt == 4) {                                                                                                \
-            LAUNCH(4)                                                                                                  \
-        } else {                                                                                                       \
-            LAUNCH(8)                                                                                                  \
-        }                                                                                                              \
+        LAUNCH(4)                                                                                                      \
     } else if (ppt == 1) {                                                                                             \
         LAUNCH(1)                                                                                                      \
     } else if (ppt == 2) {                                                                                             \
@@ -773,7 +799,7 @@ int db2k_rms_norm(int dtype, const void *x, int64_t rows, int64_t cols, int64_t 
         constexpr int N = 16 / sizeof(T);
         NormArgs<T> a{static_cast<const T *>(x), static_cast<const T *>(residual), static_cast<const T *>(weight),
                       static_cast<T *>(sum), res, nullptr, static_cast<wide_t<T> *>(rstd), rows, cols, x_ld,
-                      residual_ld, sum_ld, res_ld, 0, 0, 0, (wide_t<T>)eps};
+                      residual_ld, sum_ld, res_ld, 0, 0, 0, (wide_t<T>)eps, wide_t<T>(1) / wide_t<T>(cols)};
         auto packed = [&](int n) {
             const size_t b = n * sizeof(T);
             return cols % n == 0 && rows_aligned(x, x_ld, sizeof(T), b) && rows_aligned(residual, residual_ld, sizeof(T), b) &&
@@ -807,7 +833,7 @@ int db2k_rms_norm_q8(int dtype, const void *x, int64_t rows, int64_t cols, int64
         constexpr int N = 16 / sizeof(T);
         NormArgs<T> a{static_cast<const T *>(x), static_cast<const T *>(residual), static_cast<const T *>(weight),
                       static_cast<T *>(sum), res, static_cast<float *>(scales), static_cast<float *>(rstd), rows, cols,
-                      x_ld, residual_ld, sum_ld, res_ld, scales_ld, group, groups, (float)eps};
+                      x_ld, residual_ld, sum_ld, res_ld, scales_ld, group, groups, (float)eps, 1.0f / (float)cols};
         auto packed = [&](int n) {
             const size_t b = n * sizeof(T);
             return cols % n == 0 && rows_aligned(x, x_ld, sizeof(T), b) && rows_aligned(residual, residual_ld, sizeof(T), b) &&
@@ -851,7 +877,7 @@ int db2k_rms_norm_grad(int dtype, const void *grad, int64_t grad_ld, int64_t row
         NormGradArgs<T> a{static_cast<const T *>(grad), static_cast<const T *>(sum), static_cast<const T *>(weight),
                           static_cast<const T *>(dsum), static_cast<const wide_t<T> *>(rstd), static_cast<T *>(dx),
                           dweight ? static_cast<wide_t<T> *>(scratch) : nullptr, rows, cols, grad_ld, sum_ld, dsum_ld,
-                          dx_ld, part_ld_of(cols)};
+                          dx_ld, part_ld_of(cols), wide_t<T>(1) / wide_t<T>(cols)};
         auto packed = [&](int n) {
             const size_t b = n * sizeof(T);
             return cols % n == 0 && rows_aligned(grad, grad_ld, sizeof(T), b) && rows_aligned(sum, sum_ld, sizeof(T), b) &&
