@@ -34,7 +34,8 @@ template <typename T> struct ScanArgs {
     T *h, *dg, *dx;
     const W *h0, *init; // init: the state that enters (forward: h0; gradient: the gradient of the last state)
     W *last;            // the state that leaves (forward: last state; gradient: dh0)
-    W *part;            // split sequences: (A, B) per block
+    W *part;            // split sequences: (A, B) per block, then a copy of init (last may be written over init before
+                        // the CTA of another block has read it)
     const int64_t *off;
     int64_t g_ld, x_ld, grad_ld, above_ld, h_ld, dg_ld, dx_ld, h0_ld, init_ld, last_ld, part_ld;
     int64_t rows, cols, seqs, strips;
@@ -120,6 +121,8 @@ __global__ void __launch_bounds__(WARPS * 32, WARPS == 4 ? 3 : 1) gated_scan_ker
     for (int k = 0; k < VEC; k++) {
         prod[k] = W(1);
         state[k] = !AGGREGATE && in && a.init ? a.init[seq * a.init_ld + c + k] : W(0);
+        if (AGGREGATE && in && a.init && blk == 0 && warp == 0) // the copy that the second pass reads
+            a.part[(a.seqs * a.blocks * 2 + seq) * a.part_ld + c + k] = a.init[seq * a.init_ld + c + k];
     }
     if (!AGGREGATE && blk > 0) { // the blocks in front: a share for each warp, then the shares in order
         const int64_t share = (blk + WARPS - 1) / WARPS, b0 = warp * share, b1 = b0 + share < blk ? b0 + share : blk;
@@ -400,6 +403,10 @@ template <typename T, int VEC, int WARPS, bool BACK, bool SIGMOID> int scan_laun
         if (a.blocks > 1) {
             aggregate<<<(unsigned)ctas, 128, stage * 2, st>>>(a);
             DB2_TRY(after_launch("gated_scan_kernel"));
+            if (a.init) {
+                a.init = a.part + a.seqs * a.blocks * 2 * a.part_ld;
+                a.init_ld = a.part_ld;
+            }
         }
     whole<<<(unsigned)ctas, WARPS * 32, stage * operands, st>>>(a);
     return after_launch("gated_scan_kernel");
@@ -505,7 +512,7 @@ size_t db2k_gated_scan_scratch_bytes(int dtype, int64_t rows, int64_t cols, int6
                         : es == 4 ? scan_plan<float>(rows, cols, seqs, 1)
                                   : scan_plan<__half>(rows, cols, seqs, 1))
                            .blocks;
-    return blocks < 2 ? 0 : (size_t)seqs * blocks * 2 * scan_part_ld(cols) * (dtype == DB2_F64 ? 8 : 4);
+    return blocks < 2 ? 0 : (size_t)seqs * (blocks * 2 + 1) * scan_part_ld(cols) * (dtype == DB2_F64 ? 8 : 4);
 }
 
 int db2k_gated_scan(int dtype, int gate, const void *g, int64_t g_ld, const void *x, int64_t x_ld, int64_t rows,

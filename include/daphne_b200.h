@@ -266,7 +266,7 @@ int db2k_solve(int dtype, void *a_work, int64_t n, void *x_inout, int32_t *dev_s
 /* Embedding: res[i] = scale * table[tokens[i]] for n tokens (DB2_I64 or DB2_I32, stride tokens_ld) and a table of vocab
  * rows.  Token -1 marks padding and gives a row of zeros; any other token outside [0, vocab) gives a row of zeros and
  * sets *dev_status (a device int32, may be NULL; never cleared here) to 1.  The product of one-hot rows with the table,
- * without the one-hot rows. */
+ * without the one-hot rows.  res overlaps nothing. */
 int db2k_embed(int dtype, const void *table, int64_t vocab, int64_t cols, int64_t table_ld, int index_dtype,
                const void *tokens, int64_t tokens_ld, int64_t n, double scale, void *res, int64_t res_ld,
                int32_t *dev_status, void *stream);

@@ -298,6 +298,23 @@ def test_result_in_the_place_of_an_operand(rows, cols):
 
 
 @gpu
+@pytest.mark.parametrize("rows,cols,off", [(130, 70, [0, 0, 50, 130]), (20000, 5, 1), (9001, 34, [0, 1500, 1501, 9000])])
+def test_last_states_in_the_place_of_the_first(rows, cols, off):
+    off, dev = _offsets(rows, off)
+    seqs = len(off) - 1
+    for tname in ALL:
+        t, code = TYPES[tname]
+        G, X, H0 = _inputs(tname, SIGMOID, rows, cols, off)
+        H, L = _scan(tname, SIGMOID, G, X, seqs, dev, H0)
+        exp, last = H.view.clone(), L.view.clone()
+        n = lib.db2k_gated_scan_scratch_bytes(code, rows, cols, seqs)
+        s = scratch(n)
+        check(lib.db2k_gated_scan(code, SIGMOID, *G.at, *X.at, rows, cols, None if dev is None else dev.data_ptr(), seqs,
+                                  *H0.at, *H.at, *H0.at, s.data_ptr(), n, stream()))
+        assert torch.equal(H.view, exp) and torch.equal(H0.view, last) and H0.guards_intact()
+
+
+@gpu
 def test_offsets_that_break_their_rules_stay_within_the_matrices():
     G, X, H0 = _inputs("f32", DECAY, 100, 40, np.arange(5))
     dev = torch.tensor([-50, 40, 20, 1 << 40, 90], dtype=torch.int64, device="cuda")
