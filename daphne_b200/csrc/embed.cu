@@ -477,20 +477,33 @@ __global__ void __launch_bounds__(SUM_THREADS)
 }
 
 // Tokens whose rows span several runs: the run in which such a token starts adds the partial sums behind it, in order.
-// A CTA looks at one run and 32 x JOIN_N columns; its warps take equal shares of the runs, whose sums are added in the
-// order of the shares.  Most CTAs find nothing to do.
-constexpr int JOIN_Y = 8, JOIN_N = 4;
+// A CTA looks at `per` runs and 32 x JOIN_N columns; for each run that has something to join, its warps take equal shares
+// of the parts, whose sums are added in the order of the shares.  Most runs have nothing to join: where they are many, a
+// CTA looks at up to JOIN_RUNS of them, so that fewer CTAs are started for nothing (16 per SM).
+constexpr int JOIN_Y = 8, JOIN_N = 4, JOIN_RUNS = 8;
 template <typename T, typename R, bool ADD>
 __global__ void __launch_bounds__(32 * JOIN_Y)
-    embed_join_kernel(SumArgs a, wide_t<T> scale, R *__restrict__ res, const wide_t<T> *__restrict__ part) {
+    embed_join_kernel(SumArgs a, wide_t<T> scale, R *__restrict__ res, const wide_t<T> *__restrict__ part, int per) {
     using W = wide_t<T>;
     __shared__ W sums[JOIN_Y][32 * JOIN_N];
     const int tx = threadIdx.x % 32, ty = threadIdx.x / 32;
-    for (int64_t run = blockIdx.x; run + 1 < a.runs; run += gridDim.x) {
-        const int64_t b = run * SUM_RUN, e = b + SUM_RUN; // e < n: the run is not the last
-        const uint32_t v = a.key[e - 1], next = a.key[e], start = a.key[b], before = b > 0 ? a.key[b - 1] : 0xffffffffu;
-        if (v >= (uint32_t)a.vocab || next != v || (start == v && before == v))
-            continue; // uniform over the CTA: the last token ends here, or started in an earlier run
+    __shared__ uint32_t token[JOIN_RUNS]; // the token to join, or the number of table rows
+    if (threadIdx.x < per) {
+        const int64_t run = (int64_t)blockIdx.x * per + threadIdx.x, b = run * SUM_RUN, e = b + SUM_RUN;
+        uint32_t v = (uint32_t)a.vocab;
+        if (run + 1 < a.runs) { // not the last run: e < n
+            const uint32_t last = a.key[e - 1], next = a.key[e], start = a.key[b], before = b > 0 ? a.key[b - 1] : 0xffffffffu;
+            if (last < v && next == last && !(start == last && before == last))
+                v = last; // it goes on behind this run and starts in it
+        }
+        token[threadIdx.x] = v;
+    }
+    __syncthreads();
+    for (int i = 0; i < per; i++) {
+        const int64_t run = (int64_t)blockIdx.x * per + i;
+        const uint32_t v = token[i];
+        if (v == (uint32_t)a.vocab)
+            continue; // uniform over the CTA
         // runs behind this one that hold a part: those that begin with this token
         int64_t more = 0;
         for (;;) {
@@ -525,11 +538,11 @@ __global__ void __launch_bounds__(32 * JOIN_Y)
             for (int k = 0; k < JOIN_N; k++)
                 sums[ty][tx * JOIN_N + k] = acc[k];
             __syncthreads();
-            for (int i = threadIdx.x; i < 32 * JOIN_N && c0 + i < a.cols; i += 32 * JOIN_Y) {
-                W s = sums[0][i];
+            for (int j = threadIdx.x; j < 32 * JOIN_N && c0 + j < a.cols; j += 32 * JOIN_Y) {
+                W s = sums[0][j];
                 for (int k = 1; k < JOIN_Y; k++)
-                    s += sums[k][i];
-                R *dst = res + (int64_t)v * a.res_ld + c0 + i;
+                    s += sums[k][j];
+                R *dst = res + (int64_t)v * a.res_ld + c0 + j;
                 *dst = narrow<R>(ADD ? W(widen(*dst)) + s * scale : s * scale);
             }
         }
@@ -641,10 +654,11 @@ int embed_sum(SumArgs a, const void *grad, double scale, void *res, void *part, 
     if (a.runs > 1) {
         int64_t jy = (a.cols + 32 * JOIN_N - 1) / (32 * JOIN_N);
         jy = jy > 64 ? 64 : jy;
-        int64_t jx = a.runs - 1;
-        jx = jx > 65536 / jy ? 65536 / jy : jx;
+        int64_t per = a.runs * jy / ((int64_t)sm_count() * 16);
+        per = per < 1 ? 1 : (per > JOIN_RUNS ? JOIN_RUNS : per);
+        const int64_t jx = (a.runs - 1 + per - 1) / per;
         embed_join_kernel<T, R, ADD><<<dim3((unsigned)jx, (unsigned)jy), 32 * JOIN_Y, 0, st>>>(
-            a, (wide_t<T>)scale, static_cast<R *>(res), static_cast<const wide_t<T> *>(part));
+            a, (wide_t<T>)scale, static_cast<R *>(res), static_cast<const wide_t<T> *>(part), (int)per);
         DB2_TRY(after_launch("embed_join_kernel"));
     }
     return DB2_OK;
