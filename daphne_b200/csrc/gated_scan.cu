@@ -8,7 +8,7 @@
 //     c = f[t] * delta[t]      dx = delta          (SIGMOID: delta * (1 - f))                      dh0 = the last c
 //
 // Both are first-order recurrences v <- a * v + b, and the composition of two such steps is one again: (A, B) of a run of
-// rows says all about it.  A warp holds SCAN_R consecutive rows of 32 lanes x VEC columns in registers and forms their
+// rows says all about it.  A warp holds 8 (gradient: 4) consecutive rows of 32 lanes x VEC columns in registers and forms their
 // (A, B); the warps of a CTA exchange theirs through shared memory; every warp then walks its rows once more, from the
 // value that really enters them.  So each operand is read once and each result written once.
 //
@@ -21,7 +21,7 @@ namespace db2 {
 
 namespace {
 
-// A lane takes 8 bytes of a row, a warp SCAN_R consecutive rows at once.  More rows would spread the exchange between the
+// A lane takes 8 bytes of a row, a warp several consecutive rows at once.  More rows would spread the exchange between the
 // warps over more work, but the gates and inputs of a thread's rows have to stay in its registers.
 template <typename T> constexpr int widest() { return 8 / sizeof(T); }
 template <bool BACK> constexpr int scan_rows() { return BACK ? 4 : 8; }
