@@ -74,7 +74,7 @@ __device__ __forceinline__ void gate_pair(double g, double *f, double *o) {
 }
 
 // A product of gates as it is passed on: finite, so that gates above 1 whose product overflows do not turn a state of zero
-// into NaN.  (A NaN among the gates is in the composed step's b as well.)
+// into NaN.  (A gate that is itself not finite makes the composed step's b so, too.)
 __device__ __forceinline__ float finite(float a) { return fminf(fmaxf(a, -3.40282347e38f), 3.40282347e38f); }
 __device__ __forceinline__ double finite(double a) { return fmin(fmax(a, -1.7976931348623157e308), 1.7976931348623157e308); }
 
@@ -255,7 +255,8 @@ __global__ void __launch_bounds__(WARPS * 32, WARPS == 4 ? 3 : 1) gated_scan_ker
 #pragma unroll
         for (int k = 0; k < VEC; k++) {
             A[k] = f[0][k];
-            B[k] = BACK ? f[0][k] * b[0][k] : b[0][k];
+            // 0 * f: a gate that is not finite leaves its mark in B, where finite() does not reach
+            B[k] = BACK ? f[0][k] * b[0][k] : f[0][k] * W(0) + b[0][k];
         }
 #pragma unroll
         for (int i = 1; i < R; i++)

@@ -266,6 +266,32 @@ def test_non_finite_values_stay_in_their_column_and_sequence(rows):
 
 
 @gpu
+@pytest.mark.parametrize("rows", [200, 20000])
+@pytest.mark.parametrize("row", [0, 3, 8, 31, 32, 64, 77])
+def test_gates_that_are_not_finite(rows, row):
+    """They reach all later rows of their column and sequence (earlier ones in the gradient), whatever the state is."""
+    off, dev = _offsets(rows, [0, rows // 2, rows])
+    for tname in ("f32", "f64", "bf16"):
+        t = TYPES[tname][0]
+        for bad in (float("nan"), float("inf")):
+            g = np.full((rows, 5), 0.5)
+            g[row, 1] = bad
+            G, X = Mat(g, t), Mat(np.zeros((rows, 5)), t)
+            H, L = _scan(tname, DECAY, G, X, 2, dev, None)  # a state of zero in front of it
+            h = H.f64()
+            assert not np.isfinite(h[row:rows // 2, 1]).any() and not np.isfinite(L.f64()[0, 1])
+            keep = np.ones(h.shape, dtype=bool)
+            keep[row:rows // 2, 1] = False
+            assert not h[keep].any() and not L.f64()[1].any()
+            D = Mat(np.ones((rows, 5)), t)
+            clean = _scan(tname, DECAY, Mat(np.full((rows, 5), 0.5), t), X, 2, dev, None)[0]
+            DG, DX, DH0 = _grad(tname, DECAY, G, X, clean, D, 2, dev, None, None)
+            assert not np.isfinite(DX.f64()[:row, 1]).any() and not np.isfinite(DH0.f64()[0, 1])
+            assert np.isfinite(np.delete(DX.f64(), 1, 1)).all() and np.isfinite(DX.f64()[row:, 1]).all()
+            assert np.isfinite(DH0.f64()[1]).all()
+
+
+@gpu
 def test_extreme_gates():
     # large gates on a state of zero: the overflowing product of the gates does not reach it
     for rows in (300, 20000):
