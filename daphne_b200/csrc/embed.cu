@@ -166,6 +166,7 @@ __global__ void __launch_bounds__(SORT_CHUNK)
         write_zeros_any(z, blockIdx.x - chunks, gridDim.x - chunks);
         return;
     }
+    start_next(); // (the CTAs above say so by their end: their stores come first)
     __shared__ uint4 quads[SORT_CHUNK / 4];
     const int base = blockIdx.x * SORT_CHUNK, t = threadIdx.x;
     // places behind the last token hold a key behind all others
@@ -203,6 +204,8 @@ __global__ void __launch_bounds__(MERGE_THREADS)
     token_merge_kernel(const uint32_t *__restrict__ key, const uint32_t *__restrict__ pos, int n,
                        uint32_t *__restrict__ key_out, uint32_t *__restrict__ pos_out, int per_cta) {
     extern __shared__ uint32_t k[];
+    wait_for_last();
+    start_next();
 #pragma unroll 8
     for (int i = threadIdx.x; i < n; i += MERGE_THREADS)
         k[i / SORT_CHUNK * MERGE_PITCH + i % SORT_CHUNK] = key[i];
@@ -399,6 +402,8 @@ __global__ void __launch_bounds__(SUM_THREADS)
     __shared__ uint32_t keys[(SUM_THREADS >> SUM_MIN_LOG) * SUM_RUN + 2], rows[(SUM_THREADS >> SUM_MIN_LOG) * SUM_RUN];
     const int tpr = 1 << a.log_tpr, tx = threadIdx.x & (tpr - 1), ty = threadIdx.x >> a.log_tpr;
     const int here = (SUM_THREADS >> a.log_tpr) * SUM_RUN;
+    wait_for_last();
+    start_next();
     const int64_t cta_first = (int64_t)blockIdx.x * here;
     for (int i = threadIdx.x; i < here + 2; i += SUM_THREADS) {
         const int64_t at = cta_first + i - 1;
@@ -487,6 +492,7 @@ __global__ void __launch_bounds__(32 * JOIN_Y)
     using W = wide_t<T>;
     __shared__ W sums[JOIN_Y][32 * JOIN_N];
     const int tx = threadIdx.x % 32, ty = threadIdx.x / 32;
+    wait_for_last();
     __shared__ uint32_t token[JOIN_RUNS]; // the token to join, or the number of table rows
     if (threadIdx.x < per) {
         const int64_t run = (int64_t)blockIdx.x * per + threadIdx.x, b = run * SUM_RUN, e = b + SUM_RUN;
@@ -607,9 +613,8 @@ int embed_sort(const GradPlan &p, const void *tokens, int64_t tokens_ld, int64_t
         }
         // every CTA reads all keys: no more CTAs than SMs, of whole rounds of MERGE_ROUND tokens
         const int per_cta = (int)((n + sm_count() * MERGE_ROUND - 1) / (sm_count() * MERGE_ROUND)) * MERGE_ROUND;
-        token_merge_kernel<<<(unsigned)((n + per_cta - 1) / per_cta), MERGE_THREADS, (size_t)chunks * MERGE_PITCH * 4, st>>>(
-            k[0], q[0], (int)n, k[1], q[1], per_cta);
-        DB2_TRY(after_launch("token_merge_kernel"));
+        DB2_TRY(launch_next("token_merge_kernel", token_merge_kernel, dim3((unsigned)((n + per_cta - 1) / per_cta)),
+                            MERGE_THREADS, (size_t)chunks * MERGE_PITCH * 4, st, k[0], q[0], (int)n, k[1], q[1], per_cta));
         *key = k[1];
         *pos = q[1];
         return DB2_OK;
@@ -648,18 +653,17 @@ int embed_sum(SumArgs a, const void *grad, double scale, void *res, void *part, 
     const int64_t gx = (a.runs + groups - 1) / groups;
     int64_t gy = (packets + (1 << a.log_tpr) - 1) >> a.log_tpr;
     gy = gy > 1024 ? 1024 : gy;
-    embed_sum_kernel<T, R, N, ADD><<<dim3((unsigned)gx, (unsigned)gy), SUM_THREADS, 0, st>>>(
-        a, static_cast<const T *>(grad), (wide_t<T>)scale, static_cast<R *>(res), static_cast<wide_t<T> *>(part));
-    DB2_TRY(after_launch("embed_sum_kernel"));
+    DB2_TRY(launch_next("embed_sum_kernel", embed_sum_kernel<T, R, N, ADD>, dim3((unsigned)gx, (unsigned)gy), SUM_THREADS, 0,
+                        st, a, static_cast<const T *>(grad), (wide_t<T>)scale, static_cast<R *>(res),
+                        static_cast<wide_t<T> *>(part)));
     if (a.runs > 1) {
         int64_t jy = (a.cols + 32 * JOIN_N - 1) / (32 * JOIN_N);
         jy = jy > 64 ? 64 : jy;
         int64_t per = a.runs * jy / ((int64_t)sm_count() * 16);
         per = per < 1 ? 1 : (per > JOIN_RUNS ? JOIN_RUNS : per);
         const int64_t jx = (a.runs - 1 + per - 1) / per;
-        embed_join_kernel<T, R, ADD><<<dim3((unsigned)jx, (unsigned)jy), 32 * JOIN_Y, 0, st>>>(
-            a, (wide_t<T>)scale, static_cast<R *>(res), static_cast<const wide_t<T> *>(part), (int)per);
-        DB2_TRY(after_launch("embed_join_kernel"));
+        DB2_TRY(launch_next("embed_join_kernel", embed_join_kernel<T, R, ADD>, dim3((unsigned)jx, (unsigned)jy), 32 * JOIN_Y, 0,
+                            st, a, (wide_t<T>)scale, static_cast<R *>(res), static_cast<const wide_t<T> *>(part), (int)per));
     }
     return DB2_OK;
 }

@@ -109,6 +109,10 @@ __global__ void __launch_bounds__(WARPS * 32, WARPS == 4 ? 3 : 1) gated_scan_ker
     const int64_t blk = rest % a.blocks, seq = rest / a.blocks;
     const int64_t c = (strip * 32 + lane) * VEC;
     const bool in = c < a.cols; // cols is a multiple of VEC
+    if (AGGREGATE)
+        start_next();
+    else
+        wait_for_last();
     int64_t begin, end;
     sequence(a, seq, &begin, &end);
     // rows of the block, a multiple of the tile each: n rows from `first` on, in the direction of the recurrence
@@ -408,6 +412,7 @@ template <typename T, int VEC, int WARPS, bool BACK, bool SIGMOID> int scan_laun
                 a.init = a.part + a.seqs * a.blocks * 2 * a.part_ld;
                 a.init_ld = a.part_ld;
             }
+            return launch_next("gated_scan_kernel", whole, dim3((unsigned)ctas), WARPS * 32, stage * operands, st, a);
         }
     whole<<<(unsigned)ctas, WARPS * 32, stage * operands, st>>>(a);
     return after_launch("gated_scan_kernel");

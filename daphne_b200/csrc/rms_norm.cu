@@ -457,6 +457,7 @@ __global__ void __launch_bounds__(NORM_MAX_WARPS * 32) norm_grad_rows_kernel(Nor
         }
         ring.next();
     }
+    start_next(); // not earlier: CTAs that only wait take their places among those that work
     if (!a.part)
         return;
     W *part = a.part + (int64_t)blockIdx.x * a.part_ld;
@@ -554,6 +555,7 @@ template <typename W>
 __global__ void __launch_bounds__(32 * JOIN_SHARES)
     norm_join_kernel(const W *__restrict__ part, int parts, int64_t cols, int64_t part_ld, W *__restrict__ res) {
     __shared__ W sums[JOIN_SHARES][33];
+    wait_for_last();
     const int tx = threadIdx.x % 32, ty = threadIdx.x / 32;
     const int64_t c = (int64_t)blockIdx.x * 32 + tx;
     const int share = (parts + JOIN_SHARES - 1) / JOIN_SHARES, first = ty * share;
@@ -692,9 +694,8 @@ template <typename T, int N> int norm_grad_launch(NormGradArgs<T> a, wide_t<T> *
         parts = (int)grid;
     }
     if (a.part) {
-        norm_join_kernel<wide_t<T>><<<(unsigned)((a.cols + 31) / 32), 32 * JOIN_SHARES, 0, st>>>(a.part, parts, a.cols,
-                                                                                                 a.part_ld, dweight);
-        DB2_TRY(after_launch("norm_join_kernel"));
+        DB2_TRY(launch_next("norm_join_kernel", norm_join_kernel<wide_t<T>>, dim3((unsigned)((a.cols + 31) / 32)),
+                            32 * JOIN_SHARES, 0, st, a.part, parts, a.cols, a.part_ld, dweight));
     }
     return DB2_OK;
 }

@@ -171,6 +171,28 @@ template <typename T, int N> __device__ __forceinline__ void fetch(T *to, const 
 __device__ __forceinline__ void fetch_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int K> __device__ __forceinline__ void fetch_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(K) : "memory"); }
 
+// A kernel that follows another one of the same call may be set up while that one still runs: launch_next starts it early,
+// and wait_for_last, the first thing that all its threads do, returns when the kernel before it has finished and its
+// writes are visible.  start_next, in the kernel before, says that all its CTAs are on their way.  (A call's first kernel is
+// launched the ordinary way and so waits for everything in front of it.)
+__device__ __forceinline__ void wait_for_last() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void start_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+template <typename... P, typename... A>
+int launch_next(const char *what, void (*kernel)(P...), dim3 grid, int block, size_t smem, cudaStream_t st, A... args) {
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3((unsigned)block);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    DB2_CUDA(cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...));
+    return after_launch(what);
+}
+
 // whether rows of ld elements of es bytes starting at p all lie on multiples of `bytes` (absent operands do)
 inline bool rows_aligned(const void *p, int64_t ld, size_t es, size_t bytes) {
     return !p || (reinterpret_cast<uintptr_t>(p) % bytes == 0 && (size_t)ld * es % bytes == 0);
