@@ -189,8 +189,8 @@ int launch_next(const char *what, void (*kernel)(P...), dim3 grid, int block, si
     cfg.stream = st;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    DB2_CUDA(cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...));
-    return after_launch(what);
+    cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
+    return after_launch(what); // takes the error of a launch that failed
 }
 
 // whether rows of ld elements of es bytes starting at p all lie on multiples of `bytes` (absent operands do)
