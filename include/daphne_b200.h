@@ -289,9 +289,10 @@ int db2k_rms_norm(int dtype, const void *x, int64_t rows, int64_t cols, int64_t 
                   int64_t residual_ld, const void *weight, double eps, void *sum, int64_t sum_ld, void *res,
                   int64_t res_ld, void *rstd, void *stream);
 /* The same with an 8-bit result (DB2_F8E4M3): per row and group of `group` columns (16, 32, ..., 512; 0: the whole row;
- * the last group may be narrower) scale = max|y| / 448 and res = y / scale, rounded to nearest; scale is 1 where all y
- * are zero and never below the smallest normal float.  scales: rows x ceil(cols / group) floats (rows x 1 for group 0).
- * A group with a NaN gets a NaN scale.  Not for DB2_F64.  res overlaps nothing. */
+ * the last group may be narrower) scale = max|y| / 448 and res = y / scale; scale is 1 where all y are zero and never
+ * below the smallest normal float.  The quotient is formed from s * weight, not from a rounded y: for bf16 it is rounded
+ * once, to nearest even; f16 and float round the product s * weight first.  scales: rows x ceil(cols / group) floats (rows x
+ * 1 for group 0).  A group with a NaN gets a NaN scale.  Not for DB2_F64.  res overlaps nothing. */
 int db2k_rms_norm_q8(int dtype, const void *x, int64_t rows, int64_t cols, int64_t x_ld, const void *residual,
                      int64_t residual_ld, const void *weight, double eps, void *sum, int64_t sum_ld, void *res,
                      int64_t res_ld, void *scales, int64_t scales_ld, int64_t group, void *rstd, void *stream);
