@@ -315,7 +315,8 @@ int db2k_rms_norm_grad(int dtype, const void *grad, int64_t grad_ld, int64_t row
  * are left as they are, in h as in the gradients.  A sequence may be empty.  h0 (seqs x cols wide values, NULL: zeros) is the
  * state in front of every sequence; last (seqs x cols wide values, may be NULL, may be h0 itself) receives the state behind
  * it, unrounded.  h may be g or x itself (same pointer and leading dimension); no other overlap.
- * In float arithmetic sigmoid(g) does not go below 2^-125 (g = -infinity gives that, too).
+ * In float arithmetic sigmoid(g) does not go below 2^-125 (g = -infinity gives that, too), and 1 - sigmoid(g) is zero from g =
+ * 87.4 on; elsewhere both are good to a few units in the last place.
  * A NaN or an infinity stays within its column and sequence; what follows it there is not finite, but which of the
  * non-finite values is not specified.  Gates are expected within [-1, 1]: products of larger ones over many rows may
  * overflow where the recurrence itself does not. */

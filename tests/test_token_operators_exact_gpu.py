@@ -73,3 +73,34 @@ def test_eight_bit_scales_far_from_one():
     y = (s / np.sqrt((s * s).mean() + 1.0))[0, :4]
     v = Y.view.cpu().view(torch.float8_e4m3fn).double().numpy()[0]
     assert Q.f64()[0, 0] == 2.0 ** -126 and (np.abs(v[:4] - y) <= np.abs(y) * 2.0 ** -4).all() and not v[4:].any()
+
+
+def _gate_values(tname, g):
+    """f and 1 - f as the kernels have them: steps from a state of one without an input, and from none with an input of one."""
+    t, code = TYPES[tname]
+    G, n = Mat(g, t), g.shape[1]
+    out = []
+    for state in (1.0, 0.0):
+        X, S, N = Mat(torch.full((1, n), 1.0 - state), t), Mat(torch.full((1, n), state), torch.float32), Mat.empty(1, n, torch.float32)
+        check(lib.db2k_gated_step(code, names.GATE_SIGMOID, *G.at, *X.at, 1, n, *S.at, *N.at, None, 0, stream()))
+        out.append(N.f64()[0])
+    return G.f64()[0], *out
+
+
+@gpu
+@pytest.mark.parametrize("tname", ["f32", "f16", "bf16"])
+def test_sigmoid_is_as_accurate_for_large_arguments_as_for_small_ones(tname):
+    """Half steps (2^-24) that the parts of e = exp(-g), f = 1 / (1 + e) and 1 - f = e f may be off by: the base-2
+    exponential 2^-22.5, so 2.9; its correction 1; 1 + e 1; the reciprocal (a unit) 2; the last product 1; the sums and
+    products of the step round nothing.  One more for all second-order terms: 9."""
+    rng = np.random.default_rng(2)
+    g = np.concatenate([rng.uniform(-86, 86, 20000), rng.standard_normal(5000) * 2, np.linspace(-86, 86, 173), [0.0, -0.0]])
+    g, f, o = _gate_values(tname, g[None, :])
+    ef, eo = 1 / (1 + np.exp(-g)), 1 / (1 + np.exp(g))
+    assert (np.abs(f - ef) <= 9 * 2.0 ** -24 * ef).all(), np.max(np.abs(f - ef) / ef) * 2 ** 24
+    assert (np.abs(o - eo) <= 9 * 2.0 ** -24 * eo).all(), np.max(np.abs(o - eo) / eo) * 2 ** 24
+    # the ends: f stays at 2^-125 and above, 1 - f becomes zero, and nothing else happens there
+    g, f, o = _gate_values(tname, np.array([[-86.7, -90.0, -1e3, -6e4, -np.inf, 88.0, 150.0, 1e3, 6e4, np.inf, np.nan]]))
+    assert (f[:5] >= 2.0 ** -125).all() and (f[:5] <= 2.0 ** -124).all() and (o[:5] == 1).all()
+    assert (f[5:10] == 1).all() and (o[5:10] <= 2.0 ** -125).all() and (o[5:10] >= 0).all()
+    assert np.isnan(f[10]) and np.isnan(o[10])
