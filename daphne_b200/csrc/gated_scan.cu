@@ -732,10 +732,10 @@ int db2_gatedStep(db2_context *ctx, int gate, db2_matrix **h, db2_matrix **new_s
     // a new state in the place of the old one is written where it is: each element is read before it is written
     const bool in_place = *new_state == state;
     const DeviceOperand dg(g), dx(x);
-    DB2_TRY(prepare_result(ctx, h, g->dtype, g->rows, g->cols));
     if (in_place)
         DB2_TRY(prepare_update(state));
-    const DeviceOperand ds(state);
+    const DeviceOperand ds(state); // before any result is prepared, which may name it
+    DB2_TRY(prepare_result(ctx, h, g->dtype, g->rows, g->cols));
     if (!in_place)
         DB2_TRY(prepare_result(ctx, new_state, wide_dtype(g->dtype), g->rows, g->cols));
     DB2_TRY(db2k_gated_step(g->dtype, gate, dg.ptr, dg.ld, dx.ptr, dx.ld, g->rows, g->cols, ds.ptr, ds.ld,
