@@ -155,6 +155,27 @@ __device__ __forceinline__ uint32_t token_key(const void *tokens, int64_t ld, in
     return (uint32_t)vocab;
 }
 
+// Tokens of a call that has nothing to compute (no table rows, no columns): they are looked at for their status only.
+template <typename I>
+__global__ void __launch_bounds__(EMB_THREADS)
+    token_check_kernel(const void *tokens, int64_t tokens_ld, int64_t n, int64_t vocab, int32_t *status) {
+    for (int64_t i = (int64_t)blockIdx.x * EMB_THREADS + threadIdx.x; i < n; i += (int64_t)gridDim.x * EMB_THREADS)
+        token_key<I>(tokens, tokens_ld, i, vocab, status);
+}
+int check_tokens(const char *what, int index_dtype, const void *tokens, int64_t tokens_ld, int64_t n, int64_t vocab,
+                 int32_t *status, cudaStream_t st) {
+    if (n == 0 || !status)
+        return DB2_OK;
+    DB2_CHECK(tokens && ld_ok(tokens_ld, n, 1), DB2_EINVAL, "%s: null tokens or their stride too small", what);
+    const int64_t want = (n + EMB_THREADS - 1) / EMB_THREADS, cap = (int64_t)sm_count() * 8;
+    const unsigned grid = (unsigned)(want < cap ? want : cap);
+    if (index_dtype == DB2_I64)
+        token_check_kernel<int64_t><<<grid, EMB_THREADS, 0, st>>>(tokens, tokens_ld, n, vocab, status);
+    else
+        token_check_kernel<int32_t><<<grid, EMB_THREADS, 0, st>>>(tokens, tokens_ld, n, vocab, status);
+    return after_launch("token_check_kernel");
+}
+
 // Chunks of SORT_CHUNK tokens, each sorted by (key, position): a token's place is how many keys of its chunk are smaller, or
 // the same and in front of it.  A thread per token compares it with all of them, four at a time; what comes before and
 // behind the warp's own 32 tokens needs one comparison each.  (A bitonic network over chunks of 1024 takes 9 us.)
@@ -758,7 +779,7 @@ int db2k_embed(int dtype, const void *table, int64_t vocab, int64_t cols, int64_
     DB2_CHECK(index_dtype == DB2_I64 || index_dtype == DB2_I32, DB2_EUNSUPPORTED, "embed: tokens are int64 or int32");
     DB2_CHECK(vocab >= 0 && cols >= 0 && n >= 0, DB2_EINVAL, "embed: negative shape");
     if (n == 0 || cols == 0)
-        return DB2_OK;
+        return check_tokens("embed", index_dtype, tokens, tokens_ld, n, vocab, dev_status, as_stream(stream));
     DB2_CHECK((table || vocab == 0) && tokens && res, DB2_EINVAL, "embed: null operand");
     DB2_CHECK(ld_ok(table_ld, vocab, cols) && ld_ok(res_ld, n, cols) && ld_ok(tokens_ld, n, 1), DB2_EINVAL,
               "embed: a leading dimension is smaller than the number of columns");
@@ -805,7 +826,7 @@ int db2k_embed_grad(int dtype, const void *grad, int64_t grad_ld, int64_t n, int
     DB2_CHECK(n < ((int64_t)1 << 31) && vocab < ((int64_t)1 << 31) - 1, DB2_EUNSUPPORTED,
               "embedGrad: fewer than 2^31 tokens and table rows");
     if (vocab == 0 || cols == 0)
-        return DB2_OK;
+        return check_tokens("embedGrad", index_dtype, tokens, tokens_ld, n, vocab, dev_status, as_stream(stream));
     DB2_CHECK(res && ld_ok(res_ld, vocab, cols), DB2_EINVAL, "embedGrad: null result or a leading dimension too small");
     cudaStream_t st = as_stream(stream);
     if (n == 0) {
