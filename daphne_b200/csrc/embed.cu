@@ -745,6 +745,26 @@ DeviceOperand::DeviceOperand(db2_matrix *m) {
     ld = m->dev_ld;
 }
 
+int Results::add(const char *what, db2_matrix **slot, int dtype, int64_t rows, int64_t cols) {
+    if (!slot)
+        return DB2_OK;
+    for (int i = 0; i < n; i++)
+        DB2_CHECK(slot != slots[i] && (!*slot || *slot != *slots[i]), DB2_EINVAL, "%s: two results are to go to one matrix",
+                  what);
+    if (*slot)
+        DB2_TRY(check_result(*slot, dtype, rows, cols));
+    slots[n] = slot;
+    fresh[n++] = !*slot;
+    return DB2_OK;
+}
+Results::~Results() {
+    for (int i = 0; i < n && !is_done; i++)
+        if (fresh[i] && *slots[i]) {
+            db2_matrix_decref(*slots[i]);
+            *slots[i] = nullptr;
+        }
+}
+
 int prepare_update(db2_matrix *m) {
     DB2_TRY(ensure_device(m));
     if (!m->is_view && m->dev.use_count() > 1) {
@@ -881,12 +901,15 @@ int db2_embed(db2_context *ctx, db2_matrix **res, db2_matrix *table, db2_matrix 
     bind_device(ctx);
     const uint64_t before = g_launches.load();
     const DeviceOperand dt(table), di(tokens);
+    Results results;
+    DB2_TRY(results.add("embed", res, table->dtype, tokens->rows, table->cols));
     DB2_TRY(prepare_result(ctx, res, table->dtype, tokens->rows, table->cols));
     DB2_TRY(clear_status(ctx));
     DB2_TRY(db2k_embed(table->dtype, dt.ptr, table->rows, table->cols, dt.ld, tokens->dtype, di.ptr, di.ld, tokens->rows,
                        scale, (*res)->dev_ptr(), (*res)->dev_ld, ctx->dev_status + EMB_STATUS, ctx->stream));
     count(ctx, before);
-    return check_status(ctx, "embed", table->rows);
+    DB2_TRY(check_status(ctx, "embed", table->rows));
+    return results.done();
     DB2_API_END
 }
 
@@ -907,6 +930,7 @@ int db2_embedGrad(db2_context *ctx, db2_matrix **res, db2_matrix *grad, db2_matr
     bind_device(ctx);
     const uint64_t before = g_launches.load();
     const DeviceOperand dg(grad), di(tokens);
+    Results results;
     if (accumulate) {
         DB2_CHECK((*res)->dtype == res_dtype && (*res)->rows == vocab && (*res)->cols == grad->cols, DB2_EINVAL,
                   "embedGrad: the matrix to add to has shape (%lld x %lld) / type %d, expected (%lld x %lld) / type %d",
@@ -914,6 +938,7 @@ int db2_embedGrad(db2_context *ctx, db2_matrix **res, db2_matrix *grad, db2_matr
                   (long long)grad->cols, res_dtype);
         DB2_TRY(prepare_update(*res));
     } else {
+        DB2_TRY(results.add("embedGrad", res, res_dtype, vocab, grad->cols));
         DB2_TRY(prepare_result(ctx, res, res_dtype, vocab, grad->cols));
     }
     const size_t sb = db2k_embed_grad_scratch_bytes(grad->dtype, vocab, grad->cols, grad->rows);
@@ -924,7 +949,8 @@ int db2_embedGrad(db2_context *ctx, db2_matrix **res, db2_matrix *grad, db2_matr
                             res_dtype, (*res)->dev_ptr(), vocab, (*res)->dev_ld, accumulate, scratch,
                             ctx->scratch_bytes, ctx->dev_status + EMB_STATUS, ctx->stream));
     count(ctx, before);
-    return check_status(ctx, "embedGrad", vocab);
+    DB2_TRY(check_status(ctx, "embedGrad", vocab));
+    return results.done();
     DB2_API_END
 }
 

@@ -501,13 +501,8 @@ int sequences(db2_context *ctx, const char *what, const db2_matrix *g, db2_matri
 }
 // results that cover all rows: rows of no sequence keep what is there, so a fresh matrix starts as zeros
 int prepare_rows(db2_context *ctx, db2_matrix **res, const db2_matrix *g, bool all_rows) {
-    if (*res) {
-        DB2_CHECK((*res)->dtype == g->dtype && (*res)->rows == g->rows && (*res)->cols == g->cols, DB2_EINVAL,
-                  "pre-allocated result has shape (%lld x %lld) / type %d, expected (%lld x %lld) / type %d",
-                  (long long)(*res)->rows, (long long)(*res)->cols, (*res)->dtype, (long long)g->rows,
-                  (long long)g->cols, g->dtype);
+    if (*res)
         return prepare_update(*res);
-    }
     return db2_matrix_create(ctx, g->dtype, g->rows, g->cols, all_rows ? 0 : 1, res);
 }
 } // namespace
@@ -661,7 +656,9 @@ int db2_gatedScan(db2_context *ctx, int gate, db2_matrix **h, db2_matrix **last,
     int64_t seqs = 1;
     DB2_TRY(sequences(ctx, "gatedScan", g, offsets, &seqs));
     DB2_TRY(check_state("gatedScan", g, h0, seqs, "h0"));
-    DB2_CHECK(!last || !*last || *last != *h, DB2_EINVAL, "gatedScan: two results are to go to one matrix");
+    Results results;
+    DB2_TRY(results.add("gatedScan", h, g->dtype, g->rows, g->cols));
+    DB2_TRY(results.add("gatedScan", last, wide_dtype(g->dtype), seqs, g->cols));
     const uint64_t before = g_launches.load();
     const DeviceOperand dg(g), dx(x), doff(offsets), dh0(h0);
     DB2_CHECK(!offsets || doff.ld == 1 || seqs == 0, DB2_EUNSUPPORTED, "gatedScan: offsets are a strided view");
@@ -676,7 +673,7 @@ int db2_gatedScan(db2_context *ctx, int gate, db2_matrix **h, db2_matrix **last,
                             (*h)->dev_ld, last ? (*last)->dev_ptr() : nullptr, last ? (*last)->dev_ld : 0, scratch,
                             ctx->scratch_bytes, ctx->stream));
     count(ctx, before);
-    return DB2_OK;
+    return results.done();
     DB2_API_END
 }
 
@@ -695,10 +692,10 @@ int db2_gatedScanGrad(db2_context *ctx, int gate, db2_matrix **dg, db2_matrix **
     DB2_TRY(sequences(ctx, "gatedScanGrad", g, offsets, &seqs));
     DB2_TRY(check_state("gatedScanGrad", g, h0, seqs, "h0"));
     DB2_TRY(check_state("gatedScanGrad", g, grad_last, seqs, "grad_last"));
-    db2_matrix *slots[3] = {*dg, *dx, dh0 ? *dh0 : nullptr};
-    for (int i = 0; i < 3; i++)
-        for (int j = 0; j < i; j++)
-            DB2_CHECK(!slots[i] || slots[i] != slots[j], DB2_EINVAL, "gatedScanGrad: two results are to go to one matrix");
+    Results results;
+    DB2_TRY(results.add("gatedScanGrad", dg, g->dtype, g->rows, g->cols));
+    DB2_TRY(results.add("gatedScanGrad", dx, g->dtype, g->rows, g->cols));
+    DB2_TRY(results.add("gatedScanGrad", dh0, wide_dtype(g->dtype), seqs, g->cols));
     const uint64_t before = g_launches.load();
     const DeviceOperand og(g), ox(x), oh(h), od(grad), ooff(offsets), oh0(h0), ol(grad_last);
     DB2_CHECK(!offsets || ooff.ld == 1 || seqs == 0, DB2_EUNSUPPORTED, "gatedScanGrad: offsets are a strided view");
@@ -715,7 +712,7 @@ int db2_gatedScanGrad(db2_context *ctx, int gate, db2_matrix **dg, db2_matrix **
                                  dh0 ? (*dh0)->dev_ptr() : nullptr, dh0 ? (*dh0)->dev_ld : 0, scratch,
                                  ctx->scratch_bytes, ctx->stream));
     count(ctx, before);
-    return DB2_OK;
+    return results.done();
     DB2_API_END
 }
 
@@ -726,7 +723,9 @@ int db2_gatedStep(db2_context *ctx, int gate, db2_matrix **h, db2_matrix **new_s
     DB2_TRY(check_scan("gatedStep", g->dtype, gate, g->rows, g->cols, nullptr, 1));
     DB2_TRY(check_rows("gatedStep", g, x, "x"));
     DB2_TRY(check_state("gatedStep", g, state, g->rows, "state"));
-    DB2_CHECK(!*h || *h != *new_state, DB2_EINVAL, "gatedStep: two results are to go to one matrix");
+    Results results;
+    DB2_TRY(results.add("gatedStep", h, g->dtype, g->rows, g->cols));
+    DB2_TRY(results.add("gatedStep", new_state, wide_dtype(g->dtype), g->rows, g->cols));
     bind_device(ctx);
     const uint64_t before = g_launches.load();
     // a new state in the place of the old one is written where it is: each element is read before it is written
@@ -741,7 +740,7 @@ int db2_gatedStep(db2_context *ctx, int gate, db2_matrix **h, db2_matrix **new_s
     DB2_TRY(db2k_gated_step(g->dtype, gate, dg.ptr, dg.ld, dx.ptr, dx.ld, g->rows, g->cols, ds.ptr, ds.ld,
                             (*new_state)->dev_ptr(), (*new_state)->dev_ld, (*h)->dev_ptr(), (*h)->dev_ld, ctx->stream));
     count(ctx, before);
-    return DB2_OK;
+    return results.done();
     DB2_API_END
 }
 

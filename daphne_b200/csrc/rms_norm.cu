@@ -772,25 +772,28 @@ int norm_on_handles(db2_context *ctx, const char *what, db2_matrix **res, db2_ma
     DB2_CHECK(x->cols > 0 || x->rows == 0, DB2_EINVAL, "%s: rows without columns have no mean", what);
     DB2_TRY(check_operands(what, x, residual, "residual"));
     DB2_TRY(check_weight(what, x, weight));
-    db2_matrix *slots[4] = {*res, scales ? *scales : nullptr, sum ? *sum : nullptr, rstd ? *rstd : nullptr};
-    for (int i = 0; i < 4; i++)
-        for (int j = 0; j < i; j++)
-            DB2_CHECK(!slots[i] || slots[i] != slots[j], DB2_EINVAL, "%s: two results are to go to one matrix", what);
     DB2_CHECK(!scales || group == 0 || (group >= 16 && group <= 512 && (group & (group - 1)) == 0), DB2_EINVAL,
               "%s: groups of 16, 32, 64, 128, 256 or 512 columns, or 0 for the whole row (got %lld)", what,
               (long long)group);
     bind_device(ctx);
     const uint64_t before = g_launches.load();
+    Results results;
+    DB2_TRY(results.add(what, res, scales ? DB2_F8E4M3 : x->dtype, x->rows, x->cols));
+    DB2_TRY(results.add(what, scales, DB2_F32, x->rows, group ? (x->cols + group - 1) / group : 1));
+    DB2_TRY(results.add(what, sum, x->dtype, x->rows, x->cols));
+    DB2_TRY(results.add(what, rstd, wide_dtype(x->dtype), x->rows, 1));
     const DeviceOperand dx(x), dres(residual), dw(weight);
+    // (a buffer that others read as well is replaced)
+    DB2_CHECK(!rstd || !*rstd || x->rows <= 1 || !(*rstd)->dev || (*rstd)->dev_ld == 1 ||
+                  (!(*rstd)->is_view && (*rstd)->dev.use_count() > 1),
+              DB2_EUNSUPPORTED, "%s: rstd into a strided result view", what);
     DB2_TRY(prepare_result(ctx, res, scales ? DB2_F8E4M3 : x->dtype, x->rows, x->cols));
     if (scales)
         DB2_TRY(prepare_result(ctx, scales, DB2_F32, x->rows, group ? (x->cols + group - 1) / group : 1));
     if (sum)
         DB2_TRY(prepare_result(ctx, sum, x->dtype, x->rows, x->cols));
-    if (rstd) {
+    if (rstd)
         DB2_TRY(prepare_result(ctx, rstd, wide_dtype(x->dtype), x->rows, 1));
-        DB2_CHECK((*rstd)->dev_ld == 1 || x->rows <= 1, DB2_EUNSUPPORTED, "%s: rstd into a strided result view", what);
-    }
     if (x->rows > 0) {
         void *sp = sum ? (*sum)->dev_ptr() : nullptr, *tp = rstd ? (*rstd)->dev_ptr() : nullptr;
         const int64_t sld = sum ? (*sum)->dev_ld : 0;
@@ -803,7 +806,7 @@ int norm_on_handles(db2_context *ctx, const char *what, db2_matrix **res, db2_ma
                                   (*res)->dev_ptr(), (*res)->dev_ld, tp, ctx->stream));
     }
     count(ctx, before);
-    return DB2_OK;
+    return results.done();
 }
 
 } // namespace
@@ -945,12 +948,13 @@ int db2_rmsNormGrad(db2_context *ctx, db2_matrix **dx, db2_matrix **dweight, db2
     DB2_TRY(check_weight("rmsNormGrad", grad, weight));
     DB2_CHECK(rstd->dtype == wide_dtype(grad->dtype) && rstd->rows == grad->rows && rstd->cols == 1, DB2_EINVAL,
               "rmsNormGrad: rstd must be the column matrix that rmsNorm gave");
-    DB2_CHECK(!dweight || !*dweight || *dweight != *dx, DB2_EINVAL,
-              "rmsNormGrad: two results are to go to one matrix");
     bind_device(ctx);
     const uint64_t before = g_launches.load();
     const DeviceOperand dg(grad), ds(sum), dw(weight), dr(rstd), dd(dsum);
     DB2_CHECK(dr.ld == 1 || grad->rows <= 1, DB2_EUNSUPPORTED, "rmsNormGrad: rstd is a strided view");
+    Results results;
+    DB2_TRY(results.add("rmsNormGrad", dx, grad->dtype, grad->rows, grad->cols));
+    DB2_TRY(results.add("rmsNormGrad", dweight, wide_dtype(grad->dtype), 1, grad->cols));
     DB2_TRY(prepare_result(ctx, dx, grad->dtype, grad->rows, grad->cols));
     if (dweight)
         DB2_TRY(prepare_result(ctx, dweight, wide_dtype(grad->dtype), 1, grad->cols));
@@ -961,7 +965,7 @@ int db2_rmsNormGrad(db2_context *ctx, db2_matrix **dx, db2_matrix **dweight, db2
                                dd.ld, (*dx)->dev_ptr(), (*dx)->dev_ld, dweight ? (*dweight)->dev_ptr() : nullptr,
                                scratch, ctx->scratch_bytes, ctx->stream));
     count(ctx, before);
-    return DB2_OK;
+    return results.done();
     DB2_API_END
 }
 

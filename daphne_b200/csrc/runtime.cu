@@ -178,14 +178,19 @@ int ensure_device(db2_matrix *m) {
     return DB2_OK;
 }
 
+int check_result(const db2_matrix *r, int dtype, int64_t rows, int64_t cols) {
+    DB2_CHECK(r->dtype == dtype && r->rows == rows && r->cols == cols, DB2_EINVAL,
+              "pre-allocated result has shape (%lld x %lld) / type %d, expected (%lld x %lld) / type %d",
+              (long long)r->rows, (long long)r->cols, r->dtype, (long long)rows, (long long)cols, dtype);
+    return DB2_OK;
+}
+
 int prepare_result(db2_context *ctx, db2_matrix **res, int dtype, int64_t rows, int64_t cols) {
     DB2_CHECK(res, DB2_EINVAL, "null result slot");
     if (*res == nullptr)
         return db2_matrix_create(ctx, dtype, rows, cols, 0, res);
     db2_matrix *r = *res;
-    DB2_CHECK(r->dtype == dtype && r->rows == rows && r->cols == cols, DB2_EINVAL,
-              "pre-allocated result has shape (%lld x %lld) / type %d, expected (%lld x %lld) / type %d",
-              (long long)r->rows, (long long)r->cols, r->dtype, (long long)rows, (long long)cols, dtype);
+    DB2_TRY(check_result(r, dtype, rows, cols));
     if (r->deferred()) {
         lazy_forget(r);
         r->lazy.reset();

@@ -274,6 +274,8 @@ int nccl_allreduce_group(const std::vector<db2_context *> &ctxs, const std::vect
 int ensure_device(db2_matrix *m);
 // result allocation following the reference's "*res == nullptr means allocate" convention; checks shape/type otherwise
 int prepare_result(db2_context *ctx, db2_matrix **res, int dtype, int64_t rows, int64_t cols);
+// whether r can be the result: the shape and type that prepare_result asks for
+int check_result(const db2_matrix *r, int dtype, int64_t rows, int64_t cols);
 // A device-resident operand (or none, for a null handle) that keeps its buffer: a result that is prepared afterwards and
 // names the same matrix gets a buffer of its own instead of the operand's values.  Views are written in place.
 struct DeviceOperand {
@@ -281,6 +283,26 @@ struct DeviceOperand {
     const void *ptr = nullptr;
     int64_t ld = 0;
     explicit DeviceOperand(db2_matrix *m); // throws Error (embed.cu)
+};
+// The results of one call, checked together before the first of them is prepared: a call that is refused leaves all of them
+// as they were.  Slots that held no matrix hold none again unless the call says that it is done.
+class Results {
+  public:
+    // the slot of a result that is not wanted is null
+    int add(const char *what, db2_matrix **slot, int dtype, int64_t rows, int64_t cols);
+    int done() {
+        is_done = true;
+        return DB2_OK;
+    }
+    Results() = default;
+    Results(const Results &) = delete;
+    ~Results();
+
+  private:
+    db2_matrix **slots[4] = {};
+    bool fresh[4] = {};
+    int n = 0;
+    bool is_done = false;
 };
 // makes m the target of an update in place: current on the device, in a buffer that no other handle reads (embed.cu)
 int prepare_update(db2_matrix *m);

@@ -494,7 +494,10 @@ int db2_randMatrix(db2_context *ctx, db2_matrix **res, int dtype, int64_t rows, 
 int db2_castObj(db2_context *ctx, db2_matrix **res, db2_matrix *arg, int dtype);
 /* Operators on sequences of tokens: db2k_embed, db2k_embed_grad (see there) on handles.  tokens: column matrix of int64
  * or int32.  A token outside the table that is not -1 is DB2_EDOMAIN; to say so the calls wait for the device (the
- * db2k_ forms do not).  embedGrad with accumulate adds to *res, which must be given. */
+ * db2k_ forms do not); a given result then holds what the db2k_ form leaves in it.  embedGrad with accumulate adds to *res,
+ * which must be given.
+ * Of these operators as a whole: a call that is refused for the shape, type or slot of a result leaves all results as they
+ * were, and a call that fails leaves no matrix in a slot that held none. */
 int db2_embed(db2_context *ctx, db2_matrix **res, db2_matrix *table, db2_matrix *tokens, double scale);
 int db2_embedGrad(db2_context *ctx, db2_matrix **res, db2_matrix *grad, db2_matrix *tokens, int64_t vocab, double scale,
                   int res_dtype, int accumulate);

@@ -87,3 +87,78 @@ def test_token_status_on_pointers_where_nothing_is_computed(index):
             check(lib.db2k_embed_grad(names.F32, p, cols, n, cols, code, tok.data_ptr(), 2, 1.0, names.F32, p, vocab, cols, 0,
                                       None, 0, st.data_ptr() + 4, stream()))
             assert st.tolist() == [exp, exp], (n, vocab, cols)
+
+
+def _calls(ctx, k):
+    """(The operands, to be kept; every operator with several results: the names of its slots, a call with their values.)"""
+    rng = np.random.default_rng(7)
+    n, c = 40, 6
+    M = lambda r, q=c, t=np.float32: k.DenseMatrix.from_numpy(ctx, rng.standard_normal((r, q)).astype(t))  # noqa: E731
+    d, s = int(k.Gate.DECAY), ctx.handle
+    off = k.DenseMatrix.from_numpy(ctx, np.array([[0], [15], [40]]))
+    x, r, w, v, st, g, last = M(n), M(n), M(1), M(n, 1), M(2), M(n), M(2)
+    state = M(n)
+    ref = C.byref
+    return [x, r, w, v, st, g, last, state, off], {
+        "rmsNorm": (["res", "sum", "rstd"], lambda a, b, e: lib.db2_rmsNorm(s, ref(a), ref(b), ref(e), x.handle, r.handle, w.handle, 1e-6)),
+        "rmsNormQ8": (["res", "scales", "sum", "rstd"], lambda a, b, e, f: lib.db2_rmsNormQ8(
+            s, ref(a), ref(b), ref(e), ref(f), x.handle, r.handle, w.handle, 1e-6, 16)),
+        "rmsNormGrad": (["dx", "dweight"], lambda a, b: lib.db2_rmsNormGrad(s, ref(a), ref(b), x.handle, r.handle, w.handle, v.handle, None)),
+        "gatedScan": (["h", "last"], lambda a, b: lib.db2_gatedScan(s, d, ref(a), ref(b), g.handle, x.handle, off.handle, st.handle)),
+        "gatedScanGrad": (["dg", "dx", "dh0"], lambda a, b, e: lib.db2_gatedScanGrad(
+            s, d, ref(a), ref(b), ref(e), g.handle, x.handle, r.handle, x.handle, off.handle, st.handle, last.handle)),
+        "gatedStep": (["h", "new_state"], lambda a, b: lib.db2_gatedStep(s, d, ref(a), ref(b), g.handle, x.handle, state.handle)),
+    }
+
+
+@gpu
+@pytest.mark.parametrize("name", ["rmsNorm", "rmsNormQ8", "rmsNormGrad", "gatedScan", "gatedScanGrad", "gatedStep"])
+def test_a_refused_result_leaves_the_others_as_they_were(ctx, name):
+    """Each result in turn has the wrong shape: no other slot is touched, also not one that
+    names an operand whose values lie on the host only, and nothing is made."""
+    import daphne_b200.kernels as k
+    keep, calls = _calls(ctx, k)
+    slots, call = calls[name]
+    assert call(*[C.c_void_p() for _ in slots]) == 0
+    for wrong in range(len(slots)):
+        bad = k.fill(ctx, 7.0, 3, 3, dtype=np.float32)
+        for over in range(len(slots)):  # which other slot holds a given matrix, whose values have to stay
+            given = [C.c_void_p() for _ in slots]
+            given[wrong] = C.c_void_p(bad.handle.value)
+            own = None
+            if over != wrong and slots[over] in ("res", "sum", "dx", "h", "dg", "new_state") and (name, slots[over]) != ("rmsNormQ8", "res"):
+                own = k.DenseMatrix.from_numpy(ctx, np.full((40, 6), 3.0, dtype=np.float32))
+                given[over] = C.c_void_p(own.handle.value)
+            before = [h.value for h in given]
+            assert call(*given) == 1, (slots[wrong], over)
+            assert [h.value for h in given] == before, (slots[wrong], over)
+            assert (bad.to_numpy() == 7).all()
+            if own is not None:
+                assert (own.to_numpy() == 3).all(), (slots[wrong], slots[over])
+
+
+@gpu
+@pytest.mark.parametrize("name", ["rmsNorm", "rmsNormQ8", "rmsNormGrad", "gatedScan", "gatedScanGrad", "gatedStep"])
+def test_one_slot_for_two_results_is_refused(ctx, name):
+    import daphne_b200.kernels as k
+    keep, calls = _calls(ctx, k)
+    slots, call = calls[name]
+    for i in range(len(slots)):
+        for j in range(i):
+            given = [C.c_void_p() for _ in slots]
+            given[i] = given[j]
+            assert call(*given) == 1 and all(h.value is None for h in given), (slots[i], slots[j])
+
+
+@gpu
+def test_a_token_outside_the_table_leaves_no_result_behind(ctx):
+    import daphne_b200.kernels as k
+    x = k.DenseMatrix.from_numpy(ctx, np.ones((4, 3)))
+    tok = k.DenseMatrix.from_numpy(ctx, np.array([[0], [4], [1], [2]]))
+    for call in (lambda h: lib.db2_embed(ctx.handle, C.byref(h), x.handle, tok.handle, 1.0),
+                 lambda h: lib.db2_embedGrad(ctx.handle, C.byref(h), x.handle, tok.handle, 4, 1.0, x.dtype_code, 0)):
+        h = C.c_void_p()
+        assert call(h) == 5 and h.value is None
+        given = k.fill(ctx, 2.0, 4, 3)
+        h = C.c_void_p(given.handle.value)
+        assert call(h) == 5 and h.value == given.handle.value
