@@ -489,7 +489,8 @@ int db2_castObj(db2_context *ctx, db2_matrix **res, db2_matrix *arg, int dtype) 
     DB2_CAST(DB2_I64, int64_t, DB2_I64, int64_t)
     DB2_CAST(DB2_U64, uint64_t, DB2_U64, uint64_t)
 #undef DB2_CAST
-// 16-bit and 8-bit floating point from and to double and float: one rounding to nearest even
+// 16-bit floating point from and to double, float and each other, 8-bit floating point to all of them: one rounding to
+// nearest even
 #define DB2_CAST_SEQ(FROM_CODE, FROM_T, TO_CODE, TO_T)                                                                 \
     if (arg->dtype == FROM_CODE && dtype == TO_CODE) {                                                                 \
         cast_seq_kernel<TO_T, FROM_T><<<grid, 256, 0, ctx->stream>>>(static_cast<const FROM_T *>(arg->dev_ptr()),      \
@@ -509,6 +510,12 @@ int db2_castObj(db2_context *ctx, db2_matrix **res, db2_matrix *arg, int dtype) 
     DB2_CAST_SEQ(DB2_BF16, __nv_bfloat16, DB2_F32, float)
     DB2_CAST_SEQ(DB2_F8E4M3, __nv_fp8_e4m3, DB2_F64, double)
     DB2_CAST_SEQ(DB2_F8E4M3, __nv_fp8_e4m3, DB2_F32, float)
+    DB2_CAST_SEQ(DB2_F8E4M3, __nv_fp8_e4m3, DB2_F16, __half)
+    DB2_CAST_SEQ(DB2_F8E4M3, __nv_fp8_e4m3, DB2_BF16, __nv_bfloat16)
+    DB2_CAST_SEQ(DB2_F16, __half, DB2_BF16, __nv_bfloat16)
+    DB2_CAST_SEQ(DB2_BF16, __nv_bfloat16, DB2_F16, __half)
+    DB2_CAST_SEQ(DB2_F16, __half, DB2_F16, __half)
+    DB2_CAST_SEQ(DB2_BF16, __nv_bfloat16, DB2_BF16, __nv_bfloat16)
 #undef DB2_CAST_SEQ
     return set_error(DB2_EUNSUPPORTED, "castObj from value type %d to %d", arg->dtype, dtype);
     DB2_API_END

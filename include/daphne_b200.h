@@ -489,8 +489,8 @@ int db2_sliceCol(db2_context *ctx, db2_matrix **res, db2_matrix *arg, int64_t lo
  * of `dtype`.  Replaces RandMatrix<DenseMatrix<VT>, VT> (src/runtime/local/kernels/RandMatrix.h:82-161). */
 int db2_randMatrix(db2_context *ctx, db2_matrix **res, int dtype, int64_t rows, int64_t cols, const void *min,
                    const void *max, double sparsity, int64_t seed);
-/* value-type cast between f64 / i64 / u64 (CastObj, used for idxMin results feeding ctable), f64 / f32, and from and to
- * the 16-bit floating-point types (from DB2_F8E4M3 only) */
+/* value-type cast between f64 / i64 / u64 (CastObj, used for idxMin results feeding ctable), f64 / f32, between f64, f32 and the
+ * 16-bit floating-point types, and from DB2_F8E4M3 to those four */
 int db2_castObj(db2_context *ctx, db2_matrix **res, db2_matrix *arg, int dtype);
 /* Operators on sequences of tokens: db2k_embed, db2k_embed_grad (see there) on handles.  tokens: column matrix of int64
  * or int32.  A token outside the table that is not -1 is DB2_EDOMAIN; to say so the calls wait for the device (the

@@ -104,3 +104,24 @@ def test_sigmoid_is_as_accurate_for_large_arguments_as_for_small_ones(tname):
     assert (f[:5] >= 2.0 ** -125).all() and (f[:5] <= 2.0 ** -124).all() and (o[:5] == 1).all()
     assert (f[5:10] == 1).all() and (o[5:10] <= 2.0 ** -125).all() and (o[5:10] >= 0).all()
     assert np.isnan(f[10]) and np.isnan(o[10])
+
+
+@gpu
+@pytest.mark.parametrize("src", ["float16", "bfloat16", "float8_e4m3"])
+@pytest.mark.parametrize("dst", ["float16", "bfloat16"])
+def test_casts_between_the_short_types(ctx, src, dst):
+    """Every bit pattern of the source, rounded once to nearest even; a cast to the type itself is a copy."""
+    import daphne_b200.kernels as k
+    t = {"float16": torch.float16, "bfloat16": torch.bfloat16, "float8_e4m3": torch.float8_e4m3fn}
+    code = {"float16": np.float16, "bfloat16": k.BFLOAT16, "float8_e4m3": k.FLOAT8_E4M3}
+    bits = torch.arange(256 if src == "float8_e4m3" else 65536).to(torch.uint8 if src == "float8_e4m3" else torch.int32)
+    bits = bits.view(-1, 64) if src == "float8_e4m3" else bits.to(torch.int16).view(-1, 64)
+    d = bits.cuda()
+    m = k.DenseMatrix.wrap_device(ctx, d.data_ptr(), d.shape[0], 64, 64, code[src], keep=d)
+    torch.cuda.synchronize()
+    got = k.castObj(k.sliceCol(m, 1, 64), code[dst]).to_numpy().view(np.int16)
+    x = bits[:, 1:].contiguous().view(t[src])
+    exp = x.to(t[dst])
+    nan = x.float().isnan()
+    assert torch.equal(torch.as_tensor(got.copy())[~nan], exp.view(torch.int16)[~nan])
+    assert bool(torch.as_tensor(got.copy()).view(t[dst]).float()[nan].isnan().all())
