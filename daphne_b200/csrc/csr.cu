@@ -11,6 +11,7 @@
 #include "fused_step.cuh"
 #include "runtime.h"
 
+#include <algorithm>
 
 struct db2_csr {
     std::atomic<int> refs{1};
@@ -570,7 +571,30 @@ static int csr_ensure_device(db2_csr *m) {
     return DB2_OK;
 }
 
+// products that wait to be computed, of all contexts
+static std::mutex waiting_mu;
+static std::vector<db2_csr *> &waiting = *new std::vector<db2_csr *>; // (handles may outlive the library's statics)
+
+int csr_settle(const db2_matrix *m) {
+    for (;;) {
+        db2_csr *next = nullptr;
+        {
+            std::lock_guard<std::mutex> lock(waiting_mu);
+            for (db2_csr *c : waiting)
+                if (c->lazy_rhs == m || (m->dev && c->lazy_rhs->dev == m->dev))
+                    next = c;
+        }
+        if (!next)
+            return DB2_OK;
+        DB2_TRY(csr_ensure_device(next));
+    }
+}
+
 static void drop_lazy(db2_csr *m) {
+    if (m->lazy_lhs) {
+        std::lock_guard<std::mutex> lock(waiting_mu);
+        waiting.erase(std::remove(waiting.begin(), waiting.end(), m), waiting.end());
+    }
     if (m->lazy_lhs) {
         db2_csr_decref(m->lazy_lhs);
         m->lazy_lhs = nullptr;
@@ -777,6 +801,9 @@ int db2_ewMulCsrDense(db2_context *ctx, db2_csr **res, db2_csr *lhs, db2_matrix 
     db2_matrix_incref(rhs);
     if (ctx->eager) {
         DB2_TRY(csr_ensure_device(m.get()));
+    } else {
+        std::lock_guard<std::mutex> lock(waiting_mu);
+        waiting.push_back(m.get());
     }
     *res = m.release();
     return DB2_OK;

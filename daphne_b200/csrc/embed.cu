@@ -767,6 +767,7 @@ Results::~Results() {
 
 int prepare_update(db2_matrix *m) {
     DB2_TRY(ensure_device(m));
+    DB2_TRY(lazy_settle(m));
     if (!m->is_view && m->dev.use_count() > 1) {
         // other handles read the buffer: the update goes to a copy
         auto fresh = make_devbuf(m->ctx, (size_t)m->rows * m->cols * m->esize());

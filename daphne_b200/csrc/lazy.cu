@@ -540,6 +540,38 @@ int lazy_force(db2_matrix *m) {
     return rc;
 }
 
+static bool reads(const Expr &e, const DevBuf *b) {
+    if (e.base.buf.get() == b || (e.gemm && (e.gemm->A.buf.get() == b || e.gemm->B.buf.get() == b)))
+        return true;
+    for (const ExprStep &s : e.steps)
+        if (s.operand.buf.get() == b)
+            return true;
+    return false;
+}
+
+int lazy_settle(db2_matrix *m) {
+    DB2_TRY(csr_settle(m));
+    // (chains hold buffers: a matrix that is no view moves to another buffer instead)
+    if (!m->is_view || !m->dev || m->dev.use_count() == 1)
+        return DB2_OK;
+    db2_context *ctx = m->ctx;
+    const DevBuf *b = m->dev.get();
+    if (ctx->syrk_waiting && ctx->syrk_waiting->syrk_of && ctx->syrk_waiting->syrk_of->buf.get() == b)
+        DB2_TRY(lazy_force(ctx->syrk_waiting));
+    for (;;) { // one at a time: a pass may serve several of them
+        db2_matrix *next = nullptr;
+        for (db2_matrix *p : ctx->pending)
+            if (!next && reads(*p->pend_src, b))
+                next = p;
+        for (db2_matrix *l : ctx->lazies)
+            if (!next && reads(*l->lazy, b))
+                next = l;
+        if (!next)
+            return DB2_OK;
+        DB2_TRY(lazy_force(next));
+    }
+}
+
 int lazy_flush_all(db2_context *ctx) {
     while (!ctx->pending.empty())
         DB2_TRY(lazy_force(ctx->pending.front()));

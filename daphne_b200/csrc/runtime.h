@@ -264,6 +264,9 @@ int lazy_try_agg_all_start(db2_context *ctx, int op, double *pinned, db2_matrix 
 int lazy_force(db2_matrix *m);          // materialises a deferred matrix (and the pending siblings it can serve)
 int lazy_flush_all(db2_context *ctx);   // produces every pending aggregation
 void lazy_forget(db2_matrix *m);        // a deferred matrix is being destroyed
+// m is about to be updated in place: what has been asked for before and would still read its old values is computed now
+int lazy_settle(db2_matrix *m);
+int csr_settle(const db2_matrix *m); // the same for deferred products of CSR matrices with m (csr.cu)
 
 // device groups (comm.cu): NCCL communicators for the contexts of one process, grouped all-reduce
 int nccl_init_group(const std::vector<db2_context *> &ctxs);

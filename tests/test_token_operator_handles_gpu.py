@@ -162,3 +162,113 @@ def test_a_token_outside_the_table_leaves_no_result_behind(ctx):
         given = k.fill(ctx, 2.0, 4, 3)
         h = C.c_void_p(given.handle.value)
         assert call(h) == 5 and h.value == given.handle.value
+
+
+@gpu
+def test_updates_through_a_view_leave_earlier_results_alone(ctx):
+    """What was asked for before an update in place has the values of that time, also where it is computed later: chains,
+    row aggregations, products of the whole matrix and of other views of it."""
+    import daphne_b200.kernels as k
+    rng = np.random.default_rng(3)
+    p, g, x = (rng.integers(-4, 5, s).astype(np.float64) for s in ((600, 300), (260, 300), (260, 300)))
+    tok = rng.integers(0, 260, (50, 1))
+    dy = rng.integers(-4, 5, (50, 300)).astype(np.float64)
+    M = lambda a: k.DenseMatrix.from_numpy(ctx, a)  # noqa: E731
+    for update in ("step", "table gradient"):
+        P = M(p)
+        P.device_ptr()
+        v, other = k.sliceRow(P, 20, 280), k.sliceRow(P, 100, 500)
+        twice, less = k.ewBinaryObjSca(k.BinaryOpCode.MUL, P, 2.0), k.ewBinaryMat(k.BinaryOpCode.SUB, other, M(p[100:500]))
+        plus = k.ewBinaryMat(k.BinaryOpCode.ADD, M(p * 3), P)
+        rows, gram = k.aggRow(k.AggOpCode.SUM, k.ewUnaryMat(k.UnaryOpCode.ABS, P)), k.syrk(P)
+        new = p.copy()
+        if update == "step":
+            k.gatedStep(k.Gate.DECAY, M(g), M(x), v)
+            new[20:280] = g * p[20:280] + x
+        else:
+            k.embedGrad(M(dy), M(tok), 260, add_to=v)
+            np.add.at(new, 20 + tok[:, 0], dy)
+        assert np.array_equal(P.to_numpy(), new) and np.array_equal(v.to_numpy(), new[20:280])
+        assert np.array_equal(twice.to_numpy(), 2 * p) and not less.to_numpy().any() and np.array_equal(plus.to_numpy(), 4 * p)
+        assert np.array_equal(rows.to_numpy()[:, 0], np.abs(p).sum(1)) and np.array_equal(gram.to_numpy(), p.T @ p)
+        assert np.array_equal(k.ewBinaryObjSca(k.BinaryOpCode.MUL, P, 2.0).to_numpy(), 2 * new)
+
+
+@gpu
+def test_updates_leave_earlier_sparse_products_alone(ctx):
+    """A deferred product of a CSR matrix with a dense one has the dense one's values of the time it was asked for."""
+    import daphne_b200.kernels as k
+    val, col, off = np.ones(6), np.array([0, 2, 1, 0, 1, 2], dtype=np.uint64), np.array([0, 2, 3, 6], dtype=np.uint64)
+    full = np.array([[1.0, 0, 1], [0, 1, 0], [1, 1, 1]])
+    w, g, x = np.array([[2.0, 3.0, 5.0]]), np.array([[4.0, 4.0, 4.0]]), np.array([[1.0, 1.0, 1.0]])
+    M = lambda a: k.DenseMatrix.from_numpy(ctx, a)  # noqa: E731
+    for part in (False, True):
+        W = M(np.vstack([w, w]) if part else w)
+        W.device_ptr()
+        v = k.sliceRow(W, 0, 1) if part else W
+        G = k.CSRMatrix.from_arrays(ctx, 3, 3, val, col, off)
+        prod = k.ewMulCsrDense(G, v)
+        k.gatedStep(k.Gate.DECAY, M(g), M(x), v)
+        assert np.array_equal(v.to_numpy(), g * w + x)
+        assert np.array_equal(k.aggRowCsr(k.AggOpCode.SUM, prod).to_numpy()[:, 0], (full * w).sum(1))
+
+
+@gpu
+def test_updates_leave_a_product_of_a_tall_matrix_with_itself_alone(ctx):
+    import daphne_b200.kernels as k
+    p = np.random.default_rng(5).integers(-3, 4, (1 << 16, 64)).astype(np.float64)
+    P = k.DenseMatrix.from_numpy(ctx, p)
+    P.device_ptr()
+    v, gram = k.sliceRow(P, 100, 200), k.syrk(P)
+    k.gatedStep(k.Gate.DECAY, k.fill(ctx, 2.0, 100, 64), k.fill(ctx, 1.0, 100, 64), v)
+    assert np.array_equal(gram.to_numpy(), p.T @ p) and np.array_equal(v.to_numpy(), 2 * p[100:200] + 1)
+
+
+@gpu
+def test_operands_that_are_deferred_and_results_that_name_them(ctx):
+    """Chains that are not computed yet as operands, and results in the operand's own handle."""
+    import daphne_b200.kernels as k
+    rng = np.random.default_rng(4)
+    r, c = SHAPE
+    a, b = rng.standard_normal(SHAPE), rng.standard_normal(SHAPE)
+    off = np.array([[0], [100], [260]])
+    M = lambda m: k.DenseMatrix.from_numpy(ctx, m)  # noqa: E731
+    twice = lambda m: k.ewBinaryObjSca(k.BinaryOpCode.MUL, M(m), 2.0)  # noqa: E731
+    s, d, ref = ctx.handle, int(k.Gate.DECAY), C.byref
+    tok = rng.integers(0, r, (r, 1))
+    w, h0 = rng.standard_normal((1, c)), rng.standard_normal((2, c))
+    W, H0, OFF, T = M(w), M(h0), M(off), M(tok)
+    none = lambda: C.c_void_p()  # noqa: E731
+    calls = {
+        "embed": (1, lambda o, x, y: lib.db2_embed(s, ref(o[0]), x.handle, T.handle, 1.0)),
+        "embedGrad": (1, lambda o, x, y: lib.db2_embedGrad(s, ref(o[0]), x.handle, T.handle, r, 1.0, 0, 0)),
+        "rmsNorm": (3, lambda o, x, y: lib.db2_rmsNorm(s, ref(o[0]), ref(o[1]), ref(o[2]), x.handle, y.handle, W.handle, 1e-6)),
+        "rmsNormGrad": (2, lambda o, x, y: lib.db2_rmsNormGrad(s, ref(o[0]), ref(o[1]), x.handle, y.handle, W.handle, V.handle, x.handle)),
+        "gatedScan": (2, lambda o, x, y: lib.db2_gatedScan(s, d, ref(o[0]), ref(o[1]), x.handle, y.handle, OFF.handle, H0.handle)),
+        "gatedScanGrad": (3, lambda o, x, y: lib.db2_gatedScanGrad(s, d, ref(o[0]), ref(o[1]), ref(o[2]), x.handle, y.handle, y.handle,
+                                                                 x.handle, OFF.handle, H0.handle, H0.handle)),
+        "gatedStep": (2, lambda o, x, y: lib.db2_gatedStep(s, d, ref(o[0]), ref(o[1]), x.handle, y.handle, x.handle)),
+    }
+    V = M(np.abs(rng.standard_normal((r, 1))))
+    for name, (n, call) in calls.items():
+        def run(slots, x, y):
+            check(call(slots, x, y))
+            return [k.DenseMatrix(ctx, o).to_numpy() if own is None else own.to_numpy() for o, own in zip(slots, owners)]
+        owners = [None] * n
+        exp = run([none() for _ in range(n)], M(2 * a), M(2 * b))
+        assert all(np.isfinite(e).all() for e in exp)
+        got = run([none() for _ in range(n)], twice(a), twice(b))
+        assert all(np.array_equal(e, q) for e, q in zip(exp, got)), name
+        for i, e in enumerate(exp):  # every result of that shape in the place of either operand
+            if e.shape != SHAPE:
+                continue
+            for which in (0, 1):
+                x, y = twice(a), twice(b)
+                keep = [k.ewBinaryObjSca(k.BinaryOpCode.ADD, m, 1.0) for m in (x, y)]
+                owners = [None] * n
+                owners[i] = (x, y)[which]
+                slots = [none() for _ in range(n)]
+                slots[i] = C.c_void_p(owners[i].handle.value)
+                got = run(slots, x, y)
+                assert all(np.array_equal(p, q) for p, q in zip(exp, got)), (name, i, which)
+                assert np.array_equal(keep[0].to_numpy(), 2 * a + 1) and np.array_equal(keep[1].to_numpy(), 2 * b + 1), (name, i, which)
