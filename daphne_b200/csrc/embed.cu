@@ -96,13 +96,16 @@ int embed_launch(const void *table, int64_t vocab, int64_t cols, int64_t table_l
 // `vocab`, behind all others.
 
 constexpr int SORT_CHUNK = 512;            // tokens that a CTA sorts by itself
-constexpr int MERGE_MAX = 80 * SORT_CHUNK; // tokens that are merged in one go: their sorted chunks lie in shared memory
+// Tokens that are merged in one go: their sorted chunks lie in shared memory.  Every CTA reads all keys and searches every
+// chunk, so merging grows with the square of the tokens, the radix passes hardly: 16384 tokens of 128256 take 33 us merged
+// (whole gradient, 8 columns) and 63 by radix, 28672 take 58 and 65, 40960 take 71 and 69, 49152 take 82 and 67 to 70.
+constexpr int MERGE_MAX = 80 * SORT_CHUNK;
 constexpr int MERGE_THREADS = 512, MERGE_ROUND = MERGE_THREADS / 8; // of a CTA; tokens that eight lanes each share
 // chunks lie one word apart from multiples of the 32 banks: lanes at the same step of their searches do not collide
 constexpr int MERGE_PITCH = SORT_CHUNK + 1;
 
-// The table's rows, which become zero before the sums are written: the sorting kernels, which keep
-// few SMs busy, do it with further CTAs.  A CTA writes 128 packets of a row at a time.
+// The table's rows, which become zero before the sums are written: further CTAs of the kernel that sorts chunks, which keeps
+// few SMs busy, do it, or a kernel in front of the radix passes.  A CTA writes 128 packets of a row at a time.
 struct Zeros {
     char *at;
     int64_t rows, row_bytes, ld_bytes;
@@ -413,7 +416,8 @@ struct SumArgs {
 // where the token changes, the sum is finished -- written to the table when all its rows lie in the run, to `part`
 // otherwise: part[run][0] holds the sum of a token that came over from the run before, part[run][1] that of a token that
 // starts in the run and goes on behind it.  Equal amounts of work whatever the tokens' frequencies.
-// Bound by memory: every gradient row is read once, every table row written once.
+// Bound by memory: every gradient row is read once, every row of a token that occurs written once here (and once before,
+// when the table was cleared).
 template <typename T, typename R, int N, bool ADD>
 __global__ void __launch_bounds__(SUM_THREADS)
     embed_sum_kernel(SumArgs a, const T *__restrict__ grad, wide_t<T> scale, R *__restrict__ res,

@@ -13,7 +13,9 @@
 // value that really enters them.  So each operand is read once and each result written once.
 //
 // Bound by memory.  States, gates and products are float (double for double); the stored h is rounded once, the running
-// state never.
+// state never.  The gradient reads h as it was stored, which is what a caller has: where a rounded h enters dg = delta *
+// h[t-1], dg is off by 1.85e-3 of its size in bf16, with the state of the forward pass it would be by the 1.66e-3 that its
+// own rounding costs.
 #include "runtime.h"
 #include "seq.cuh"
 
@@ -66,7 +68,7 @@ __device__ __forceinline__ void gate_pair(float g, float *f, float *o) {
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(c) : "f"(g), "f"(-86.6433945f));
     asm("min.NaN.f32 %0, %1, %2;" : "=f"(c) : "f"(c), "f"(128.0f));
     const float t = c * -1.44269504f;
-    // ln 2 in two parts
+    // ln 2 in two parts, as in Cody and Waite's reduction of arguments
     const float lost = fmaf(t, 1.90465421e-9f, fmaf(t, -0.693147182f, -c));
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t));
     e = fmaf(e, lost, e);
@@ -100,8 +102,9 @@ template <typename W, int VEC> __device__ __forceinline__ void put(Steps<W, VEC>
 // CTA (sequence, strip of 32 x VEC columns, block of rows).  AGGREGATE: only (A, B) of the block, into part.  Otherwise the
 // results; the state that enters a block is init, advanced by part of the blocks in front of it.
 // Registers: three CTAs of four warps, or one of eight, on an SM.  With 128 registers a thread, four CTAs fit, but the
-// loads of a tile no longer stand together in front of their uses: 30000 x 2560 f16 in 37 sequences takes 135 us instead
-// of 105, 8 x 4096 x 2048 bf16 (forward and backward, eight warps) 385 instead of 266.
+// loads of a tile no longer stand together in front of their uses: 30000 x 2560 f16 in 37 sequences took 135 us instead
+// of 105, 8 x 4096 x 2048 bf16 (forward and backward, eight warps) 385 instead of 266 (before the sigmoid's correction, with
+// which they take 115 to 125 and 272).
 template <typename T, int VEC, int WARPS, bool BACK, bool SIGMOID, bool AGGREGATE>
 __global__ void __launch_bounds__(WARPS * 32, WARPS == 4 ? 3 : 1) gated_scan_kernel(ScanArgs<T> a) {
     using W = wide_t<T>;
@@ -392,6 +395,10 @@ template <typename T> ScanPlan scan_plan(int64_t rows, int64_t cols, int64_t seq
     // a narrow matrix leaves lanes of its last strip without columns: single elements waste fewer
     if (cols % (32 * vec) != 0)
         p.vec = 1;
+    // Below 1024 rows a sequence two passes gain little or nothing.  One sequence, two passes against one: of 512 rows (in
+    // blocks of 128) 19.7 and 16.6 us at 1024 columns bf16; of 1024 rows 19.5 and 27, 31 and 29 at 8192 columns; of 2048
+    // rows 20 and 52, 44 and 52.  As many blocks as make three CTAs for an SM, what fits there: 16384 x 4096 bf16 takes
+    // 166 us with two, 136 with three, 134 with six; 4096 x 4096 takes 52, 41 and 52.
     const int64_t want = sms * 3 / fewest, most = rows / seqs / 256;
     p.blocks = (int)(want < most ? want : most);
     return p;
