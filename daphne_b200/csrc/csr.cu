@@ -581,7 +581,7 @@ int csr_settle(const db2_matrix *m) {
         {
             std::lock_guard<std::mutex> lock(waiting_mu);
             for (db2_csr *c : waiting)
-                if (c->lazy_rhs == m || (m->dev && c->lazy_rhs->dev == m->dev))
+                if (!c->dev_valid && (c->lazy_rhs == m || (m->dev && c->lazy_rhs->dev == m->dev)))
                     next = c;
         }
         if (!next)
