@@ -749,16 +749,43 @@ DeviceOperand::DeviceOperand(db2_matrix *m) {
     ld = m->dev_ld;
 }
 
+// whether two matrices have elements in common, as far as their placements on the device tell
+static bool overlap(const db2_matrix *a, const db2_matrix *b) {
+    if (!a || !b || !a->dev || a->dev != b->dev || a->rows * a->cols == 0 || b->rows * b->cols == 0)
+        return false;
+    const int64_t a_end = a->dev_off + (a->rows - 1) * a->dev_ld + a->cols, b_end = b->dev_off + (b->rows - 1) * b->dev_ld + b->cols;
+    if (a_end <= b->dev_off || b_end <= a->dev_off)
+        return false;
+    const int64_t ld = a->dev_ld;
+    if (a->esize() != b->esize() || ld != b->dev_ld || ld <= 0)
+        return true;
+    const int64_t ca = a->dev_off % ld, cb = b->dev_off % ld; // views of one matrix: their columns may lie side by side
+    return ca + a->cols > ld || cb + b->cols > ld || (ca < cb + b->cols && cb < ca + a->cols);
+}
 int Results::add(const char *what, db2_matrix **slot, int dtype, int64_t rows, int64_t cols) {
     if (!slot)
         return DB2_OK;
     for (int i = 0; i < n; i++)
-        DB2_CHECK(slot != slots[i] && (!*slot || *slot != *slots[i]), DB2_EINVAL, "%s: two results are to go to one matrix",
-                  what);
+        DB2_CHECK(slot != slots[i] && (!*slot || (*slot != *slots[i] && !(*slots[i] && (*slot)->is_view && (*slots[i])->is_view &&
+                                                                         overlap(*slot, *slots[i])))),
+                  DB2_EINVAL, "%s: two results are to go to one matrix", what);
     if (*slot)
         DB2_TRY(check_result(*slot, dtype, rows, cols));
     slots[n] = slot;
     fresh[n++] = !*slot;
+    return DB2_OK;
+}
+int Results::apart(const char *what, const db2_matrix *m, std::initializer_list<db2_matrix **> may_be) const {
+    for (int i = 0; i < n; i++) {
+        const db2_matrix *r = *slots[i];
+        if (!r || !r->is_view || !overlap(r, m))
+            continue;
+        bool same = false;
+        for (db2_matrix **s : may_be)
+            same = same || (s == slots[i] && r->dtype == m->dtype && r->rows == m->rows && r->cols == m->cols &&
+                            r->dev_off == m->dev_off && (r->dev_ld == m->dev_ld || r->rows <= 1));
+        DB2_CHECK(same, DB2_EINVAL, "%s: a result is a view that overlaps an operand", what);
+    }
     return DB2_OK;
 }
 Results::~Results() {
@@ -908,6 +935,7 @@ int db2_embed(db2_context *ctx, db2_matrix **res, db2_matrix *table, db2_matrix 
     const DeviceOperand dt(table), di(tokens);
     Results results;
     DB2_TRY(results.add("embed", res, table->dtype, tokens->rows, table->cols));
+    DB2_TRY(results.apart("embed", table));
     DB2_TRY(prepare_result(ctx, res, table->dtype, tokens->rows, table->cols));
     DB2_TRY(clear_status(ctx));
     DB2_TRY(db2k_embed(table->dtype, dt.ptr, table->rows, table->cols, dt.ld, tokens->dtype, di.ptr, di.ld, tokens->rows,
@@ -941,9 +969,12 @@ int db2_embedGrad(db2_context *ctx, db2_matrix **res, db2_matrix *grad, db2_matr
                   "embedGrad: the matrix to add to has shape (%lld x %lld) / type %d, expected (%lld x %lld) / type %d",
                   (long long)(*res)->rows, (long long)(*res)->cols, (*res)->dtype, (long long)vocab,
                   (long long)grad->cols, res_dtype);
+        DB2_TRY(results.add("embedGrad", res, res_dtype, vocab, grad->cols));
+        DB2_TRY(results.apart("embedGrad", grad));
         DB2_TRY(prepare_update(*res));
     } else {
         DB2_TRY(results.add("embedGrad", res, res_dtype, vocab, grad->cols));
+        DB2_TRY(results.apart("embedGrad", grad));
         DB2_TRY(prepare_result(ctx, res, res_dtype, vocab, grad->cols));
     }
     const size_t sb = db2k_embed_grad_scratch_bytes(grad->dtype, vocab, grad->cols, grad->rows);

@@ -669,6 +669,9 @@ int db2_gatedScan(db2_context *ctx, int gate, db2_matrix **h, db2_matrix **last,
     const uint64_t before = g_launches.load();
     const DeviceOperand dg(g), dx(x), doff(offsets), dh0(h0);
     DB2_CHECK(!offsets || doff.ld == 1 || seqs == 0, DB2_EUNSUPPORTED, "gatedScan: offsets are a strided view");
+    DB2_TRY(results.apart("gatedScan", g, {h}));
+    DB2_TRY(results.apart("gatedScan", x, {h}));
+    DB2_TRY(results.apart("gatedScan", h0, {last}));
     DB2_TRY(prepare_rows(ctx, h, g, !offsets));
     if (last)
         DB2_TRY(prepare_result(ctx, last, wide_dtype(g->dtype), seqs, g->cols));
@@ -706,6 +709,8 @@ int db2_gatedScanGrad(db2_context *ctx, int gate, db2_matrix **dg, db2_matrix **
     const uint64_t before = g_launches.load();
     const DeviceOperand og(g), ox(x), oh(h), od(grad), ooff(offsets), oh0(h0), ol(grad_last);
     DB2_CHECK(!offsets || ooff.ld == 1 || seqs == 0, DB2_EUNSUPPORTED, "gatedScanGrad: offsets are a strided view");
+    for (const db2_matrix *m : {g, gate == DB2_GATE_SIGMOID ? x : nullptr, h, grad, h0, grad_last})
+        DB2_TRY(results.apart("gatedScanGrad", m));
     DB2_TRY(prepare_rows(ctx, dg, g, !offsets));
     DB2_TRY(prepare_rows(ctx, dx, g, !offsets));
     if (dh0)
@@ -738,6 +743,9 @@ int db2_gatedStep(db2_context *ctx, int gate, db2_matrix **h, db2_matrix **new_s
     // a new state in the place of the old one is written where it is: each element is read before it is written
     const bool in_place = *new_state == state;
     const DeviceOperand dg(g), dx(x);
+    DB2_TRY(ensure_device(state));
+    for (const db2_matrix *m : {g, x, state}) // an element of each is read before the results' are written
+        DB2_TRY(results.apart("gatedStep", m, {h, new_state}));
     if (in_place)
         DB2_TRY(prepare_update(state));
     const DeviceOperand ds(state); // before any result is prepared, which may name it

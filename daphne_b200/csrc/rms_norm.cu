@@ -783,6 +783,9 @@ int norm_on_handles(db2_context *ctx, const char *what, db2_matrix **res, db2_ma
     DB2_TRY(results.add(what, sum, x->dtype, x->rows, x->cols));
     DB2_TRY(results.add(what, rstd, wide_dtype(x->dtype), x->rows, 1));
     const DeviceOperand dx(x), dres(residual), dw(weight);
+    DB2_TRY(results.apart(what, x, {res, sum}));
+    DB2_TRY(results.apart(what, residual, {res, sum}));
+    DB2_TRY(results.apart(what, weight));
     // (a buffer that others read as well is replaced)
     DB2_CHECK(!rstd || !*rstd || x->rows <= 1 || !(*rstd)->dev || (*rstd)->dev_ld == 1 ||
                   (!(*rstd)->is_view && (*rstd)->dev.use_count() > 1),
@@ -955,6 +958,10 @@ int db2_rmsNormGrad(db2_context *ctx, db2_matrix **dx, db2_matrix **dweight, db2
     Results results;
     DB2_TRY(results.add("rmsNormGrad", dx, grad->dtype, grad->rows, grad->cols));
     DB2_TRY(results.add("rmsNormGrad", dweight, wide_dtype(grad->dtype), 1, grad->cols));
+    for (const db2_matrix *m : {grad, sum, dsum})
+        DB2_TRY(results.apart("rmsNormGrad", m, {dx}));
+    for (const db2_matrix *m : {weight, rstd})
+        DB2_TRY(results.apart("rmsNormGrad", m));
     DB2_TRY(prepare_result(ctx, dx, grad->dtype, grad->rows, grad->cols));
     if (dweight)
         DB2_TRY(prepare_result(ctx, dweight, wide_dtype(grad->dtype), 1, grad->cols));

@@ -293,6 +293,9 @@ class Results {
   public:
     // the slot of a result that is not wanted is null
     int add(const char *what, db2_matrix **slot, int dtype, int64_t rows, int64_t cols);
+    // a result that is a view is written where it lies: it must not overlap the operand, which is on the device (those
+    // of `may_be` may be the very same elements)
+    int apart(const char *what, const db2_matrix *operand, std::initializer_list<db2_matrix **> may_be = {}) const;
     int done() {
         is_done = true;
         return DB2_OK;

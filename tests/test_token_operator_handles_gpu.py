@@ -272,3 +272,60 @@ def test_operands_that_are_deferred_and_results_that_name_them(ctx):
                 got = run(slots, x, y)
                 assert all(np.array_equal(p, q) for p, q in zip(exp, got)), (name, i, which)
                 assert np.array_equal(keep[0].to_numpy(), 2 * a + 1) and np.array_equal(keep[1].to_numpy(), 2 * b + 1), (name, i, which)
+
+
+@gpu
+def test_results_in_views_that_overlap_operands_are_refused(ctx):
+    """A view is written where it lies.  Over the very elements of an operand that is allowed where the operator allows it;
+    anything else that an operand or another result would share is refused, and nothing is written."""
+    import daphne_b200.kernels as k
+    rng = np.random.default_rng(6)
+    p = rng.integers(-4, 5, (60, 20)).astype(np.float64)
+    d, s, ref = int(k.Gate.DECAY), ctx.handle, C.byref
+    M = lambda a: k.DenseMatrix.from_numpy(ctx, a)  # noqa: E731
+    tok = M(rng.integers(0, 10, (10, 1)))
+    slot = lambda m: C.c_void_p(m.handle.value)  # noqa: E731
+    other = [M(rng.standard_normal((10, 8))) for _ in range(4)]
+    v, st, w = M(np.ones((10, 1))), M(np.zeros((1, 8))), M(np.ones((1, 8)))
+    o0, o1, o2, o3 = (m.handle for m in other)
+
+    def calls(a):  # a: the operand; results by name, and whether they may be the operand itself
+        z = a.handle
+        return {
+            "embed": lambda r: lib.db2_embed(s, ref(r), z, tok.handle, 1.0),
+            "embedGrad": lambda r: lib.db2_embedGrad(s, ref(r), z, tok.handle, 10, 1.0, 0, 0),
+            "embedGrad, added": lambda r: lib.db2_embedGrad(s, ref(r), z, tok.handle, 10, 1.0, 0, 1),
+            "rmsNorm": lambda r: lib.db2_rmsNorm(s, ref(r), None, None, z, None, w.handle, 1e-6),
+            "rmsNorm, sum": lambda r: lib.db2_rmsNorm(s, ref(C.c_void_p()), ref(r), None, o0, z, w.handle, 1e-6),
+            "rmsNormGrad": lambda r: lib.db2_rmsNormGrad(s, ref(r), None, o0, z, w.handle, v.handle, None),
+            "gatedScan": lambda r: lib.db2_gatedScan(s, d, ref(r), None, o0, z, None, None),
+            "gatedScanGrad": lambda r: lib.db2_gatedScanGrad(s, d, ref(r), ref(C.c_void_p()), None, o0, None, z, o1, None, None, None),
+            "gatedScanGrad, dx": lambda r: lib.db2_gatedScanGrad(s, d, ref(C.c_void_p()), ref(r), None, z, None, o2, o1, None, None, None),
+            "gatedStep": lambda r: lib.db2_gatedStep(s, d, ref(r), ref(C.c_void_p()), z, o0, o1),
+            "gatedStep, state": lambda r: lib.db2_gatedStep(s, d, ref(C.c_void_p()), ref(r), o0, z, r),
+        }
+    itself = {"rmsNorm", "rmsNorm, sum", "rmsNormGrad", "gatedScan", "gatedStep", "gatedStep, state"}
+    for name in calls(other[0]):
+        for rows, cols in ((0, 0), (3, 0), (0, 4), (9, 7), (5, -3), (10, 0), (0, 8), (40, 2)):
+            P = M(p)
+            P.device_ptr()
+            a = k.sliceCol(k.sliceRow(P, 10, 20), 5, 13)
+            r0, c0 = 10 + rows, 5 + cols
+            r = k.sliceCol(k.sliceRow(P, r0, r0 + 10), c0, min(c0 + 8, 20)) if c0 + 8 <= 20 else None
+            if r is None:
+                continue
+            apart = abs(rows) >= 10 or abs(cols) >= 8
+            rc = calls(a)[name](slot(r))
+            same = rows == 0 and cols == 0
+            assert rc == (0 if apart or (same and name in itself) else 1), (name, rows, cols, rc)
+            now = P.to_numpy()
+            if rc:
+                assert np.array_equal(now, p), (name, rows, cols)
+            now[r0:r0 + 10, c0:c0 + 8] = p[r0:r0 + 10, c0:c0 + 8]
+            assert np.array_equal(now, p), (name, rows, cols)
+    P = M(p)
+    P.device_ptr()
+    a, b = k.sliceRow(P, 0, 10), k.sliceRow(P, 9, 19)
+    g = M(rng.standard_normal((10, 20)))
+    assert lib.db2_gatedStep(s, d, ref(slot(a)), ref(slot(b)), g.handle, g.handle, g.handle) == 1
+    assert lib.db2_gatedStep(s, d, ref(slot(a)), ref(slot(k.sliceRow(P, 10, 20))), g.handle, g.handle, g.handle) == 0
