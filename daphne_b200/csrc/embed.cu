@@ -796,10 +796,11 @@ Results::~Results() {
         }
 }
 
-int prepare_update(db2_matrix *m) {
+int prepare_update(db2_matrix *m, bool lent) {
     DB2_TRY(ensure_device(m));
-    DB2_TRY(lazy_settle(m));
-    if (!m->is_view && m->dev.use_count() > 1) {
+    const bool stays = m->is_view || (lent && !m->dev->owned);
+    DB2_TRY(lazy_settle(m, stays));
+    if (!stays && m->dev.use_count() > 1) {
         // other handles read the buffer: the update goes to a copy
         auto fresh = make_devbuf(m->ctx, (size_t)m->rows * m->cols * m->esize());
         if (m->rows * m->cols > 0)
@@ -971,7 +972,7 @@ int db2_embedGrad(db2_context *ctx, db2_matrix **res, db2_matrix *grad, db2_matr
                   (long long)grad->cols, res_dtype);
         DB2_TRY(results.add("embedGrad", res, res_dtype, vocab, grad->cols));
         DB2_TRY(results.apart("embedGrad", grad));
-        DB2_TRY(prepare_update(*res));
+        DB2_TRY(prepare_update(*res, (*res)->dev != grad->dev)); // (its own operand is read before it is added to)
     } else {
         DB2_TRY(results.add("embedGrad", res, res_dtype, vocab, grad->cols));
         DB2_TRY(results.apart("embedGrad", grad));

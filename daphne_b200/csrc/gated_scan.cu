@@ -747,7 +747,7 @@ int db2_gatedStep(db2_context *ctx, int gate, db2_matrix **h, db2_matrix **new_s
     for (const db2_matrix *m : {g, x, state}) // an element of each is read before the results' are written
         DB2_TRY(results.apart("gatedStep", m, {h, new_state}));
     if (in_place)
-        DB2_TRY(prepare_update(state));
+        DB2_TRY(prepare_update(state, true));
     const DeviceOperand ds(state); // before any result is prepared, which may name it
     DB2_TRY(prepare_result(ctx, h, g->dtype, g->rows, g->cols));
     if (!in_place)

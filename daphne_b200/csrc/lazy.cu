@@ -549,10 +549,10 @@ static bool reads(const Expr &e, const DevBuf *b) {
     return false;
 }
 
-int lazy_settle(db2_matrix *m) {
+int lazy_settle(db2_matrix *m, bool stays) {
     DB2_TRY(csr_settle(m));
-    // (chains hold buffers: a matrix that is no view moves to another buffer instead)
-    if (!m->is_view || !m->dev || m->dev.use_count() == 1)
+    // (chains hold buffers: a matrix that does not stay in its one moves to another instead)
+    if (!stays || !m->dev || m->dev.use_count() == 1)
         return DB2_OK;
     db2_context *ctx = m->ctx;
     const DevBuf *b = m->dev.get();

@@ -264,8 +264,9 @@ int lazy_try_agg_all_start(db2_context *ctx, int op, double *pinned, db2_matrix 
 int lazy_force(db2_matrix *m);          // materialises a deferred matrix (and the pending siblings it can serve)
 int lazy_flush_all(db2_context *ctx);   // produces every pending aggregation
 void lazy_forget(db2_matrix *m);        // a deferred matrix is being destroyed
-// m is about to be updated in place: what has been asked for before and would still read its old values is computed now
-int lazy_settle(db2_matrix *m);
+// m is about to be updated: what has been asked for before and would still read its old values is computed now.  `stays`: its
+// buffer is the one that is written, whoever else holds it
+int lazy_settle(db2_matrix *m, bool stays);
 int csr_settle(const db2_matrix *m); // the same for deferred products of CSR matrices with m (csr.cu)
 
 // device groups (comm.cu): NCCL communicators for the contexts of one process, grouped all-reduce
@@ -310,8 +311,9 @@ class Results {
     int n = 0;
     bool is_done = false;
 };
-// makes m the target of an update in place: current on the device, in a buffer that no other handle reads (embed.cu)
-int prepare_update(db2_matrix *m);
+// makes m the target of an update in place: current on the device, in a buffer that no other handle reads (embed.cu).  Views
+// stay where they lie, and so does, with `lent`, a caller's device memory.
+int prepare_update(db2_matrix *m, bool lent = false);
 } // namespace db2
 
 #define DB2_API_BEGIN try {

@@ -499,7 +499,9 @@ int db2_castObj(db2_context *ctx, db2_matrix **res, db2_matrix *arg, int dtype);
  * Of these operators as a whole: a call that is refused for the shape, type or slot of a result leaves all results as they
  * were, and a call that fails leaves no matrix in a slot that held none.  A result may name an operand: it gets a buffer of its
  * own.  A result that is a view is written where it lies: over the very elements of an operand where the db2k_ form allows
- * that, any other overlap with an operand or another result is DB2_EINVAL. */
+ * that, any other overlap with an operand or another result is DB2_EINVAL.  The state of gatedStep and the matrix that
+ * embedGrad adds to, where they wrap device memory of the caller, are updated there.  What was asked for before such an
+ * update and is still deferred keeps the values of that time. */
 int db2_embed(db2_context *ctx, db2_matrix **res, db2_matrix *table, db2_matrix *tokens, double scale);
 int db2_embedGrad(db2_context *ctx, db2_matrix **res, db2_matrix *grad, db2_matrix *tokens, int64_t vocab, double scale,
                   int res_dtype, int accumulate);

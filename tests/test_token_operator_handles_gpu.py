@@ -329,3 +329,60 @@ def test_results_in_views_that_overlap_operands_are_refused(ctx):
     g = M(rng.standard_normal((10, 20)))
     assert lib.db2_gatedStep(s, d, ref(slot(a)), ref(slot(b)), g.handle, g.handle, g.handle) == 1
     assert lib.db2_gatedStep(s, d, ref(slot(a)), ref(slot(k.sliceRow(P, 10, 20))), g.handle, g.handle, g.handle) == 0
+
+
+@gpu
+@pytest.mark.parametrize("update", ["step", "table gradient"])
+@pytest.mark.parametrize("reader", ["none", "chain", "view", "sparse product"])
+def test_updates_of_memory_that_a_caller_lent(ctx, update, reader):
+    """A matrix that wraps a caller's device memory is updated there, whoever else reads it; what was asked for before keeps the
+    values of that time."""
+    import daphne_b200.kernels as k
+    import torch
+    rng = np.random.default_rng(8)
+    p, g, x = (rng.integers(-4, 5, SHAPE).astype(np.float64) for _ in range(3))
+    t = torch.as_tensor(p).cuda()
+    torch.cuda.synchronize()
+    P = k.DenseMatrix.wrap_device(ctx, t.data_ptr(), *SHAPE, SHAPE[1], np.float64, keep=t)
+    M = lambda a: k.DenseMatrix.from_numpy(ctx, a)  # noqa: E731
+    got, exp = None, 2 * p
+    if reader == "chain":
+        got = k.ewBinaryObjSca(k.BinaryOpCode.MUL, P, 2.0)
+    elif reader == "view":
+        got = k.sliceRow(P, 3, 7)
+    elif reader == "sparse product":
+        n = SHAPE[0]
+        G = k.CSRMatrix.from_arrays(ctx, n, SHAPE[1], np.full(n, 2.0), np.zeros(n, dtype=np.uint64), np.arange(n + 1, dtype=np.uint64))
+        got = k.ewMulCsrDense(G, P)
+    if update == "step":
+        k.gatedStep(k.Gate.DECAY, M(g), M(x), P)
+        new = g * p + x
+    else:
+        tok, dy = rng.integers(0, SHAPE[0], (40, 1)), rng.integers(-4, 5, (40, SHAPE[1])).astype(np.float64)
+        k.embedGrad(M(dy), M(tok), SHAPE[0], add_to=P)
+        new = p.copy()
+        np.add.at(new, tok[:, 0], dy)
+    ctx.sync()
+    assert np.array_equal(t.cpu().numpy(), new) and np.array_equal(P.to_numpy(), new)
+    if reader == "chain":
+        assert np.array_equal(got.to_numpy(), exp)
+    elif reader == "view":
+        assert np.array_equal(got.to_numpy(), new[3:7])
+    elif reader == "sparse product":
+        assert np.array_equal(k.aggRowCsr(k.AggOpCode.SUM, got).to_numpy()[:, 0], exp[:, 0])
+
+
+@gpu
+def test_a_table_gradient_added_to_its_own_operand(ctx):
+    """The rows are read before they are added to, also where the memory is a caller's: the matrix then moves."""
+    import daphne_b200.kernels as k
+    import torch
+    rng = np.random.default_rng(9)
+    p, tok = rng.integers(-4, 5, (50, 30)).astype(np.float64), rng.integers(0, 50, (50, 1))
+    exp = p.copy()
+    np.add.at(exp, tok[:, 0], p)
+    t = torch.as_tensor(p).cuda()
+    torch.cuda.synchronize()
+    for P in (k.DenseMatrix.from_numpy(ctx, p), k.DenseMatrix.wrap_device(ctx, t.data_ptr(), 50, 30, 30, np.float64, keep=t)):
+        k.embedGrad(P, k.DenseMatrix.from_numpy(ctx, tok), 50, add_to=P)
+        assert np.array_equal(P.to_numpy(), exp)
